@@ -7,7 +7,7 @@ missing or cannot be loaded, every entry point raises.
 from __future__ import annotations
 
 import ctypes
-from ctypes import POINTER, c_char_p, c_int32, c_int64, c_void_p
+from ctypes import POINTER, c_char_p, c_double, c_int32, c_int64, c_void_p
 from pathlib import Path
 from typing import Iterable, Sequence
 
@@ -17,14 +17,14 @@ LIB_PATH = PKG / "libeinsum_ir_b200.so"
 # ---- enums (values of include/eir_cuda.h)
 SUCCESS = 0
 DIM_C, DIM_M, DIM_N, DIM_K, DIM_CPX = 0, 1, 2, 3, 4
-FP32, FP64, BF16 = 0, 1, 2
+FP32, FP64, BF16, INT8 = 0, 1, 2, 3
 COMPUTE_DEFAULT, COMPUTE_FP32, COMPUTE_TF32, COMPUTE_FP64, COMPUTE_BF16 = 0, 1, 2, 3, 4
 KTYPE_ZERO, KTYPE_RELU, KTYPE_ADD, KTYPE_COPY, KTYPE_MADD, KTYPE_UNDEFINED = 0, 1, 2, 3, 4, 99
 KTYPE_CPX_ZERO, KTYPE_CPX_MADD = 6, 8
-FAMILY_NONE, FAMILY_SIMT, FAMILY_TC, FAMILY_PERMUTE, FAMILY_DMMA = 0, 1, 2, 3, 4
+FAMILY_NONE, FAMILY_SIMT, FAMILY_TC, FAMILY_PERMUTE, FAMILY_DMMA, FAMILY_ROW = 0, 1, 2, 3, 4, 5
 FLAG_FORCE_SIMT, FLAG_NO_PREPACK = 1, 2
 
-# every symbol include/eir_cuda.h declares (checked by the CPU test suite)
+# every symbol the headers under include/ declare (checked by the CPU test suite)
 EXPORTS = [
     "eir_contract_plan_create", "eir_contract", "eir_contract_num_ops",
     "eir_permute_plan_create", "eir_permute", "eir_plan_destroy", "eir_plan_kernel_family",
@@ -39,6 +39,10 @@ EXPORTS = [
     # include/eir_tensor_operation.h
     "eir_top_create", "eir_top_destroy", "eir_top_setup", "eir_top_execute", "eir_top_plan",
     "eir_top_default_optimization_config", "eir_top_optimize",
+    # include/eir_operators.h
+    "eir_norm_plan_create", "eir_norm", "eir_norm_backward", "eir_quantize_plan_create",
+    "eir_quantize", "eir_contract_int8_plan_create", "eir_contract_int8", "eir_logprob_plan_create",
+    "eir_logprob", "eir_logprob_backward",
 ]
 
 
@@ -54,6 +58,30 @@ class EirContractDesc(ctypes.Structure):
                 ("ktype_first_touch", c_int32), ("ktype_main", c_int32),
                 ("ktype_last_touch", c_int32), ("flags", c_int32), ("pad_", c_int32),
                 ("dims", POINTER(EirDim))]
+
+
+class EirNormDesc(ctypes.Structure):
+    _fields_ = [("rows", c_int64), ("cols", c_int64), ("dtype", c_int32), ("dtype_weight", c_int32),
+                ("dtype_out", c_int32), ("dtype_grad", c_int32), ("eps", c_double),
+                ("stride_x", c_int64), ("stride_residual", c_int64), ("stride_sum", c_int64),
+                ("stride_out", c_int64), ("stride_h", c_int64), ("stride_dy", c_int64),
+                ("stride_dsum", c_int64), ("stride_dx", c_int64)]
+
+
+class EirQuantizeDesc(ctypes.Structure):
+    _fields_ = [("rows", c_int64), ("cols", c_int64), ("dtype", c_int32), ("pad_", c_int32),
+                ("stride_x", c_int64), ("stride_out", c_int64)]
+
+
+class EirContractInt8Desc(ctypes.Structure):
+    _fields_ = [("m", c_int64), ("n", c_int64), ("k", c_int64), ("dtype_out", c_int32),
+                ("activation", c_int32), ("stride_left", c_int64), ("stride_right", c_int64),
+                ("stride_out", c_int64)]
+
+
+class EirLogprobDesc(ctypes.Structure):
+    _fields_ = [("rows", c_int64), ("vocab", c_int64), ("dtype", c_int32), ("top", c_int32),
+                ("stride_logits", c_int64), ("stride_dlogits", c_int64)]
 
 
 class EirError(RuntimeError):
@@ -120,6 +148,16 @@ def lib() -> ctypes.CDLL:
         L.eir_launch_count.restype = c_int64
         L.eir_plan_profile.argtypes = [c_void_p, c_int32]
         L.eir_plan_profile_read.argtypes = [c_void_p, POINTER(ctypes.c_double), POINTER(c_int64)]
+        L.eir_norm_plan_create.argtypes = [POINTER(EirNormDesc), POINTER(c_void_p)]
+        L.eir_norm.argtypes = [c_void_p] * 9
+        L.eir_norm_backward.argtypes = [c_void_p] * 9
+        L.eir_quantize_plan_create.argtypes = [POINTER(EirQuantizeDesc), POINTER(c_void_p)]
+        L.eir_quantize.argtypes = [c_void_p] * 5
+        L.eir_contract_int8_plan_create.argtypes = [POINTER(EirContractInt8Desc), POINTER(c_void_p)]
+        L.eir_contract_int8.argtypes = [c_void_p] * 8
+        L.eir_logprob_plan_create.argtypes = [POINTER(EirLogprobDesc), POINTER(c_void_p)]
+        L.eir_logprob.argtypes = [c_void_p] * 9
+        L.eir_logprob_backward.argtypes = [c_void_p] * 9
         if hasattr(L, "eir_expression_create"):
             L.eir_expression_create.argtypes = [c_char_p, c_char_p, c_char_p, c_int32, c_int32,
                                                  POINTER(c_void_p)]

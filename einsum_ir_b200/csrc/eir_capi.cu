@@ -30,6 +30,7 @@
 #include "eir_plan.h"
 
 using eir::LDim;
+using eir::ProfScope;
 
 namespace {
 
@@ -791,32 +792,6 @@ void plan_gather(eir_plan *p) {
   }
 }
 
-// events around a plan's main kernel when profiling is enabled
-struct ProfScope {
-  eir_plan *p;
-  cudaStream_t st;
-  cudaEvent_t e1 = nullptr;
-  ProfScope(eir_plan *plan, cudaStream_t s) : p(plan), st(s) {
-    if (!p->profile) return;
-    if (p->prof_used == p->prof_events.size()) {
-      cudaEvent_t a, b;
-      if (cudaEventCreate(&a) != cudaSuccess) return;
-      if (cudaEventCreate(&b) != cudaSuccess) {
-        cudaEventDestroy(a);
-        return;
-      }
-      p->prof_events.emplace_back(a, b);
-    }
-    cudaEventRecord(p->prof_events[p->prof_used].first, st);
-    e1 = p->prof_events[p->prof_used].second;
-  }
-  ~ProfScope() {
-    if (e1 == nullptr) return;
-    cudaEventRecord(e1, st);
-    p->prof_used++;
-  }
-};
-
 int run_simt(eir_plan *p, void const *l, void const *r, void const *aux, void *out,
              eir::PeerOutputs const *peers, cudaStream_t st) {
   ProfScope prof(p, st);
@@ -843,6 +818,14 @@ int api_set_error(int code, char const *msg) { return set_error(code, msg); }
 int api_cuda_fail(cudaError_t e, char const *where) { return cuda_fail(e, where); }
 int api_encode_map(MapSpec const &s, void const *ptr, CUtensorMap *m) { return encode_map(s, ptr, m); }
 void api_count_launch() { g_launches.fetch_add(1, std::memory_order_relaxed); }
+int api_device(int *num_sms, uint32_t **err) {
+  DeviceState *ds = nullptr;
+  int rc = device_state(&ds);
+  if (rc != EIR_SUCCESS) return rc;
+  *num_sms = ds->num_sms;
+  *err = ds->err;
+  return EIR_SUCCESS;
+}
 int api_launch_tc_split(eir_plan const *p, CUtensorMap const &ma, CUtensorMap const &mb,
                         TcParams const &tp, void const *aux, void *out, float *ws, int num_sms,
                         cudaStream_t st) {

@@ -1,0 +1,336 @@
+// C-ABI of the row operators and the 8-bit contraction (eir_operators.h):
+// argument checks, workspaces and launches.
+#include <algorithm>
+#include <cstdio>
+#include <new>
+#include <string>
+#include "eir_operators.h"
+#include "eir_plan.h"
+
+namespace {
+
+using eir::ProfScope;
+
+enum { kWhatNorm = 3, kWhatQuantize = 4, kWhatInt8 = 5, kWhatLogprob = 6 };
+
+int fail(int code, char const *msg) { return eir::api_set_error(code, msg); }
+int bad_argument(char const *msg) { return fail(EIR_INVALID_ARGUMENT, msg); }
+int null_pointer(char const *msg) { return fail(EIR_NO_DATA_PTR_PROVIDED, msg); }
+
+bool is_float(int dt) { return dt == EIR_FP32 || dt == EIR_BF16; }
+char const *type_text(int dt) { return dt == EIR_FP32 ? "fp32" : dt == EIR_BF16 ? "bf16" : "int8"; }
+int64_t type_bytes(int dt) { return dt == EIR_FP32 ? 4 : dt == EIR_BF16 ? 2 : 1; }
+
+// rows x cols within the range of the kernels' 64-bit offsets and 31-bit grids
+bool sizes_ok(int64_t rows, int64_t cols) {
+  return rows >= 0 && rows <= INT32_MAX && cols >= 1 && cols <= INT32_MAX;
+}
+bool stride_in_ok(int64_t s) { return s >= 0 && s < ((int64_t)1 << 40); }
+bool stride_out_ok(int64_t s, int64_t cols, int64_t rows) {
+  return stride_in_ok(s) && (rows <= 1 || s >= cols);
+}
+bool aligned(void const *p, int64_t bytes) { return reinterpret_cast<uintptr_t>(p) % (uintptr_t)bytes == 0; }
+
+// the plan object, or null when memory is out (no exception leaves the C entry)
+template <typename Fill>
+int make_plan(eir_plan **out, int what, int family, Fill fill) {
+  eir_plan *p = nullptr;
+  try {
+    p = new eir_plan();
+    p->what = what;
+    p->family = family;
+    fill(p);
+  } catch (std::exception const &) {
+    delete p;
+    return fail(EIR_UNDEFINED_ERROR, "out of host memory");
+  }
+  *out = p;
+  return EIR_SUCCESS;
+}
+
+// the plan's own workspace on the current device, allocated on first use
+int workspace(eir_plan *p, void **ws) {
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return eir::api_cuda_fail(e, "cudaGetDevice");
+  if (p->ws == nullptr || p->ws_device != dev) {
+    if (p->ws != nullptr) cudaFree(p->ws);
+    e = cudaMalloc(&p->ws, (size_t)p->ws_bytes);
+    if (e != cudaSuccess) {
+      p->ws = nullptr;
+      return eir::api_cuda_fail(e, "cudaMalloc(workspace)");
+    }
+    p->ws_device = dev;
+  }
+  *ws = p->ws;
+  return EIR_SUCCESS;
+}
+
+int launched(cudaError_t e, char const *where) {
+  if (e != cudaSuccess) return eir::api_cuda_fail(e, where);
+  eir::api_count_launch();
+  return EIR_SUCCESS;
+}
+
+}  // namespace
+
+extern "C" {
+
+// ---------------------------------------------------------------- norm
+
+int eir_norm_plan_create(eir_norm_desc const *d, eir_plan **out) {
+  if (d == nullptr || out == nullptr) return bad_argument("null descriptor or plan pointer");
+  if (!sizes_ok(d->rows, d->cols)) return bad_argument("norm: rows must be 0 .. 2^31 - 1 and cols 1 .. 2^31 - 1");
+  if (!is_float(d->dtype) || !is_float(d->dtype_weight) || !is_float(d->dtype_grad) ||
+      !(is_float(d->dtype_out) || d->dtype_out == EIR_INT8))
+    return fail(EIR_INVALID_DTYPE, "norm: FP32 or BF16 data (dtype_out: INT8 too)");
+  if (!(d->eps >= 0.0) || d->eps > 3.0e38) return bad_argument("norm: eps must be a finite number >= 0");
+  for (int64_t s : {d->stride_x, d->stride_residual, d->stride_h, d->stride_dy, d->stride_dsum})
+    if (!stride_in_ok(s)) return bad_argument("norm: an input's row stride must be >= 0");
+  for (int64_t s : {d->stride_sum, d->stride_out, d->stride_dx})
+    if (!stride_out_ok(s, d->cols, d->rows)) return bad_argument("norm: an output's row stride must be >= cols");
+  return make_plan(out, kWhatNorm, EIR_FAMILY_ROW, [&](eir_plan *p) {
+    eir::NormParams &n = p->norm;
+    n.rows = d->rows;
+    n.cols = d->cols;
+    n.dt = d->dtype;
+    n.dt_w = d->dtype_weight;
+    n.dt_out = d->dtype_out;
+    n.dt_grad = d->dtype_grad;
+    n.eps = (float)d->eps;
+    n.s_x = d->stride_x;
+    n.s_res = d->stride_residual;
+    n.s_sum = d->stride_sum;
+    n.s_out = d->stride_out;
+    n.s_h = d->stride_h;
+    n.s_dy = d->stride_dy;
+    n.s_dsum = d->stride_dsum;
+    n.s_dx = d->stride_dx;
+    p->empty = d->rows == 0;
+    // partial rows of the weight gradient: at most one per CTA of the backward kernel
+    p->ws_bytes = eir::norm_backward_ctas(n, eir::kMaxSms) * d->cols * 4;
+    p->text = std::string("norm ") + type_text(n.dt) + " -> " + type_text(n.dt_out) + " rows=" +
+              std::to_string(n.rows) + " cols=" + std::to_string(n.cols);
+  });
+}
+
+int eir_norm(eir_plan *p, void const *x, void const *residual, void const *weight, void *sum, void *out,
+             float *scale, float *rstd, void *stream) {
+  if (p == nullptr || p->what != kWhatNorm) return bad_argument("not a norm plan");
+  if (p->empty) return EIR_SUCCESS;
+  eir::NormParams const &n = p->norm;
+  if (x == nullptr || out == nullptr) return null_pointer("norm: null x or out");
+  if (n.dt_out == EIR_INT8 && scale == nullptr) return null_pointer("norm: INT8 output needs scale");
+  const int64_t e = type_bytes(n.dt);
+  if (!aligned(x, e) || !aligned(residual, e) || !aligned(sum, e) || !aligned(weight, type_bytes(n.dt_w)) ||
+      !aligned(out, type_bytes(n.dt_out)) || !aligned(scale, 4) || !aligned(rstd, 4))
+    return bad_argument("norm: a pointer is not aligned to its element");
+  int num_sms = 0;
+  uint32_t *err = nullptr;
+  int rc = eir::api_device(&num_sms, &err);
+  if (rc != EIR_SUCCESS) return rc;
+  const eir::NormPtrs a{x, residual, weight, sum, out, scale, rstd};
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  ProfScope prof(p, st);
+  return launched(eir::launch_norm(n, a, num_sms, st), "norm launch");
+}
+
+int eir_norm_backward(eir_plan *p, void const *dy, void const *h, void const *weight, float const *rstd,
+                      void const *dsum, void *dx, float *dweight, void *stream) {
+  if (p == nullptr || p->what != kWhatNorm) return bad_argument("not a norm plan");
+  eir::NormParams const &n = p->norm;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if (!aligned(dweight, 4)) return bad_argument("norm backward: a pointer is not aligned to its element");
+  if (p->empty) {  // a sum over no rows
+    if (dweight == nullptr) return EIR_SUCCESS;
+    cudaError_t e = cudaMemsetAsync(dweight, 0, (size_t)n.cols * 4, st);
+    return e == cudaSuccess ? EIR_SUCCESS : eir::api_cuda_fail(e, "cudaMemsetAsync(dweight)");
+  }
+  if (dy == nullptr || h == nullptr || rstd == nullptr || dx == nullptr)
+    return null_pointer("norm backward: null dy, h, rstd or dx");
+  const int64_t e = type_bytes(n.dt), g = type_bytes(n.dt_grad);
+  if (!aligned(h, e) || !aligned(dy, g) || !aligned(dsum, g) || !aligned(dx, g) || !aligned(rstd, 4) ||
+      !aligned(weight, type_bytes(n.dt_w)))
+    return bad_argument("norm backward: a pointer is not aligned to its element");
+  int num_sms = 0;
+  uint32_t *err = nullptr;
+  int rc = eir::api_device(&num_sms, &err);
+  if (rc != EIR_SUCCESS) return rc;
+  num_sms = std::min(num_sms, eir::kMaxSms);
+  eir::NormGradPtrs a{dy, h, weight, dsum, rstd, dx, dweight, nullptr};
+  const int64_t ctas = eir::norm_backward_ctas(n, num_sms);
+  if (dweight != nullptr) {
+    void *ws = nullptr;
+    rc = workspace(p, &ws);
+    if (rc != EIR_SUCCESS) return rc;
+    a.part = static_cast<float *>(ws);
+  }
+  {
+    ProfScope prof(p, st);
+    rc = launched(eir::launch_norm_backward(n, a, num_sms, st), "norm backward launch");
+  }
+  if (rc != EIR_SUCCESS || dweight == nullptr) return rc;
+  return launched(eir::launch_norm_dweight(n, a.part, ctas, dweight, st), "norm weight gradient launch");
+}
+
+// ---------------------------------------------------------------- quantize
+
+int eir_quantize_plan_create(eir_quantize_desc const *d, eir_plan **out) {
+  if (d == nullptr || out == nullptr) return bad_argument("null descriptor or plan pointer");
+  if (!sizes_ok(d->rows, d->cols))
+    return bad_argument("quantize: rows must be 0 .. 2^31 - 1 and cols 1 .. 2^31 - 1");
+  if (!is_float(d->dtype)) return fail(EIR_INVALID_DTYPE, "quantize: FP32 or BF16 data");
+  if (!stride_in_ok(d->stride_x)) return bad_argument("quantize: the input's row stride must be >= 0");
+  if (!stride_out_ok(d->stride_out, d->cols, d->rows))
+    return bad_argument("quantize: the output's row stride must be >= cols");
+  return make_plan(out, kWhatQuantize, EIR_FAMILY_ROW, [&](eir_plan *p) {
+    p->quant.rows = d->rows;
+    p->quant.cols = d->cols;
+    p->quant.dt = d->dtype;
+    p->quant.s_x = d->stride_x;
+    p->quant.s_out = d->stride_out;
+    p->empty = d->rows == 0;
+    p->text = std::string("quantize ") + type_text(d->dtype) + " rows=" + std::to_string(d->rows) +
+              " cols=" + std::to_string(d->cols);
+  });
+}
+
+int eir_quantize(eir_plan *p, void const *x, void *q, float *scale, void *stream) {
+  if (p == nullptr || p->what != kWhatQuantize) return bad_argument("not a quantize plan");
+  if (p->empty) return EIR_SUCCESS;
+  if (x == nullptr || q == nullptr || scale == nullptr) return null_pointer("quantize: null x, q or scale");
+  if (!aligned(x, type_bytes(p->quant.dt)) || !aligned(scale, 4))
+    return bad_argument("quantize: a pointer is not aligned to its element");
+  int num_sms = 0;
+  uint32_t *err = nullptr;
+  int rc = eir::api_device(&num_sms, &err);
+  if (rc != EIR_SUCCESS) return rc;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  ProfScope prof(p, st);
+  return launched(eir::launch_quantize(p->quant, x, static_cast<int8_t *>(q), scale, num_sms, st),
+                  "quantize launch");
+}
+
+// ---------------------------------------------------------------- 8-bit contraction
+
+int eir_contract_int8_plan_create(eir_contract_int8_desc const *d, eir_plan **out) {
+  if (d == nullptr || out == nullptr) return bad_argument("null descriptor or plan pointer");
+  if (d->m < 0 || d->n < 0 || d->k < 0 || d->m > INT32_MAX || d->n > INT32_MAX)
+    return bad_argument("8-bit contraction: m, n must be 0 .. 2^31 - 1");
+  if (d->k > 131071) return bad_argument("8-bit contraction: k must be at most 131071 (32-bit sums)");
+  if (!is_float(d->dtype_out)) return fail(EIR_INVALID_DTYPE, "8-bit contraction: dtype_out FP32 or BF16");
+  if (d->activation < EIR_ACT_NONE || d->activation > EIR_ACT_GATED_SILU)
+    return fail(EIR_INVALID_KTYPE, "8-bit contraction: unknown activation");
+  const bool gated = d->activation == EIR_ACT_GATED_SILU;
+  if (gated && d->n % 2 != 0) return bad_argument("8-bit contraction: gated SiLU needs an even n");
+  if (!stride_in_ok(d->stride_left) || !stride_in_ok(d->stride_right))
+    return bad_argument("8-bit contraction: an input's row stride must be >= 0");
+  const int64_t n_out = gated ? d->n / 2 : d->n;
+  if (!stride_out_ok(d->stride_out, n_out, d->m))
+    return bad_argument("8-bit contraction: the output's row stride must be >= its columns");
+  return make_plan(out, kWhatInt8, EIR_FAMILY_SIMT, [&](eir_plan *p) {
+    eir::I8Params &q = p->i8;
+    q.m = d->m;
+    q.n = d->n;
+    q.k = d->k;
+    q.dt_out = d->dtype_out;
+    q.act = d->activation;
+    q.s_l = d->stride_left;
+    q.s_r = d->stride_right;
+    q.s_out = d->stride_out;
+    p->empty = d->m == 0 || n_out == 0;
+    p->text = std::string("int8 simt m=") + std::to_string(d->m) + " n=" + std::to_string(d->n) +
+              " k=" + std::to_string(d->k);
+  });
+}
+
+int eir_contract_int8(eir_plan *p, void const *left, void const *right, float const *scale_left,
+                      float const *scale_right, float const *bias, void *out, void *stream) {
+  if (p == nullptr || p->what != kWhatInt8) return bad_argument("not an 8-bit contraction plan");
+  if (p->empty) return EIR_SUCCESS;
+  if (out == nullptr || (p->i8.k > 0 && (left == nullptr || right == nullptr)))
+    return null_pointer("8-bit contraction: null operand pointer");
+  if (!aligned(scale_left, 4) || !aligned(scale_right, 4) || !aligned(bias, 4) ||
+      !aligned(out, type_bytes(p->i8.dt_out)))
+    return bad_argument("8-bit contraction: a pointer is not aligned to its element");
+  const eir::I8Ptrs a{static_cast<int8_t const *>(left), static_cast<int8_t const *>(right),
+                      scale_left, scale_right, bias, out};
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  ProfScope prof(p, st);
+  return launched(eir::launch_i8_simt(p->i8, a, st), "8-bit contraction launch");
+}
+
+// ---------------------------------------------------------------- log probabilities
+
+int eir_logprob_plan_create(eir_logprob_desc const *d, eir_plan **out) {
+  if (d == nullptr || out == nullptr) return bad_argument("null descriptor or plan pointer");
+  if (!sizes_ok(d->rows, d->vocab))
+    return bad_argument("logprob: rows must be 0 .. 2^31 - 1 and vocab 1 .. 2^31 - 1");
+  if (!is_float(d->dtype)) return fail(EIR_INVALID_DTYPE, "logprob: FP32 or BF16 logits");
+  if (d->top < 0 || d->top > 32 || d->top > d->vocab)
+    return bad_argument("logprob: top must be 0 .. min(32, vocab)");
+  if (!stride_in_ok(d->stride_logits)) return bad_argument("logprob: the logits' row stride must be >= 0");
+  if (!stride_out_ok(d->stride_dlogits, d->vocab, d->rows))
+    return bad_argument("logprob: the gradient's row stride must be >= vocab");
+  return make_plan(out, kWhatLogprob, EIR_FAMILY_ROW, [&](eir_plan *p) {
+    eir::LogprobParams &l = p->logprob;
+    l.rows = d->rows;
+    l.vocab = d->vocab;
+    l.dt = d->dtype;
+    l.top = d->top;
+    l.s_x = d->stride_logits;
+    l.s_dx = d->stride_dlogits;
+    p->empty = d->rows == 0;
+    p->text = std::string("logprob ") + type_text(l.dt) + " rows=" + std::to_string(l.rows) +
+              " vocab=" + std::to_string(l.vocab) + " top=" + std::to_string(l.top);
+  });
+}
+
+int eir_logprob(eir_plan *p, void const *logits, int64_t const *targets, float *logprob, float *entropy,
+                float *lse, float *top_logprob, int64_t *top_index, void *stream) {
+  if (p == nullptr || p->what != kWhatLogprob) return bad_argument("not a log-probability plan");
+  if (p->empty) return EIR_SUCCESS;
+  if (logits == nullptr) return null_pointer("logprob: null logits");
+  if ((targets == nullptr) != (logprob == nullptr))
+    return null_pointer("logprob: targets and logprob go together");
+  if (!aligned(logits, type_bytes(p->logprob.dt)) || !aligned(targets, 8) || !aligned(top_index, 8) ||
+      !aligned(logprob, 4) || !aligned(entropy, 4) || !aligned(lse, 4) || !aligned(top_logprob, 4))
+    return bad_argument("logprob: a pointer is not aligned to its element");
+  int num_sms = 0;
+  uint32_t *err = nullptr;
+  int rc = eir::api_device(&num_sms, &err);
+  if (rc != EIR_SUCCESS) return rc;
+  eir::LogprobParams q = p->logprob;
+  if (top_logprob == nullptr && top_index == nullptr) q.top = 0;
+  const eir::LogprobPtrs a{logits, targets, logprob, entropy, lse, top_logprob, top_index};
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  ProfScope prof(p, st);
+  return launched(eir::launch_logprob(q, a, num_sms, st), "logprob launch");
+}
+
+int eir_logprob_backward(eir_plan *p, void const *logits, int64_t const *targets, float const *lse,
+                         float const *entropy, float const *dlogprob, float const *dentropy, void *dlogits,
+                         void *stream) {
+  if (p == nullptr || p->what != kWhatLogprob) return bad_argument("not a log-probability plan");
+  if (p->empty) return EIR_SUCCESS;
+  if (logits == nullptr || lse == nullptr || dlogits == nullptr)
+    return null_pointer("logprob backward: null logits, lse or dlogits");
+  if ((targets == nullptr) != (dlogprob == nullptr))
+    return null_pointer("logprob backward: targets and dlogprob go together");
+  if (dentropy != nullptr && entropy == nullptr)
+    return null_pointer("logprob backward: dentropy needs entropy");
+  const int64_t e = type_bytes(p->logprob.dt);
+  if (!aligned(logits, e) || !aligned(dlogits, e) || !aligned(targets, 8) || !aligned(lse, 4) ||
+      !aligned(entropy, 4) || !aligned(dlogprob, 4) || !aligned(dentropy, 4))
+    return bad_argument("logprob backward: a pointer is not aligned to its element");
+  int num_sms = 0;
+  uint32_t *err = nullptr;
+  int rc = eir::api_device(&num_sms, &err);
+  if (rc != EIR_SUCCESS) return rc;
+  const eir::LogprobGradPtrs a{logits, targets, lse, entropy, dlogprob, dentropy, dlogits};
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  ProfScope prof(p, st);
+  return launched(eir::launch_logprob_backward(p->logprob, a, num_sms, st), "logprob backward launch");
+}
+
+}  // extern "C"

@@ -9,6 +9,7 @@
 #include <vector>
 #include "eir_params.h"
 #include "eir_cuda.h"
+#include "op_params.h"
 
 namespace eir {
 
@@ -39,6 +40,8 @@ int api_set_error(int code, char const *msg);
 int api_cuda_fail(cudaError_t e, char const *where);
 int api_encode_map(MapSpec const &s, void const *ptr, CUtensorMap *m);
 void api_count_launch();
+// the current device's SM count and error word (allocated on first use)
+int api_device(int *num_sms, uint32_t **err);
 
 }  // namespace eir
 
@@ -69,7 +72,8 @@ int api_launch_tc_split(eir_plan const *p, CUtensorMap const &ma, CUtensorMap co
 }  // namespace eir
 
 struct eir_plan {
-  int what = 0;  // 1 = contraction, 2 = permute
+  // 1 = contraction, 2 = permute, 3 = norm, 4 = quantize, 5 = 8-bit contraction, 6 = log probabilities
+  int what = 0;
   int family = EIR_FAMILY_NONE;
   int64_t num_ops = 0;
   std::string text;
@@ -132,8 +136,42 @@ struct eir_plan {
   bool unary_zero = false;
   int esize = 4;
 
+  // ---- row operators and the 8-bit contraction (eir_operators.h)
+  eir::NormParams norm;
+  eir::QuantizeParams quant;
+  eir::I8Params i8;
+  eir::LogprobParams logprob;
+
   // ---- main-kernel timing (eir_plan_profile)
   bool profile = false;
   std::vector<std::pair<cudaEvent_t, cudaEvent_t>> prof_events;
   size_t prof_used = 0;
 };
+
+namespace eir {
+// events around a plan's main kernel when profiling is enabled
+struct ProfScope {
+  eir_plan *p;
+  cudaStream_t st;
+  cudaEvent_t e1 = nullptr;
+  ProfScope(eir_plan *plan, cudaStream_t s) : p(plan), st(s) {
+    if (!p->profile) return;
+    if (p->prof_used == p->prof_events.size()) {
+      cudaEvent_t a, b;
+      if (cudaEventCreate(&a) != cudaSuccess) return;
+      if (cudaEventCreate(&b) != cudaSuccess) {
+        cudaEventDestroy(a);
+        return;
+      }
+      p->prof_events.emplace_back(a, b);
+    }
+    cudaEventRecord(p->prof_events[p->prof_used].first, st);
+    e1 = p->prof_events[p->prof_used].second;
+  }
+  ~ProfScope() {
+    if (e1 == nullptr) return;
+    cudaEventRecord(e1, st);
+    p->prof_used++;
+  }
+};
+}  // namespace eir

@@ -1,0 +1,89 @@
+// Device helpers shared by the row operators and the 8-bit contraction.
+#pragma once
+
+#include <cstdint>
+#include <cuda_runtime.h>
+#include <cuda_bf16.h>
+#include "eir_cuda.h"
+#include "eir_operators.h"
+
+namespace eir {
+
+// below this row maximum (2^-100) 127 / m nears the end of the FP32 range: the
+// row counts as zeros
+constexpr float kQuantMin = 7.888609052210118e-31f;
+
+__device__ __forceinline__ float to_f32(float v) { return v; }
+__device__ __forceinline__ float to_f32(__nv_bfloat16 v) { return __bfloat162float(v); }
+template <typename T>
+__device__ __forceinline__ T from_f32(float v);
+template <>
+__device__ __forceinline__ float from_f32<float>(float v) { return v; }
+template <>
+__device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
+
+// one value of a tensor whose type is a run-time choice
+__device__ __forceinline__ float ld_any(void const *p, int dt, int64_t i) {
+  return dt == EIR_FP32 ? static_cast<float const *>(p)[i]
+                        : __bfloat162float(static_cast<__nv_bfloat16 const *>(p)[i]);
+}
+__device__ __forceinline__ void st_any(void *p, int dt, int64_t i, float v) {
+  if (dt == EIR_FP32) static_cast<float *>(p)[i] = v;
+  else static_cast<__nv_bfloat16 *>(p)[i] = __float2bfloat16_rn(v);
+}
+
+__device__ __forceinline__ float warp_sum(float v) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  return v;
+}
+
+// |v| as bits: the order of non-negative floats, with NaNs above infinity, so
+// that an integer maximum carries a NaN through
+__device__ __forceinline__ uint32_t abs_bits(float v) { return __float_as_uint(v) & 0x7fffffffu; }
+
+// sum of v and maximum of m over the block; every thread gets both. `red`: 2 x 32 words
+template <int WARPS>
+__device__ __forceinline__ void block_sum_max(float &v, uint32_t &m, uint32_t *red) {
+  v = warp_sum(v);
+  m = __reduce_max_sync(0xffffffffu, m);
+  if (WARPS == 1) return;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  __syncthreads();  // `red` may hold an earlier result
+  if (lane == 0) {
+    red[warp] = __float_as_uint(v);
+    red[32 + warp] = m;
+  }
+  __syncthreads();
+  float s = 0.f;
+  uint32_t t = 0;
+  if (lane < WARPS) {
+    s = __uint_as_float(red[lane]);
+    t = red[32 + lane];
+  }
+  v = warp_sum(s);
+  m = __reduce_max_sync(0xffffffffu, t);
+}
+
+// A row's 8-bit scaling from the bits of its largest magnitude: the factor
+// 127 / m of round(v * factor), and the scale m * unit / 127 of the integers.
+struct QuantScale {
+  float inv, scale;
+  bool finite;
+};
+__device__ __forceinline__ QuantScale quant_scale(uint32_t max_bits, float unit) {
+  QuantScale q;
+  const float m = __uint_as_float(max_bits);
+  q.finite = max_bits < 0x7f800000u;
+  const bool some = q.finite && m >= kQuantMin;
+  q.inv = some ? __fdiv_rn(127.f, m) : 0.f;
+  q.scale = q.finite ? (some ? __fdiv_rn(__fmul_rn(m, unit), 127.f) : 0.f) : __uint_as_float(0x7fc00000u);
+  return q;
+}
+// v in 8 bits (|v| <= m, so |v * 127 / m| rounds to 127 at most); a row with
+// an infinity or NaN is all zeros, and its scale says so
+__device__ __forceinline__ int quant_one(float v, QuantScale const &q) {
+  return q.finite ? __float2int_rn(__fmul_rn(v, q.inv)) : 0;
+}
+
+}  // namespace eir

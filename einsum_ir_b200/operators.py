@@ -1,0 +1,130 @@
+"""The row operators and the 8-bit contraction (include/eir_operators.h).
+
+``NormPlan`` (root-mean-square norm with the residual's addition, float or
+8-bit output, and its backward pass), ``QuantizePlan`` (rows to 8-bit integers
+with a scale a row), ``Int8ContractPlan`` (8-bit contraction with a scale for
+each token and channel) and ``LogprobPlan`` (log probabilities of given tokens,
+entropy, top alternatives, and their backward pass). As in ``cabi``, sizes,
+types and strides are the plan's; a call takes device pointers or tensors,
+writes into the caller's outputs and is asynchronous on ``stream``. Row strides
+are in elements and default to packed rows.
+"""
+from __future__ import annotations
+
+import ctypes
+from ctypes import c_void_p
+
+from . import cabi
+from .cabi import BF16, FP32, INT8, check
+
+ACT_NONE, ACT_RELU, ACT_GATED_SILU = 0, 1, 2
+
+__all__ = ["ACT_NONE", "ACT_RELU", "ACT_GATED_SILU", "FP32", "BF16", "INT8", "NormPlan", "QuantizePlan",
+           "Int8ContractPlan", "LogprobPlan"]
+
+
+def _ptr(x):
+    """device address of a tensor, an address, or None"""
+    if x is None or isinstance(x, int):
+        return x
+    return x.data_ptr()
+
+
+def _packed(stride, cols):
+    return cols if stride is None else stride
+
+
+class _OpPlan(cabi.Plan):
+    def __init__(self, create, desc):
+        h = c_void_p()
+        check(create(ctypes.byref(desc), ctypes.byref(h)))
+        super().__init__(h)
+
+
+class NormPlan(_OpPlan):
+    """h = x + residual; y = h * rstd * weight with rstd = (mean(h^2) + eps)^(-1/2)
+    over rows of ``cols`` elements. ``dtype``: x, residual, sum and h;
+    ``dtype_out``: y, FP32, BF16 or INT8 (default: dtype); ``dtype_grad``: dy, dsum and
+    dx (default: dtype)."""
+
+    def __init__(self, rows, cols, dtype, dtype_weight=None, dtype_out=None, dtype_grad=None, eps=1e-6,
+                 stride_x=None, stride_residual=None, stride_sum=None, stride_out=None, stride_h=None,
+                 stride_dy=None, stride_dsum=None, stride_dx=None):
+        pick = lambda t: dtype if t is None else t
+        sx = _packed(stride_x, cols)
+        super().__init__(cabi.lib().eir_norm_plan_create, cabi.EirNormDesc(
+            rows, cols, dtype, pick(dtype_weight), pick(dtype_out), pick(dtype_grad), eps, sx,
+            _packed(stride_residual, cols), _packed(stride_sum, cols), _packed(stride_out, cols),
+            sx if stride_h is None else stride_h, _packed(stride_dy, cols), _packed(stride_dsum, cols),
+            _packed(stride_dx, cols)))
+        self._norm = cabi.lib().eir_norm
+        self._backward = cabi.lib().eir_norm_backward
+
+    def norm(self, x, out, weight=None, residual=None, sum=None, scale=None, rstd=None, stream: int = 0) -> None:
+        """out = y, or with INT8 output its integers (``scale``: FP32 [rows]);
+        sum = h and rstd (FP32 [rows]) are what the backward pass reads."""
+        check(self._norm(self._h, _ptr(x), _ptr(residual), _ptr(weight), _ptr(sum), _ptr(out), _ptr(scale),
+                         _ptr(rstd), stream))
+
+    def backward(self, dy, h, rstd, dx, weight=None, dsum=None, dweight=None, stream: int = 0) -> None:
+        """dx: the gradient of x and of residual from dy and dsum (the
+        gradient that reaches h past the norm); dweight: FP32 [cols]. ``h``
+        is the forward call's sum, or its x where it had no residual; its rows
+        are ``stride_h`` apart (default: stride_x)."""
+        check(self._backward(self._h, _ptr(dy), _ptr(h), _ptr(weight), _ptr(rstd), _ptr(dsum), _ptr(dx),
+                             _ptr(dweight), stream))
+
+
+class QuantizePlan(_OpPlan):
+    """Rows to 8-bit integers: q = round(x * 127 / max|x|), scale = max|x| / 127."""
+
+    def __init__(self, rows, cols, dtype, stride_x=None, stride_out=None):
+        super().__init__(cabi.lib().eir_quantize_plan_create, cabi.EirQuantizeDesc(
+            rows, cols, dtype, 0, _packed(stride_x, cols), _packed(stride_out, cols)))
+        self._quantize = cabi.lib().eir_quantize
+
+    def quantize(self, x, q, scale, stream: int = 0) -> None:
+        check(self._quantize(self._h, _ptr(x), _ptr(q), _ptr(scale), stream))
+
+
+class Int8ContractPlan(_OpPlan):
+    """out[t, c] = act(sum_k left[t, k] right[c, k] * scale_left[t] * scale_right[c] + bias[c])
+    for int8 ``left`` [m, k] (tokens) and ``right`` [n, k] (channels). ACT_GATED_SILU: out
+    [m, n / 2] = silu(first half of the channels) * second half."""
+
+    def __init__(self, m, n, k, dtype_out=BF16, activation=ACT_NONE, stride_left=None, stride_right=None,
+                 stride_out=None):
+        n_out = n // 2 if activation == ACT_GATED_SILU else n
+        super().__init__(cabi.lib().eir_contract_int8_plan_create, cabi.EirContractInt8Desc(
+            m, n, k, dtype_out, activation, _packed(stride_left, k), _packed(stride_right, k),
+            _packed(stride_out, n_out)))
+        self._contract = cabi.lib().eir_contract_int8
+
+    def contract(self, left, right, scale_left, scale_right, out, bias=None, stream: int = 0) -> None:
+        """scale_left FP32 [m], scale_right FP32 [n] (None: ones), bias FP32 [n] or None"""
+        check(self._contract(self._h, _ptr(left), _ptr(right), _ptr(scale_left), _ptr(scale_right), _ptr(bias),
+                             _ptr(out), stream))
+
+
+class LogprobPlan(_OpPlan):
+    """Log probabilities of given tokens over rows of ``vocab`` logits, with
+    log-sum-exp, entropy and the ``top`` most likely tokens (ties: lowest index)."""
+
+    def __init__(self, rows, vocab, dtype, top=0, stride_logits=None, stride_dlogits=None):
+        super().__init__(cabi.lib().eir_logprob_plan_create, cabi.EirLogprobDesc(
+            rows, vocab, dtype, top, _packed(stride_logits, vocab), _packed(stride_dlogits, vocab)))
+        self._logprob = cabi.lib().eir_logprob
+        self._backward = cabi.lib().eir_logprob_backward
+
+    def logprob(self, logits, targets=None, logprob=None, entropy=None, lse=None, top_logprob=None,
+                top_index=None, stream: int = 0) -> None:
+        """targets int64 [rows] (negative: ignored); logprob, entropy, lse FP32
+        [rows]; top_logprob FP32 and top_index int64 [rows, top]"""
+        check(self._logprob(self._h, _ptr(logits), _ptr(targets), _ptr(logprob), _ptr(entropy), _ptr(lse),
+                            _ptr(top_logprob), _ptr(top_index), stream))
+
+    def backward(self, logits, targets, lse, dlogprob, dlogits, entropy=None, dentropy=None,
+                 stream: int = 0) -> None:
+        """dlogits from the gradients of logprob and entropy"""
+        check(self._backward(self._h, _ptr(logits), _ptr(targets), _ptr(lse), _ptr(entropy), _ptr(dlogprob),
+                             _ptr(dentropy), _ptr(dlogits), stream))

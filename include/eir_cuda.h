@@ -81,7 +81,8 @@ enum {
   EIR_FAMILY_SIMT      = 1, /* generic strided CUDA-core contraction */
   EIR_FAMILY_TC        = 2, /* tcgen05 + TMA tensor-core contraction */
   EIR_FAMILY_PERMUTE   = 3, /* permute kernel */
-  EIR_FAMILY_DMMA      = 4  /* FP64 tensor-core (mma.sync f64) contraction */
+  EIR_FAMILY_DMMA      = 4, /* FP64 tensor-core (mma.sync f64) contraction */
+  EIR_FAMILY_ROW       = 5  /* row operators (eir_operators.h) */
 };
 
 /* planner flags */

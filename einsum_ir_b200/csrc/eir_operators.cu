@@ -66,6 +66,52 @@ int workspace(eir_plan *p, void **ws) {
   return EIR_SUCCESS;
 }
 
+// Tiling of an 8-bit contraction on the tensor cores. Pair tiles once they
+// fill most of the GPU's 74 CTA pairs; else one-CTA tiles of just enough tokens, with
+// the K walk of each tile split over a cluster until two CTAs an SM (one for
+// the 128-token tiles, whose stages fill more shared memory) are in flight.
+eir::I8TcPlan i8_tiling(eir::I8Params const &p) {
+  const int64_t sms = 148, n_out = p.act == EIR_ACT_GATED_SILU ? p.n / 2 : p.n;
+  eir::I8TcPlan t;
+  t.c_tiles = (n_out + 255) / 256;
+  const int64_t pair_tokens = p.act == EIR_ACT_GATED_SILU ? 128 : 256;
+  t.t_tiles = (p.m + pair_tokens - 1) / pair_tokens;
+  if (t.c_tiles * t.t_tiles >= 64) return t;
+  t.tokens = p.m <= 16 ? 16 : p.m <= 32 ? 32 : p.m <= 64 ? 64 : 128;
+  t.c_tiles = (n_out + 127) / 128;
+  t.t_tiles = (p.m + t.tokens - 1) / t.tokens;
+  const int64_t k_blocks = (p.k + 127) / 128, most = t.tokens == 128 ? sms : 2 * sms;
+  while (t.split < 8 && 2 * t.split * t.c_tiles * t.t_tiles <= most && 2 * t.split <= k_blocks) t.split *= 2;
+  return t;
+}
+
+// an operand's rows as the TMA loads take them: read in place where base and
+// stride are multiples of 16 bytes, else copied into the workspace
+struct I8Operand {
+  int8_t const *ptr;
+  int64_t rows, stride;
+  bool copy;
+};
+int64_t packed_stride(int64_t k) { return (k + 15) / 16 * 16; }
+I8Operand i8_operand(void const *ptr, int64_t rows, int64_t k, int64_t stride) {
+  I8Operand o{static_cast<int8_t const *>(ptr), rows, stride, false};
+  if (rows == 1) o.stride = packed_stride(k);  // no second row: any stride will do
+  o.copy = !aligned(ptr, 16) || o.stride % 16 != 0 || o.stride < k;
+  return o;
+}
+
+int i8_map(I8Operand const &o, int64_t k, int box_rows, CUtensorMap *map) {
+  eir::MapSpec m;
+  m.rank = 2;
+  m.dims[0] = (uint64_t)k;
+  m.dims[1] = (uint64_t)o.rows;
+  m.strides_bytes[0] = (uint64_t)o.stride;
+  m.box[0] = 128;
+  m.box[1] = (uint32_t)box_rows;
+  m.dtype = CU_TENSOR_MAP_DATA_TYPE_UINT8;
+  return eir::api_encode_map(m, o.ptr, map);
+}
+
 int launched(cudaError_t e, char const *where) {
   if (e != cudaSuccess) return eir::api_cuda_fail(e, where);
   eir::api_count_launch();
@@ -239,8 +285,15 @@ int eir_contract_int8_plan_create(eir_contract_int8_desc const *d, eir_plan **ou
     q.s_r = d->stride_right;
     q.s_out = d->stride_out;
     p->empty = d->m == 0 || n_out == 0;
-    p->text = std::string("int8 simt m=") + std::to_string(d->m) + " n=" + std::to_string(d->n) +
-              " k=" + std::to_string(d->k);
+    if (d->k > 0 && !p->empty) {
+      p->family = EIR_FAMILY_TC;
+      p->i8_tc = i8_tiling(q);
+      // copies of operands that TMA cannot read in place
+      p->ws_bytes = (d->m + d->n) * packed_stride(d->k);
+    }
+    p->text = std::string("int8 ") + (p->family != EIR_FAMILY_TC ? "simt" : p->i8_tc.tokens == 0 ? "pair" : "split") +
+              " tokens=" + std::to_string(p->i8_tc.tokens) + " split=" + std::to_string(p->i8_tc.split) +
+              " m=" + std::to_string(d->m) + " n=" + std::to_string(d->n) + " k=" + std::to_string(d->k);
   });
 }
 
@@ -256,8 +309,36 @@ int eir_contract_int8(eir_plan *p, void const *left, void const *right, float co
   const eir::I8Ptrs a{static_cast<int8_t const *>(left), static_cast<int8_t const *>(right),
                       scale_left, scale_right, bias, out};
   cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if (p->family != EIR_FAMILY_TC) {
+    ProfScope prof(p, st);
+    return launched(eir::launch_i8_simt(p->i8, a, st), "8-bit contraction launch");
+  }
+  int num_sms = 0;
+  uint32_t *err = nullptr;
+  int rc = eir::api_device(&num_sms, &err);
+  if (rc != EIR_SUCCESS) return rc;
+  I8Operand ops[2] = {i8_operand(left, p->i8.m, p->i8.k, p->i8.s_l), i8_operand(right, p->i8.n, p->i8.k, p->i8.s_r)};
+  const int64_t ld = packed_stride(p->i8.k);
+  for (int i = 0; i < 2; ++i) {
+    I8Operand &o = ops[i];
+    if (!o.copy) continue;
+    void *ws = nullptr;
+    rc = workspace(p, &ws);
+    if (rc != EIR_SUCCESS) return rc;
+    int8_t *to = static_cast<int8_t *>(ws) + (i == 0 ? 0 : p->i8.m * ld);
+    rc = launched(eir::launch_i8_pack(o.rows, p->i8.k, i == 0 ? p->i8.s_l : p->i8.s_r, o.ptr, to, ld, num_sms, st),
+                  "8-bit operand copy");
+    if (rc != EIR_SUCCESS) return rc;
+    o.ptr = to;
+    o.stride = ld;
+  }
+  CUtensorMap map_t, map_c;
+  rc = i8_map(ops[0], p->i8.k, eir::i8_box_tokens(p->i8_tc, p->i8.act == EIR_ACT_GATED_SILU), &map_t);
+  if (rc != EIR_SUCCESS) return rc;
+  rc = i8_map(ops[1], p->i8.k, 128, &map_c);
+  if (rc != EIR_SUCCESS) return rc;
   ProfScope prof(p, st);
-  return launched(eir::launch_i8_simt(p->i8, a, st), "8-bit contraction launch");
+  return launched(eir::launch_i8_tc(p->i8_tc, map_c, map_t, p->i8, a, err, st), "8-bit contraction launch");
 }
 
 // ---------------------------------------------------------------- log probabilities

@@ -140,6 +140,7 @@ struct eir_plan {
   eir::NormParams norm;
   eir::QuantizeParams quant;
   eir::I8Params i8;
+  eir::I8TcPlan i8_tc;
   eir::LogprobParams logprob;
 
   // ---- main-kernel timing (eir_plan_profile)

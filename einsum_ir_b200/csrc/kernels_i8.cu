@@ -1,18 +1,9 @@
-// Contraction of 8-bit integers with a scale for each token (left row) and
-// channel (right row): acc = sum_k a b in 32-bit integers (exact, so any
-// order of the sum gives the same bits), then in FP32
-// z = acc sa sb + bias and the activation, rounded once when stored.
+// Contraction of 8-bit integers on the CUDA cores, for operands that the
+// tensor cores cannot take, and the copy that lays rows out for them.
 #include "eir_launch.h"
-#include "eir_common.cuh"
-#include "op_common.cuh"
-#include "op_params.h"
+#include "i8_common.cuh"
 
 namespace eir {
-
-__device__ __forceinline__ float i8_scaled(int32_t acc, float sa, float sb, float bias) {
-  return fmaf((float)acc, sa * sb, bias);
-}
-__device__ __forceinline__ float silu(float z) { return z / (1.f + expf(-z)); }
 
 // 64 tokens x 64 channels (gated: 32 gates and their 32 values) a CTA, K
 // staged in shared memory byte by byte in blocks of 64, so that any stride
@@ -56,6 +47,7 @@ __global__ void __launch_bounds__(256) i8_simt_kernel(const I8Params p, const I8
         for (int j = 0; j < 4; ++j) acc[i][j] = __dp4a((int)l[i], (int)r[j], acc[i][j]);
     }
   }
+  const float low = p.act == EIR_ACT_RELU ? 0.f : -INFINITY;
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     const int64_t t = t0 + ty + 16 * i;
@@ -72,7 +64,7 @@ __global__ void __launch_bounds__(256) i8_simt_kernel(const I8Params p, const I8
       if (c >= n_out) continue;
       float v = z(j);
       if (gated) v = silu(v) * z(j + 2 < 4 ? j + 2 : 3);
-      else if (p.act == EIR_ACT_RELU) v = v > 0.f ? v : (v != v ? v : 0.f);
+      else v = relu_from(v, low);
       st_any(a.out, p.dt_out, t * p.s_out + c, v);
     }
   }
@@ -85,6 +77,50 @@ cudaError_t launch_i8_simt(I8Params const &p, I8Ptrs const &a, cudaStream_t st) 
   if (tiles > INT32_MAX) return cudaErrorInvalidConfiguration;
   const dim3 grid((unsigned)tiles);
   return launch_kernel(i8_simt_kernel, grid, dim3(256), 0, st, p, a);
+}
+
+// Rows of k bytes into rows `ld` bytes apart (a multiple of 16): TMA needs
+// 16-byte strides and a 16-byte base. A thread writes 16 bytes, read as
+// aligned words shifted into place; a word that reaches outside the tensor's
+// bytes is read byte by byte.
+__global__ void __launch_bounds__(256) i8_pack_kernel(int64_t rows, int64_t k, int64_t stride,
+                                                      int8_t const *__restrict__ src, int8_t *__restrict__ dst,
+                                                      int64_t ld) {
+  pdl_launch_dependents();
+  pdl_wait();
+  const uintptr_t begin = reinterpret_cast<uintptr_t>(src);
+  const uintptr_t end = begin + (uintptr_t)((rows - 1) * stride + k);
+  const int64_t per_row = ld / 16, total = rows * per_row;
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
+    const int64_t r = i / per_row, b = (i - r * per_row) * 16;
+    const uintptr_t at = begin + (uintptr_t)(r * stride + b), base = at & ~(uintptr_t)3;
+    uint32_t w[5];
+#pragma unroll
+    for (int j = 0; j < 5; ++j) {
+      const uintptr_t q = base + 4 * j;
+      if (q >= begin && q + 4 <= end) {
+        w[j] = *reinterpret_cast<uint32_t const *>(q);
+      } else {
+        w[j] = 0;
+        for (int e = 0; e < 4; ++e)
+          if (q + e >= begin && q + e < end) w[j] |= (uint32_t) * reinterpret_cast<uint8_t const *>(q + e) << (8 * e);
+      }
+    }
+    const uint32_t sh = 8 * (uint32_t)(at & 3);
+    uint4 v;
+    v.x = __funnelshift_r(w[0], w[1], sh);
+    v.y = __funnelshift_r(w[1], w[2], sh);
+    v.z = __funnelshift_r(w[2], w[3], sh);
+    v.w = __funnelshift_r(w[3], w[4], sh);
+    *reinterpret_cast<uint4 *>(dst + r * ld + b) = v;
+  }
+}
+
+cudaError_t launch_i8_pack(int64_t rows, int64_t k, int64_t stride, int8_t const *src, int8_t *dst, int64_t ld,
+                           int num_sms, cudaStream_t st) {
+  const int64_t blocks = (rows * (ld / 16) + 255) / 256, most = (int64_t)num_sms * 8;
+  return launch_kernel(i8_pack_kernel, dim3((unsigned)(blocks < most ? blocks : most)), dim3(256), 0, st, rows, k,
+                       stride, src, dst, ld);
 }
 
 }  // namespace eir

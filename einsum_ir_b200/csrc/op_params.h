@@ -43,6 +43,13 @@ struct I8Params {
   int64_t s_l = 0, s_r = 0, s_out = 0;
 };
 
+// how the tensor-core kernels tile a contraction: token tiles of `tokens`
+// (0: the CTA-pair kernel), K split over clusters of `split` CTAs
+struct I8TcPlan {
+  int64_t c_tiles = 0, t_tiles = 0;
+  int tokens = 0, split = 1;
+};
+
 struct I8Ptrs {
   int8_t const *l, *r;
   float const *scale_l, *scale_r, *bias;
@@ -78,6 +85,13 @@ cudaError_t launch_norm_dweight(NormParams const &p, float const *part, int64_t 
 cudaError_t launch_quantize(QuantizeParams const &p, void const *x, int8_t *q, float *scale, int num_sms,
                             cudaStream_t st);
 cudaError_t launch_i8_simt(I8Params const &p, I8Ptrs const &a, cudaStream_t st);
+cudaError_t launch_i8_tc(I8TcPlan const &tp, CUtensorMap const &map_channels, CUtensorMap const &map_tokens,
+                         I8Params const &p, I8Ptrs const &a, uint32_t *err, cudaStream_t st);
+// token and channel rows of one TMA box of the tiling `tp`
+int i8_box_tokens(I8TcPlan const &tp, bool gated);
+// rows of k bytes, `stride` apart, into rows `ld` bytes apart
+cudaError_t launch_i8_pack(int64_t rows, int64_t k, int64_t stride, int8_t const *src, int8_t *dst, int64_t ld,
+                           int num_sms, cudaStream_t st);
 cudaError_t launch_logprob(LogprobParams const &p, LogprobPtrs const &a, int num_sms, cudaStream_t st);
 cudaError_t launch_logprob_backward(LogprobParams const &p, LogprobGradPtrs const &a, int num_sms,
                                     cudaStream_t st);

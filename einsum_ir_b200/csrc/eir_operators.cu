@@ -68,20 +68,18 @@ int workspace(eir_plan *p, void **ws) {
 
 // Tiling of an 8-bit contraction on the tensor cores. Pair tiles once they
 // fill most of the GPU's 74 CTA pairs; else one-CTA tiles of just enough tokens, with
-// the K walk of each tile split over a cluster until two CTAs an SM (one for
-// the 128-token tiles, whose stages fill more shared memory) are in flight.
+// the K walk of each tile split over a cluster until two CTAs an SM are in flight.
 eir::I8TcPlan i8_tiling(eir::I8Params const &p) {
-  const int64_t sms = 148, n_out = p.act == EIR_ACT_GATED_SILU ? p.n / 2 : p.n;
+  const int64_t sms = 148;
   eir::I8TcPlan t;
-  t.c_tiles = (n_out + 255) / 256;
-  const int64_t pair_tokens = p.act == EIR_ACT_GATED_SILU ? 128 : 256;
-  t.t_tiles = (p.m + pair_tokens - 1) / pair_tokens;
-  if (t.c_tiles * t.t_tiles >= 64) return t;
+  t.c_tiles = (p.n + 255) / 256;  // gated: 128 gates and their values a tile
+  t.t_tiles = (p.m + 255) / 256;
+  if (p.m > 128 && t.c_tiles * t.t_tiles >= 64) return t;
   t.tokens = p.m <= 16 ? 16 : p.m <= 32 ? 32 : p.m <= 64 ? 64 : 128;
-  t.c_tiles = (n_out + 127) / 128;
+  t.c_tiles = (p.n + 127) / 128;
   t.t_tiles = (p.m + t.tokens - 1) / t.tokens;
-  const int64_t k_blocks = (p.k + 127) / 128, most = t.tokens == 128 ? sms : 2 * sms;
-  while (t.split < 8 && 2 * t.split * t.c_tiles * t.t_tiles <= most && 2 * t.split <= k_blocks) t.split *= 2;
+  const int64_t k_blocks = (p.k + 127) / 128;
+  while (t.split < 8 && 2 * t.split * t.c_tiles * t.t_tiles <= 2 * sms && 2 * t.split <= k_blocks) t.split *= 2;
   return t;
 }
 
@@ -100,14 +98,19 @@ I8Operand i8_operand(void const *ptr, int64_t rows, int64_t k, int64_t stride) {
   return o;
 }
 
-int i8_map(I8Operand const &o, int64_t k, int box_rows, CUtensorMap *map) {
+// K rows of 128 bytes; `halves` (a gated layer's right operand): gate rows and
+// value rows as the third dim, 16 rows of each in a box
+int i8_map(I8Operand const &o, int64_t k, int box_rows, bool halves, CUtensorMap *map) {
   eir::MapSpec m;
-  m.rank = 2;
+  m.rank = halves ? 3 : 2;
   m.dims[0] = (uint64_t)k;
-  m.dims[1] = (uint64_t)o.rows;
+  m.dims[1] = (uint64_t)(halves ? o.rows / 2 : o.rows);
+  m.dims[2] = 2;
   m.strides_bytes[0] = (uint64_t)o.stride;
+  m.strides_bytes[1] = (uint64_t)(o.rows / 2 * o.stride);
   m.box[0] = 128;
-  m.box[1] = (uint32_t)box_rows;
+  m.box[1] = halves ? 16 : (uint32_t)box_rows;
+  m.box[2] = halves ? 2 : 1;
   m.dtype = CU_TENSOR_MAP_DATA_TYPE_UINT8;
   return eir::api_encode_map(m, o.ptr, map);
 }
@@ -333,9 +336,9 @@ int eir_contract_int8(eir_plan *p, void const *left, void const *right, float co
     o.stride = ld;
   }
   CUtensorMap map_t, map_c;
-  rc = i8_map(ops[0], p->i8.k, eir::i8_box_tokens(p->i8_tc, p->i8.act == EIR_ACT_GATED_SILU), &map_t);
+  rc = i8_map(ops[0], p->i8.k, eir::i8_box_tokens(p->i8_tc), false, &map_t);
   if (rc != EIR_SUCCESS) return rc;
-  rc = i8_map(ops[1], p->i8.k, 128, &map_c);
+  rc = i8_map(ops[1], p->i8.k, 128, p->i8.act == EIR_ACT_GATED_SILU, &map_c);
   if (rc != EIR_SUCCESS) return rc;
   ProfScope prof(p, st);
   return launched(eir::launch_i8_tc(p->i8_tc, map_c, map_t, p->i8, a, err, st), "8-bit contraction launch");

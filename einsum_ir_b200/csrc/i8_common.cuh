@@ -12,9 +12,30 @@ namespace eir {
 __device__ __forceinline__ float i8_scaled(int32_t acc, float sa, float sb, float bias) {
   return fmaf((float)acc, sa * sb, bias);
 }
-__device__ __forceinline__ float silu(float z) { return z / (1.f + expf(-z)); }
+// two of them in packed FP32 arithmetic (the same roundings)
+__device__ __forceinline__ float2 scaled2(int32_t a0, int32_t a1, float2 sa, float sb, float bias) {
+  float2 z;
+  asm("{\n\t.reg .b64 s, b, a, f, r;\n\t"
+      "mov.b64 s, {%4, %5};\n\t"
+      "mov.b64 b, {%6, %6};\n\t"
+      "mul.rn.f32x2 f, s, b;\n\t"
+      "mov.b64 a, {%2, %3};\n\t"
+      "mov.b64 b, {%7, %7};\n\t"
+      "fma.rn.f32x2 r, a, f, b;\n\t"
+      "mov.b64 {%0, %1}, r;\n\t}"
+      : "=f"(z.x), "=f"(z.y)
+      : "f"((float)a0), "f"((float)a1), "f"(sa.x), "f"(sa.y), "f"(sb), "f"(bias));
+  return z;
+}
+// silu(z) = z / (1 + e^-z) with the hardware's exponential and reciprocal: off
+// by about (|z| + 4) 2^-24 of itself, under the rounding of the sum that gave z
+__device__ __forceinline__ float silu(float z) { return __fdividef(z, 1.f + __expf(-z)); }
 // ReLU that keeps a NaN; `low` = 0, or -infinity for no activation
-__device__ __forceinline__ float relu_from(float z, float low) { return z < low ? low : z; }
+__device__ __forceinline__ float relu_from(float z, float low) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(z), "f"(low));
+  return r;
+}
 
 // 2-D tiled TMA load global -> shared, completion on an mbarrier (no multicast)
 __device__ __forceinline__ void tma_load_2d(void *dst, void const *map, uint64_t *bar, int c0, int c1) {
@@ -31,6 +52,22 @@ __device__ __forceinline__ void tma_load_2d_pair(void *dst, void const *map, uin
       "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes"
       " [%0], [%1, {%3, %4}], [%2];" ::"r"(smem_u32(dst)),
       "l"(map), "r"(bar_cluster), "r"(c0), "r"(c1)
+      : "memory");
+}
+
+__device__ __forceinline__ void tma_load_3d(void *dst, void const *map, uint64_t *bar, int c0, int c1, int c2) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes"
+      " [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(smem_u32(dst)),
+      "l"(map), "r"(smem_u32(bar)), "r"(c0), "r"(c1), "r"(c2)
+      : "memory");
+}
+__device__ __forceinline__ void tma_load_3d_pair(void *dst, void const *map, uint32_t bar_cluster, int c0, int c1,
+                                                 int c2) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes"
+      " [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(smem_u32(dst)),
+      "l"(map), "r"(bar_cluster), "r"(c0), "r"(c1), "r"(c2)
       : "memory");
 }
 
@@ -67,31 +104,6 @@ __device__ __forceinline__ void tmem_ld_32x32b_x16(uint32_t taddr, uint32_t (&v)
         "=r"(v[7]), "=r"(v[8]), "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]),
         "=r"(v[14]), "=r"(v[15])
       : "r"(taddr));
-}
-
-// The channel side of the epilogue, held by the thread that owns the channel:
-// its scale and bias (gated: the gate's and the value's)
-struct I8Channel {
-  float sb, bias, sb2, bias2;
-};
-__device__ __forceinline__ I8Channel i8_channel(I8Params const &p, I8Ptrs const &a, int64_t c, int64_t n_out,
-                                                bool gated) {
-  I8Channel h{1.f, 0.f, 1.f, 0.f};
-  if (c >= n_out) return h;
-  if (a.scale_r) h.sb = a.scale_r[c];
-  if (a.bias) h.bias = a.bias[c];
-  if (gated) {
-    if (a.scale_r) h.sb2 = a.scale_r[c + n_out];
-    if (a.bias) h.bias2 = a.bias[c + n_out];
-  }
-  return h;
-}
-// one output value from its accumulator(s)
-template <bool GATED>
-__device__ __forceinline__ float i8_value(int32_t acc, int32_t acc2, float sa, I8Channel const &h, float low) {
-  const float z = i8_scaled(acc, sa, h.sb, h.bias);
-  if (GATED) return silu(z) * i8_scaled(acc2, sa, h.sb2, h.bias2);
-  return relu_from(z, low);
 }
 
 }  // namespace eir

@@ -4,17 +4,18 @@
 // in any order; the epilogue scales, adds the bias and applies the activation
 // in FP32 and rounds once. The channels (right rows) are the MMA's M side and
 // the tokens its N side: an epilogue thread then owns one channel (its scale
-// and bias stay in registers), a warp stores 32 neighbouring channels of a
-// token at a time, and a single token is an MMA of N = 16 that costs nothing
-// beside the weights' bytes. A gated layer stages a tile of gate rows and the
-// tile of their value rows and keeps two accumulators, so that no output but the
-// activated product is written.
+// and bias stay in registers), a warp stores neighbouring channels of a token
+// together, and a single token is an MMA of N = 16 that costs nothing beside
+// the weights' bytes. A gated layer interleaves 16 gate rows and their 16 value
+// rows in the staged tile (one box of a 3-D tensor map), so that lanes l and
+// l + 16 of a warp hold a gate and its value: one shuffle joins them, the MMAs are
+// those of a plain layer, and only the activated product is written.
 //
 // Two kernels:
-// * i8_pair_kernel: CTA pairs (cta_group::2) over tiles of 256 channels x 256
-//   tokens (gated: 256 + 256 channels x 128 tokens), persistent, accumulators
-//   double-buffered in TMEM so that the epilogue runs under the next tile.
-// * i8_split_kernel: one tile of 128 channels x NT tokens (NT = 16 .. 128) for
+// * i8_pair_kernel: CTA pairs (cta_group::2) over tiles of 256 rows x 256
+//   tokens, persistent, accumulators double-buffered in TMEM so that the
+//   epilogue runs under the next tile.
+// * i8_split_kernel: one tile of 128 rows x NT tokens (NT = 16 .. 128) for
 //   problems with too few pair tiles to fill the GPU. A cluster of 1 to 8 CTAs
 //   shares the tile's K walk; each holds a partial accumulator, and the
 //   cluster adds them through distributed shared memory.
@@ -28,25 +29,127 @@
 
 namespace eir {
 
-constexpr int kI8Rows = 128;                      // channels of a CTA
-constexpr int kI8BlockK = 128;                    // K of a stage: one swizzle row
-constexpr int kI8SubBytes = kI8Rows * kI8BlockK;  // a tile of 128 rows
+constexpr int kI8Rows = 128;                      // staged right rows of a CTA
+constexpr int kI8BlockK = 128;                    // K of a block: one swizzle row
+constexpr int kI8SubBytes = kI8Rows * kI8BlockK;  // a block of 128 rows
+constexpr int kI8Chunk = 16;                      // tokens drained from TMEM at a time
+
+// output channels of a CTA's 128 rows
+template <bool GATED>
+__host__ __device__ constexpr int i8_channels() {
+  return GATED ? kI8Rows / 2 : kI8Rows;
+}
+// the output channel of tile row `row` (of a tile whose first channel is c0),
+// and whether the row is a value row
+template <bool GATED>
+__device__ __forceinline__ int64_t i8_row_channel(int64_t c0, int row) {
+  return GATED ? c0 + (row >> 5) * 16 + (row & 15) : c0 + row;
+}
+
+// one K block of the 128 right rows from channel c0 on into `dst`
+template <bool GATED, typename Load2, typename Load3>
+__device__ __forceinline__ void i8_load_rows(uint8_t *dst, int k, int c0, Load2 load2, Load3 load3) {
+  if (!GATED) {
+    load2(dst, k, c0);
+  } else {
+#pragma unroll
+    for (int b = 0; b < 4; ++b) load3(dst + b * 32 * kI8BlockK, k, c0 + 16 * b);
+  }
+}
+
+// The epilogue's row side, held by the thread that owns the tile row: its
+// channel's scale and bias
+struct I8Row {
+  float sb, bias;
+};
+template <bool GATED>
+__device__ __forceinline__ I8Row i8_row(I8Params const &p, I8Ptrs const &a, int64_t c, int row, int64_t n_out) {
+  I8Row h{1.f, 0.f};
+  if (c >= n_out) return h;
+  const int64_t r = c + (GATED && (row & 16) ? n_out : 0);
+  if (a.scale_r) h.sb = a.scale_r[r];
+  if (a.bias) h.bias = a.bias[r];
+  return h;
+}
+
+// 16 accumulators of a thread's row from TMEM, scaled: z[i] of token i
+__device__ __forceinline__ void i8_drain(uint32_t src, float const *scale, I8Row const &h, float (&z)[kI8Chunk]) {
+  uint32_t v[kI8Chunk];
+  tmem_ld_32x32b_x16(src, v);
+  tmem_ld_wait();
+#pragma unroll
+  for (int i = 0; i < kI8Chunk; i += 4) {
+    const float4 s = *reinterpret_cast<float4 const *>(scale + i);
+    const float2 z0 = scaled2((int32_t)v[i], (int32_t)v[i + 1], make_float2(s.x, s.y), h.sb, h.bias);
+    const float2 z1 = scaled2((int32_t)v[i + 2], (int32_t)v[i + 3], make_float2(s.z, s.w), h.sb, h.bias);
+    z[i] = z0.x;
+    z[i + 1] = z0.y;
+    z[i + 2] = z1.x;
+    z[i + 3] = z1.y;
+  }
+}
+
+// Stores a warp's 32 rows x 16 tokens. Gated: lanes l and l + 16 first trade
+// halves of their tokens, so that lane l holds gate and value of the even
+// tokens and lane l + 16 of the odd ones. BF16 on even rows: lanes 2j and
+// 2j + 1 then trade tokens too and store two channels in one word.
+//   out: the first token's row; c: the lane's channel; tokens: how many exist
+template <bool GATED, typename T>
+__device__ __forceinline__ void i8_store_chunk(T *out, int64_t stride, float (&z)[kI8Chunk], int64_t c, int64_t n_out,
+                                               int tokens, bool pairs, float low) {
+  constexpr int N = GATED ? kI8Chunk / 2 : kI8Chunk, STEP = GATED ? 2 : 1;  // token of w[j]: STEP j + first
+  const int lane = threadIdx.x & 31, first = GATED ? lane >> 4 : 0;
+  float w[N];
+  if (GATED) {
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+      const float got = __shfl_xor_sync(0xffffffffu, first ? z[2 * j] : z[2 * j + 1], 16);
+      w[j] = first ? silu(got) * z[2 * j + 1] : silu(z[2 * j]) * got;
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < N; ++j) w[j] = relu_from(z[j], low);
+  }
+  if (sizeof(T) == 2 && pairs && tokens == kI8Chunk) {
+    const int odd = lane & 1;
+    const uint32_t pick = odd ? 0x3276u : 0x5410u;
+    const bool two = c - odd + 1 < n_out, one = c - odd < n_out;
+    char *o = reinterpret_cast<char *>(out + (first + (odd ? STEP : 0)) * stride + c - odd);
+    const int64_t step = 4 * STEP * stride;
+#pragma unroll
+    for (int j = 0; j < N; j += 2, o += step) {
+      const __nv_bfloat162 b = __floats2bfloat162_rn(w[j], w[j + 1]);
+      const uint32_t mine = *reinterpret_cast<uint32_t const *>(&b);
+      const uint32_t both = __byte_perm(mine, __shfl_xor_sync(0xffffffffu, mine, 1), pick);
+      if (two) *reinterpret_cast<uint32_t *>(o) = both;
+      else if (one) *reinterpret_cast<uint16_t *>(o) = (uint16_t)both;
+    }
+  } else if (c < n_out) {
+    T *o = out + first * stride + c;
+#pragma unroll
+    for (int j = 0; j < N; ++j, o += STEP * stride)
+      if (STEP * j + first < tokens) *o = from_f32<T>(w[j]);
+  }
+}
+
+// two-channel stores need even rows and a base on a word
+__device__ __forceinline__ bool i8_pairs(I8Params const &p, I8Ptrs const &a) {
+  return p.s_out % 2 == 0 && (reinterpret_cast<uintptr_t>(a.out) & 3) == 0;
+}
 
 // ---------------------------------------------------------------- CTA pairs
 
-template <bool GATED>
 struct I8Pair {
-  static constexpr int kTokens = GATED ? 128 : 256;       // tokens of a tile (N of the MMA)
-  static constexpr int kABytes = kI8SubBytes * (GATED ? 2 : 1);
-  static constexpr int kBBytes = kTokens / 2 * kI8BlockK;  // each CTA stages half of the tokens
+  static constexpr int kTokens = 256;                    // tokens of a tile (N of the MMA)
+  static constexpr int kSub = 2;                         // K blocks of a stage
+  static constexpr int kBSub = kTokens / 2 * kI8BlockK;  // each CTA stages half of the tokens
+  static constexpr int kABytes = kSub * kI8SubBytes, kBBytes = kSub * kBSub;
   static constexpr int kStageBytes = kABytes + kBBytes;
   static constexpr int kStages = (232448 - 1024 - 5120) / kStageBytes;
-  static constexpr int kAccCols = kTokens * (GATED ? 2 : 1);
   static constexpr int kEpiWarps = 8;
   static constexpr int kThreads = 32 * (2 + kEpiWarps);
   static constexpr int kWarpTokens = kTokens / 2;  // columns of one epilogue warp
   static constexpr int kSmemBytes = 1024 + kStages * kStageBytes + 5120;
-  static_assert(kAccCols == 256, "two accumulators fill TMEM");
 };
 
 // pair tile -> (channel tile, token tile): bands of 8 token tiles, channels
@@ -61,10 +164,10 @@ __device__ __forceinline__ void i8_pair_tile(uint32_t t, uint32_t c_tiles, uint3
 }
 
 template <bool GATED, typename T>
-__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(I8Pair<GATED>::kThreads, 1)
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(I8Pair::kThreads, 1)
     i8_pair_kernel(const __grid_constant__ CUtensorMap map_c, const __grid_constant__ CUtensorMap map_t,
                    const I8Params p, const I8Ptrs a, uint32_t *err, uint32_t c_tiles, uint32_t t_tiles) {
-  using Cfg = I8Pair<GATED>;
+  using Cfg = I8Pair;
   constexpr int S = Cfg::kStages;
   extern __shared__ uint8_t smem_raw[];
   uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -121,19 +224,24 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(I8Pair<GATED>::kThre
       for (uint32_t t = pair_id; t < tiles && ok && !*abort_flag; t += n_pairs) {
         uint32_t ct, tt;
         i8_pair_tile(t, c_tiles, t_tiles, ct, tt);
-        const int row_c = (int)(ct * 256 + rank * kI8Rows);
+        const int c0 = (int)((2 * ct + rank) * i8_channels<GATED>());
         const int row_t = (int)(tt * Cfg::kTokens + rank * (Cfg::kTokens / 2));
-        for (int kb = 0; kb < k_blocks; ++kb) {
+        for (int kb = 0; kb < k_blocks; kb += Cfg::kSub) {
           if (!mbar_wait_bounded(&empty[stage], phase ^ 1u, abort_flag)) {
             ok = false;
             break;
           }
-          if (rank == 0) mbar_arrive_expect_tx(&full[stage], 2 * Cfg::kStageBytes);
+          const int subs = min(Cfg::kSub, k_blocks - kb);
+          if (rank == 0) mbar_arrive_expect_tx(&full[stage], 2 * subs * (kI8SubBytes + Cfg::kBSub));
           const uint32_t bar = full_leader + 8u * (uint32_t)stage;
-          uint8_t *dA = sA + stage * Cfg::kABytes;
-          tma_load_2d_pair(dA, &map_c, bar, kb * kI8BlockK, row_c);
-          if (GATED) tma_load_2d_pair(dA + kI8SubBytes, &map_c, bar, kb * kI8BlockK, row_c + (int)n_out);
-          tma_load_2d_pair(sB + stage * Cfg::kBBytes, &map_t, bar, kb * kI8BlockK, row_t);
+          for (int sub = 0; sub < subs; ++sub) {
+            const int k = (kb + sub) * kI8BlockK;
+            i8_load_rows<GATED>(
+                sA + stage * Cfg::kABytes + sub * kI8SubBytes, k, c0,
+                [&](void *dst, int x, int y) { tma_load_2d_pair(dst, &map_c, bar, x, y); },
+                [&](void *dst, int x, int y) { tma_load_3d_pair(dst, &map_c, bar, x, y, 0); });
+            tma_load_2d_pair(sB + stage * Cfg::kBBytes + sub * Cfg::kBSub, &map_t, bar, k, row_t);
+          }
           if (++stage == S) {
             stage = 0;
             phase ^= 1u;
@@ -159,35 +267,44 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(I8Pair<GATED>::kThre
       int stage = 0, acc = 0;
       uint32_t phase = 0, acc_phase = 0;
       bool ok = true;
+      // descriptors: the stage's address moves the low word only
+      const uint64_t a_desc = make_smem_desc(smem_u32(sA), 16, 1024, kLayoutSw128);
+      const uint64_t b_desc = make_smem_desc(smem_u32(sB), 16, 1024, kLayoutSw128);
+      bool ready = false;  // the stage's loads have already been seen to be complete
       for (uint32_t t = pair_id; t < tiles && ok; t += n_pairs) {
         if (!mbar_wait_bounded(&tempty[acc], acc_phase ^ 1u, abort_flag)) {
           ok = false;
           break;
         }
         tc_fence_after();
-        const uint32_t d = tmem_base + (uint32_t)(acc * Cfg::kAccCols);
-        for (int kb = 0; kb < k_blocks; ++kb) {
-          if (!mbar_wait_bounded(&full[stage], phase, abort_flag)) {
+        const uint32_t d = tmem_base + (uint32_t)(acc * Cfg::kTokens);
+        for (int kb = 0; kb < k_blocks; kb += Cfg::kSub) {
+          if (!ready && !mbar_wait_bounded(&full[stage], phase, abort_flag)) {
             ok = false;
             break;
           }
           tc_fence_after();
-          const uint32_t ab = smem_u32(sA + stage * Cfg::kABytes), bb = smem_u32(sB + stage * Cfg::kBBytes);
+          const uint64_t ad = a_desc + (uint32_t)(stage * (Cfg::kABytes >> 4));
+          const uint64_t bd = b_desc + (uint32_t)(stage * (Cfg::kBBytes >> 4));
+          const int next = stage + 1 == S ? 0 : stage + 1;
+          const uint32_t next_phase = stage + 1 == S ? phase ^ 1u : phase;
+          const bool tail = kb + Cfg::kSub > k_blocks;
 #pragma unroll
-          for (int kk = 0; kk < kI8BlockK / 32; ++kk) {
-            const uint64_t bd = make_smem_desc(bb + kk * 32, 16, 1024, kLayoutSw128);
-            const uint32_t accum = (kb > 0 || kk > 0) ? 1u : 0u;
-            umma_i8_pair(d, make_smem_desc(ab + kk * 32, 16, 1024, kLayoutSw128), bd, idesc, accum);
-            if (GATED)
-              umma_i8_pair(d + Cfg::kTokens, make_smem_desc(ab + kI8SubBytes + kk * 32, 16, 1024, kLayoutSw128),
-                           bd, idesc, accum);
+          for (int sub = 0; sub < Cfg::kSub; ++sub) {
+            if (sub > 0 && tail && kb + sub >= k_blocks) break;
+#pragma unroll
+            for (int kk = 0; kk < kI8BlockK / 32; ++kk) {
+              const uint32_t off_a = (sub * kI8SubBytes + kk * 32) >> 4, off_b = (sub * Cfg::kBSub + kk * 32) >> 4;
+              umma_i8_pair(d, ad + off_a, bd + off_b, idesc, (sub > 0 || kk > 0) ? 1u : (kb > 0 ? 1u : 0u));
+              // the next stage's barrier is looked at while the tensor cores have work queued: waiting for it
+              // after the commit left them idle (8192 x 4096 x 4096: 154 k cycles against 147 k)
+              if (kk == 1 && sub == 0) ready = mbar_test_wait(&full[next], next_phase);
+            }
           }
           umma_commit_pair(smem_u32(&empty[stage]));
           umma_commit_pair(empty_peer + 8u * (uint32_t)stage);
-          if (++stage == S) {
-            stage = 0;
-            phase ^= 1u;
-          }
+          stage = next;
+          phase = next_phase;
         }
         if (!ok) break;
         umma_commit_pair(smem_u32(&tfull[acc]));
@@ -207,17 +324,17 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(I8Pair<GATED>::kThre
     float *scale = s_scale + (warp - 2) * Cfg::kWarpTokens;
     const uint32_t tempty_leader = mapa_shared(smem_u32(tempty), 0);
     const float low = p.act == EIR_ACT_RELU ? 0.f : -INFINITY;
-    // 4-byte stores of two channels need even rows and a 4-byte base
-    const bool pairs = sizeof(T) == 2 && p.s_out % 2 == 0 && (reinterpret_cast<uintptr_t>(a.out) & 3) == 0;
+    const bool pairs = i8_pairs(p, a);
+    const int row = q * 32 + lane;
     int acc = 0;
     uint32_t acc_phase = 0;
     for (uint32_t t = pair_id; t < tiles; t += n_pairs) {
       uint32_t ct, tt;
       i8_pair_tile(t, c_tiles, t_tiles, ct, tt);
-      const int64_t c = (int64_t)ct * 256 + rank * kI8Rows + q * 32 + lane;
+      const int64_t c = i8_row_channel<GATED>((int64_t)(2 * ct + rank) * i8_channels<GATED>(), row);
       const int64_t t0 = (int64_t)tt * Cfg::kTokens + col0;
       // the tile's scales are fetched under its MMAs
-      const I8Channel h = i8_channel(p, a, c, n_out, GATED);
+      const I8Row h = i8_row<GATED>(p, a, c, row, n_out);
       __syncwarp();
       for (int i = lane; i < Cfg::kWarpTokens; i += 32)
         scale[i] = a.scale_l && t0 + i < p.m ? a.scale_l[t0 + i] : 1.f;
@@ -227,38 +344,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(I8Pair<GATED>::kThre
         break;
       }
       tc_fence_after();
-      T *out = static_cast<T *>(a.out) + t0 * p.s_out + c;
-      const uint32_t src = tmem_base + ((uint32_t)(q * 32) << 16) + (uint32_t)(acc * Cfg::kAccCols + col0);
+      T *out = static_cast<T *>(a.out) + t0 * p.s_out;
+      const uint32_t src = tmem_base + ((uint32_t)(q * 32) << 16) + (uint32_t)(acc * Cfg::kTokens + col0);
 #pragma unroll 1
-      for (int ch = 0; ch < Cfg::kWarpTokens && t0 + ch < p.m; ch += 16, out += 16 * p.s_out) {
-        uint32_t v[16], u[16];
-        tmem_ld_32x32b_x16(src + ch, v);
-        if (GATED) tmem_ld_32x32b_x16(src + Cfg::kTokens + ch, u);
-        tmem_ld_wait();
-        const int left = (int)min((int64_t)16, p.m - (t0 + ch));
-        float z[16];
-#pragma unroll
-        for (int i = 0; i < 16; ++i)
-          z[i] = i8_value<GATED>((int32_t)v[i], GATED ? (int32_t)u[i] : 0, scale[ch + i], h, low);
-        if (pairs && left == 16) {
-          // lanes 2j and 2j + 1 swap halves: each then holds two channels of one token
-          const bool odd = lane & 1;
-          T *o = out - (odd ? 1 : 0) + (odd ? p.s_out : 0);
-          const bool two = c - (odd ? 1 : 0) + 1 < n_out, one = c - (odd ? 1 : 0) < n_out;
-#pragma unroll
-          for (int i = 0; i < 16; i += 2) {
-            const __nv_bfloat162 b = __floats2bfloat162_rn(z[i], z[i + 1]);
-            const uint32_t mine = *reinterpret_cast<uint32_t const *>(&b);
-            const uint32_t theirs = __shfl_xor_sync(0xffffffffu, mine, 1);
-            const uint32_t w = odd ? __byte_perm(theirs, mine, 0x7632) : __byte_perm(mine, theirs, 0x5410);
-            if (two) *reinterpret_cast<uint32_t *>(o + i * p.s_out) = w;
-            else if (one) *reinterpret_cast<uint16_t *>(o + i * p.s_out) = (uint16_t)w;
-          }
-        } else if (c < n_out) {
-#pragma unroll
-          for (int i = 0; i < 16; ++i)
-            if (i < left) out[i * p.s_out] = from_f32<T>(z[i]);
-        }
+      for (int ch = 0; ch < Cfg::kWarpTokens && t0 + ch < p.m; ch += kI8Chunk, out += kI8Chunk * p.s_out) {
+        float z[kI8Chunk];
+        i8_drain(src + ch, scale + ch, h, z);
+        i8_store_chunk<GATED, T>(out, p.s_out, z, c, n_out, (int)min((int64_t)kI8Chunk, p.m - (t0 + ch)), pairs, low);
       }
       tc_fence_before();
       __syncwarp();
@@ -284,40 +376,41 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(I8Pair<GATED>::kThre
 
 // ---------------------------------------------------------------- split K over a cluster
 
-template <int NT, bool GATED>
+template <int NT>
 struct I8Split {
-  static constexpr int kABytes = kI8SubBytes * (GATED ? 2 : 1);
   static constexpr int kBBytes = NT * kI8BlockK;
-  static constexpr int kStageBytes = kABytes + kBBytes;
-  static constexpr int kAccBytes = NT * kI8Rows * 4 * (GATED ? 2 : 1);  // the exchanged accumulators
+  static constexpr int kStageBytes = kI8SubBytes + kBBytes;
+  static constexpr int kAccBytes = NT * kI8Rows * 4;  // the exchanged accumulators
   // about 100 KB a CTA, two CTAs on an SM: enough bytes in flight for HBM
-  static constexpr int kFit = 104 * 1024 / kStageBytes;
-  static constexpr int kStages = kFit < 2 ? 2 : kFit;
-  static constexpr int kRing = kStages * kStageBytes > kAccBytes ? kStages * kStageBytes : kAccBytes;
-  static constexpr int kCols0 = NT * (GATED ? 2 : 1);
-  static constexpr int kCols = kCols0 < 32 ? 32 : kCols0;
+  static constexpr int kStages = 104 * 1024 / kStageBytes;
+  static constexpr int kRing = kStages * kStageBytes;
+  static constexpr int kCols = NT < 32 ? 32 : NT;  // TMEM
   static constexpr int kThreads = 192;
-  static constexpr int kSmemBytes = 1024 + kRing + 512;
-  static_assert(kSmemBytes <= 232448 && kCols <= 256, "shared memory and TMEM of two CTAs");
+  static constexpr int kSmemBytes = 1024 + kRing + 512 + 512;
+  static_assert(kAccBytes <= kRing, "the exchange reuses the ring");
 };
 
-__device__ __forceinline__ int32_t ld_cluster_s32(uint32_t addr_cluster) {
-  int32_t v;
-  asm volatile("ld.shared::cluster.s32 %0, [%1];" : "=r"(v) : "r"(addr_cluster) : "memory");
+__device__ __forceinline__ int4 ld_cluster_v4(uint32_t addr_cluster) {
+  int4 v;
+  asm volatile("ld.shared::cluster.v4.s32 {%0, %1, %2, %3}, [%4];"
+               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+               : "r"(addr_cluster)
+               : "memory");
   return v;
 }
 
 template <int NT, bool GATED, typename T>
-__global__ void __launch_bounds__(192, 1)
+__global__ void __launch_bounds__(192, 2)
     i8_split_kernel(const __grid_constant__ CUtensorMap map_c, const __grid_constant__ CUtensorMap map_t,
                     const I8Params p, const I8Ptrs a, uint32_t *err, uint32_t split, uint32_t t_tiles) {
-  using Cfg = I8Split<NT, GATED>;
+  using Cfg = I8Split<NT>;
   constexpr int S = Cfg::kStages;
   extern __shared__ uint8_t smem_raw[];
   uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  uint8_t *sA = smem, *sB = smem + S * Cfg::kABytes;
-  int32_t *s_acc = reinterpret_cast<int32_t *>(smem);  // [gate, value][token][channel], after the last MMA
-  uint64_t *bars = reinterpret_cast<uint64_t *>(smem + Cfg::kRing);
+  uint8_t *sA = smem, *sB = smem + S * kI8SubBytes;
+  int32_t *s_acc = reinterpret_cast<int32_t *>(smem);  // [token][row], after the last MMA
+  float *s_scale = reinterpret_cast<float *>(smem + Cfg::kRing);  // the tile's token scales
+  uint64_t *bars = reinterpret_cast<uint64_t *>(smem + Cfg::kRing + 512);
   uint64_t *full = bars, *empty = bars + S, *tfull = bars + 2 * S;
   uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(bars + 2 * S + 1);
   volatile int *abort_flag = reinterpret_cast<volatile int *>(tmem_slot + 1);
@@ -327,7 +420,7 @@ __global__ void __launch_bounds__(192, 1)
   const uint32_t tile = blockIdx.x / split, ct = tile / t_tiles, tt = tile % t_tiles;
   const int k_blocks = (int)((p.k + kI8BlockK - 1) / kI8BlockK);
   const int kb0 = (int)((int64_t)k_blocks * rank / split), kb1 = (int)((int64_t)k_blocks * (rank + 1) / split);
-  const int64_t n_out = GATED ? p.n / 2 : p.n;
+  const int64_t n_out = GATED ? p.n / 2 : p.n, c0 = (int64_t)ct * i8_channels<GATED>();
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < S; ++s) {
@@ -348,10 +441,12 @@ __global__ void __launch_bounds__(192, 1)
   pdl_launch_dependents();
   pdl_wait();
 
+  const int64_t t0 = (int64_t)tt * NT;
+  const int tokens = (int)min((int64_t)NT, p.m - t0);
+  const float low = p.act == EIR_ACT_RELU ? 0.f : -INFINITY;
   bool ok = true;  // this thread's view: false once a wait of the CTA has given up
   if (warp == 0) {
     if (lane == 0) {
-      const int row_c = (int)(ct * kI8Rows), row_t = (int)(tt * NT);
       int stage = 0;
       uint32_t phase = 0;
       for (int kb = kb0; kb < kb1; ++kb) {
@@ -359,11 +454,13 @@ __global__ void __launch_bounds__(192, 1)
           ok = false;
           break;
         }
-        mbar_arrive_expect_tx(&full[stage], Cfg::kStageBytes);
-        uint8_t *dA = sA + stage * Cfg::kABytes;
-        tma_load_2d(dA, &map_c, &full[stage], kb * kI8BlockK, row_c);
-        if (GATED) tma_load_2d(dA + kI8SubBytes, &map_c, &full[stage], kb * kI8BlockK, row_c + (int)n_out);
-        tma_load_2d(sB + stage * Cfg::kBBytes, &map_t, &full[stage], kb * kI8BlockK, row_t);
+        uint64_t *bar = &full[stage];
+        mbar_arrive_expect_tx(bar, Cfg::kStageBytes);
+        i8_load_rows<GATED>(
+            sA + stage * kI8SubBytes, kb * kI8BlockK, (int)c0,
+            [&](void *dst, int x, int y) { tma_load_2d(dst, &map_c, bar, x, y); },
+            [&](void *dst, int x, int y) { tma_load_3d(dst, &map_c, bar, x, y, 0); });
+        tma_load_2d(sB + stage * Cfg::kBBytes, &map_t, bar, kb * kI8BlockK, (int)t0);
         if (++stage == S) {
           stage = 0;
           phase ^= 1u;
@@ -377,6 +474,8 @@ __global__ void __launch_bounds__(192, 1)
   } else if (warp == 1) {
     if (lane == 0) {
       constexpr uint32_t idesc = i8_idesc(kI8Rows, NT);
+      const uint64_t a_desc = make_smem_desc(smem_u32(sA), 16, 1024, kLayoutSw128);
+      const uint64_t b_desc = make_smem_desc(smem_u32(sB), 16, 1024, kLayoutSw128);
       int stage = 0;
       uint32_t phase = 0;
       for (int kb = kb0; kb < kb1; ++kb) {
@@ -385,16 +484,11 @@ __global__ void __launch_bounds__(192, 1)
           break;
         }
         tc_fence_after();
-        const uint32_t ab = smem_u32(sA + stage * Cfg::kABytes), bb = smem_u32(sB + stage * Cfg::kBBytes);
+        const uint64_t ad = a_desc + (uint32_t)(stage * (kI8SubBytes >> 4));
+        const uint64_t bd = b_desc + (uint32_t)(stage * (Cfg::kBBytes >> 4));
 #pragma unroll
-        for (int kk = 0; kk < kI8BlockK / 32; ++kk) {
-          const uint64_t bd = make_smem_desc(bb + kk * 32, 16, 1024, kLayoutSw128);
-          const uint32_t accum = (kb > kb0 || kk > 0) ? 1u : 0u;
-          umma_i8(tmem_base, make_smem_desc(ab + kk * 32, 16, 1024, kLayoutSw128), bd, idesc, accum);
-          if (GATED)
-            umma_i8(tmem_base + NT, make_smem_desc(ab + kI8SubBytes + kk * 32, 16, 1024, kLayoutSw128), bd, idesc,
-                    accum);
-        }
+        for (int kk = 0; kk < kI8BlockK / 32; ++kk)
+          umma_i8(tmem_base, ad + kk * 2, bd + kk * 2, idesc, kk > 0 ? 1u : (kb > kb0 ? 1u : 0u));
         umma_commit(&empty[stage]);
         if (++stage == S) {
           stage = 0;
@@ -407,11 +501,30 @@ __global__ void __launch_bounds__(192, 1)
         *abort_flag = 1;
       }
     }
+  } else {
+    for (int i = threadIdx.x - 64; i < NT; i += 128) s_scale[i] = a.scale_l && i < tokens ? a.scale_l[t0 + i] : 1.f;
+    asm volatile("bar.sync 1, 128;" ::: "memory");  // the four epilogue warps
+  }
+  // the row side of this thread's outputs, fetched under the MMAs: of its TMEM
+  // row, or of the four rows that it adds up for the cluster
+  const int q = warp & 3, row = q * 32 + lane;
+  const int64_t c = i8_row_channel<GATED>(c0, row);
+  I8Row h[4];
+  if (split == 1) {
+    if (warp >= 2) h[0] = i8_row<GATED>(p, a, c, row, n_out);
+  } else {
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      h[e] = i8_row<GATED>(p, a, i8_row_channel<GATED>(c0, 4 * lane + e), 4 * lane + e, n_out);
   }
   __syncwarp();
   // every warp waits for the accumulators: the ring is free for the exchange, and nothing is in
   // flight when the CTA ends
-  if (!mbar_wait_warp(tfull, 0u, abort_flag) && lane == 0 && !*abort_flag) {
+  int waited = 1;
+  if (lane == 0) waited = mbar_wait_bounded(tfull, 0u, abort_flag);
+  waited = __shfl_sync(0xffffffffu, waited, 0);
+  if (waited) (void)mbar_try_wait(tfull, 0u);  // every lane observes the completed phase itself
+  if (!waited && lane == 0 && !*abort_flag) {
     record_error(err, kErrTimeoutEpilogue);
     *abort_flag = 1;
   }
@@ -420,63 +533,73 @@ __global__ void __launch_bounds__(192, 1)
     for (int i = 0; i < 1000; ++i) __nanosleep(1000);  // copies issued before the abort land first
     ok = false;
   }
+  __syncwarp();
   tc_fence_after();
-  const int64_t t0 = (int64_t)tt * NT;
-  const int tokens = (int)min((int64_t)NT, p.m - t0);
-  const float low = p.act == EIR_ACT_RELU ? 0.f : -INFINITY;
-  const int q = warp & 3, row = q * 32 + lane;
-  const int64_t c = (int64_t)ct * kI8Rows + row;
   const uint32_t src = tmem_base + ((uint32_t)(q * 32) << 16);
   if (split == 1) {
     if (warp >= 2 && ok) {
-      const I8Channel h = i8_channel(p, a, c, n_out, GATED);
-      T *out = static_cast<T *>(a.out) + t0 * p.s_out + c;
+      const bool pairs = i8_pairs(p, a);
+      T *out = static_cast<T *>(a.out) + t0 * p.s_out;
 #pragma unroll 1
-      for (int ch = 0; ch < tokens; ch += 16) {
-        uint32_t v[16], u[16];
-        tmem_ld_32x32b_x16(src + ch, v);
-        if (GATED) tmem_ld_32x32b_x16(src + NT + ch, u);
-        tmem_ld_wait();
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          if (ch + i < tokens && c < n_out) {
-            const float sa = a.scale_l ? a.scale_l[t0 + ch + i] : 1.f;
-            out[(int64_t)(ch + i) * p.s_out] =
-                from_f32<T>(i8_value<GATED>((int32_t)v[i], GATED ? (int32_t)u[i] : 0, sa, h, low));
-          }
-        }
+      for (int ch = 0; ch < tokens; ch += kI8Chunk, out += kI8Chunk * p.s_out) {
+        float z[kI8Chunk];
+        i8_drain(src + ch, s_scale + ch, h[0], z);
+        i8_store_chunk<GATED, T>(out, p.s_out, z, c, n_out, min(kI8Chunk, tokens - ch), pairs, low);
       }
     }
   } else {
     if (warp >= 2 && ok) {
 #pragma unroll 1
-      for (int ch = 0; ch < tokens; ch += 16) {
+      for (int ch = 0; ch < tokens; ch += kI8Chunk) {
+        uint32_t v[kI8Chunk];
+        tmem_ld_32x32b_x16(src + ch, v);
+        tmem_ld_wait();
 #pragma unroll
-        for (int half = 0; half < (GATED ? 2 : 1); ++half) {
-          uint32_t v[16];
-          tmem_ld_32x32b_x16(src + half * NT + ch, v);
-          tmem_ld_wait();
-#pragma unroll
-          for (int i = 0; i < 16; ++i)
-            if (ch + i < tokens) s_acc[(half * NT + ch + i) * kI8Rows + row] = (int32_t)v[i];
-        }
+        for (int i = 0; i < kI8Chunk; ++i) s_acc[(ch + i) * kI8Rows + row] = (int32_t)v[i];
       }
     }
     __syncwarp();
     cluster_sync();  // every CTA's partial sums are in its shared memory
-    if (warp >= 2 && ok) {
-      const I8Channel h = i8_channel(p, a, c, n_out, GATED);
-      // CTA `rank` adds up and stores every split-th token
-      for (int j = (int)rank; j < tokens; j += (int)split) {
-        int32_t acc = 0, acc2 = 0;
-        const uint32_t at = smem_u32(s_acc + j * kI8Rows + row);
+    // CTA `rank` adds up and stores every split-th token, a warp a token, four rows a lane
+    if (ok) {
+      const bool value = GATED && (lane & 4) != 0;  // lanes l and l + 4: a gate and its value
+      const int64_t cq = i8_row_channel<GATED>(c0, 4 * lane);
+      const uint32_t at = smem_u32(s_acc) + 16u * (uint32_t)lane;
+      T *out = static_cast<T *>(a.out) + t0 * p.s_out + cq;
+      const bool wide = p.s_out % 4 == 0 && reinterpret_cast<uintptr_t>(a.out) % (4 * sizeof(T)) == 0 && cq + 4 <= n_out;
+#pragma unroll 2
+      for (int j = (int)rank + warp * (int)split; j < tokens; j += 6 * (int)split) {
+        int4 acc = make_int4(0, 0, 0, 0);
+#pragma unroll 8
         for (uint32_t r = 0; r < split; ++r) {
-          acc += ld_cluster_s32(mapa_shared(at, r));
-          if (GATED) acc2 += ld_cluster_s32(mapa_shared(at + NT * kI8Rows * 4, r));
+          const int4 v = ld_cluster_v4(mapa_shared(at + (uint32_t)(j * kI8Rows * 4), r));
+          acc.x += v.x;
+          acc.y += v.y;
+          acc.z += v.z;
+          acc.w += v.w;
         }
-        if (c < n_out) {
-          const float sa = a.scale_l ? a.scale_l[t0 + j] : 1.f;
-          static_cast<T *>(a.out)[(t0 + j) * p.s_out + c] = from_f32<T>(i8_value<GATED>(acc, acc2, sa, h, low));
+        const float sa = s_scale[j];
+        float z[4] = {i8_scaled(acc.x, sa, h[0].sb, h[0].bias), i8_scaled(acc.y, sa, h[1].sb, h[1].bias),
+                      i8_scaled(acc.z, sa, h[2].sb, h[2].bias), i8_scaled(acc.w, sa, h[3].sb, h[3].bias)};
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          if (GATED) z[e] = silu(z[e]) * __shfl_xor_sync(0xffffffffu, z[e], 4);
+          else z[e] = relu_from(z[e], low);
+        }
+        if (value) continue;
+        T *o = out + j * p.s_out;
+        if (wide) {
+          if (sizeof(T) == 2) {
+            const __nv_bfloat162 lo = __floats2bfloat162_rn(z[0], z[1]), hi = __floats2bfloat162_rn(z[2], z[3]);
+            *reinterpret_cast<uint2 *>(o) = make_uint2(*reinterpret_cast<uint32_t const *>(&lo),
+                                                       *reinterpret_cast<uint32_t const *>(&hi));
+          } else {
+            *reinterpret_cast<float4 *>(o) = make_float4(z[0], z[1], z[2], z[3]);
+          }
+        } else {
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            if (cq + e < n_out) o[e] = from_f32<T>(z[e]);
         }
       }
     }
@@ -507,7 +630,7 @@ static cudaError_t i8_allow_smem(Kern kern, int bytes, bool (&done)[32]) {
 template <bool GATED, typename T>
 static cudaError_t launch_pair(I8TcPlan const &tp, CUtensorMap const &mc, CUtensorMap const &mt, I8Params const &p,
                                I8Ptrs const &a, uint32_t *err, cudaStream_t st) {
-  using Cfg = I8Pair<GATED>;
+  using Cfg = I8Pair;
   auto kern = i8_pair_kernel<GATED, T>;
   static bool done[32] = {};
   cudaError_t e = i8_allow_smem(kern, Cfg::kSmemBytes, done);
@@ -535,7 +658,7 @@ static cudaError_t launch_pair(I8TcPlan const &tp, CUtensorMap const &mc, CUtens
 template <int NT, bool GATED, typename T>
 static cudaError_t launch_split(I8TcPlan const &tp, CUtensorMap const &mc, CUtensorMap const &mt, I8Params const &p,
                                 I8Ptrs const &a, uint32_t *err, cudaStream_t st) {
-  using Cfg = I8Split<NT, GATED>;
+  using Cfg = I8Split<NT>;
   auto kern = i8_split_kernel<NT, GATED, T>;
   static bool done[32] = {};
   cudaError_t e = i8_allow_smem(kern, Cfg::kSmemBytes, done);
@@ -575,7 +698,7 @@ static cudaError_t launch_i8_tc_t(I8TcPlan const &tp, CUtensorMap const &mc, CUt
   }
 }
 
-int i8_box_tokens(I8TcPlan const &tp, bool gated) { return tp.tokens ? tp.tokens : (gated ? 64 : 128); }
+int i8_box_tokens(I8TcPlan const &tp) { return tp.tokens ? tp.tokens : I8Pair::kTokens / 2; }
 
 cudaError_t launch_i8_tc(I8TcPlan const &tp, CUtensorMap const &mc, CUtensorMap const &mt, I8Params const &p,
                          I8Ptrs const &a, uint32_t *err, cudaStream_t st) {

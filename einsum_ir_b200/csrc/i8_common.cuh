@@ -71,6 +71,11 @@ __device__ __forceinline__ void tma_load_3d_pair(void *dst, void const *map, uin
       : "memory");
 }
 
+// arrive on an mbarrier of any CTA of the cluster without ordering earlier memory accesses
+__device__ __forceinline__ void mbar_arrive_cluster_relaxed(uint32_t bar_cluster) {
+  asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar_cluster) : "memory");
+}
+
 // instruction descriptor of kind::i8: signed 8-bit operands, both K-major, 32-bit integer accumulate
 __host__ __device__ constexpr uint32_t i8_idesc(int m, int n) {
   return (2u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(m >> 4) << 24);

@@ -32,7 +32,7 @@ namespace eir {
 constexpr int kI8Rows = 128;                      // staged right rows of a CTA
 constexpr int kI8BlockK = 128;                    // K of a block: one swizzle row
 constexpr int kI8SubBytes = kI8Rows * kI8BlockK;  // a block of 128 rows
-constexpr int kI8Chunk = 16;                      // tokens drained from TMEM at a time
+constexpr int kI8Chunk = 32;                      // tokens the pair kernel drains from TMEM at a time
 
 // output channels of a CTA's 128 rows
 template <bool GATED>
@@ -72,13 +72,12 @@ __device__ __forceinline__ I8Row i8_row(I8Params const &p, I8Ptrs const &a, int6
   return h;
 }
 
-// 16 accumulators of a thread's row from TMEM, scaled: z[i] of token i
-__device__ __forceinline__ void i8_drain(uint32_t src, float const *scale, I8Row const &h, float (&z)[kI8Chunk]) {
-  uint32_t v[kI8Chunk];
-  tmem_ld_32x32b_x16(src, v);
-  tmem_ld_wait();
+// accumulators of a thread's row (tokens 0 .. CH - 1), scaled
+template <int CH>
+__device__ __forceinline__ void i8_scale_row(uint32_t const (&v)[CH], float const *scale, I8Row const &h,
+                                             float (&z)[CH]) {
 #pragma unroll
-  for (int i = 0; i < kI8Chunk; i += 4) {
+  for (int i = 0; i < CH; i += 4) {
     const float4 s = *reinterpret_cast<float4 const *>(scale + i);
     const float2 z0 = scaled2((int32_t)v[i], (int32_t)v[i + 1], make_float2(s.x, s.y), h.sb, h.bias);
     const float2 z1 = scaled2((int32_t)v[i + 2], (int32_t)v[i + 3], make_float2(s.z, s.w), h.sb, h.bias);
@@ -89,15 +88,34 @@ __device__ __forceinline__ void i8_drain(uint32_t src, float const *scale, I8Row
   }
 }
 
-// Stores a warp's 32 rows x 16 tokens. Gated: lanes l and l + 16 first trade
+// how a warp stores its rows: fixed for a kernel's call, or for a tile
+struct I8Store {
+  bool relu;
+  bool words;         // two channels a 4-byte store (BF16, even rows, base on a word)
+  uint32_t step[4];   // byte offsets of the tokens 2, 4, 6, 8 (x 2 when gated) after the first, below 2^32
+};
+template <bool GATED, typename T>
+__device__ __forceinline__ I8Store i8_store_mode(I8Params const &p, I8Ptrs const &a) {
+  I8Store m;
+  constexpr int64_t kStep = (GATED ? 4 : 2) * sizeof(T);
+  m.relu = p.act == EIR_ACT_RELU;
+  m.words = sizeof(T) == 2 && p.s_out % 2 == 0 && (reinterpret_cast<uintptr_t>(a.out) & 3) == 0 &&
+            p.s_out < (1 << 26);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) m.step[i] = (uint32_t)((i + 1) * kStep * p.s_out);
+  return m;
+}
+
+// Stores a warp's 32 rows x CH tokens. Gated: lanes l and l + 16 first trade
 // halves of their tokens, so that lane l holds gate and value of the even
 // tokens and lane l + 16 of the odd ones. BF16 on even rows: lanes 2j and
-// 2j + 1 then trade tokens too and store two channels in one word.
+// 2j + 1 then trade tokens too and store two channels in one word (half the
+// store instructions of one channel a lane).
 //   out: the first token's row; c: the lane's channel; tokens: how many exist
-template <bool GATED, typename T>
-__device__ __forceinline__ void i8_store_chunk(T *out, int64_t stride, float (&z)[kI8Chunk], int64_t c, int64_t n_out,
-                                               int tokens, bool pairs, float low) {
-  constexpr int N = GATED ? kI8Chunk / 2 : kI8Chunk, STEP = GATED ? 2 : 1;  // token of w[j]: STEP j + first
+template <bool GATED, typename T, int CH>
+__device__ __forceinline__ void i8_store_chunk(T *out, int64_t stride, float (&z)[CH], int64_t c, int64_t n_out,
+                                               int tokens, I8Store const &m) {
+  constexpr int N = GATED ? CH / 2 : CH, STEP = GATED ? 2 : 1;  // token of w[j]: STEP j + first
   const int lane = threadIdx.x & 31, first = GATED ? lane >> 4 : 0;
   float w[N];
   if (GATED) {
@@ -108,33 +126,30 @@ __device__ __forceinline__ void i8_store_chunk(T *out, int64_t stride, float (&z
     }
   } else {
 #pragma unroll
-    for (int j = 0; j < N; ++j) w[j] = relu_from(z[j], low);
+    for (int j = 0; j < N; ++j) w[j] = z[j];
   }
-  if (sizeof(T) == 2 && pairs && tokens == kI8Chunk) {
-    const int odd = lane & 1;
+  const int odd = lane & 1;
+  if (sizeof(T) == 2 && m.words && tokens >= CH && __all_sync(0xffffffffu, c - odd + 1 < n_out)) {
     const uint32_t pick = odd ? 0x3276u : 0x5410u;
-    const bool two = c - odd + 1 < n_out, one = c - odd < n_out;
+    // the rounding is monotone, so the ReLU may follow it
+    const __nv_bfloat162 low = __float2bfloat162_rn(m.relu ? 0.f : -INFINITY);
     char *o = reinterpret_cast<char *>(out + (first + (odd ? STEP : 0)) * stride + c - odd);
-    const int64_t step = 4 * STEP * stride;
 #pragma unroll
-    for (int j = 0; j < N; j += 2, o += step) {
-      const __nv_bfloat162 b = __floats2bfloat162_rn(w[j], w[j + 1]);
+    for (int j = 0; j < N; j += 2) {
+      __nv_bfloat162 b = __floats2bfloat162_rn(w[j], w[j + 1]);
+      if (!GATED) b = __hmax2_nan(b, low);
       const uint32_t mine = *reinterpret_cast<uint32_t const *>(&b);
       const uint32_t both = __byte_perm(mine, __shfl_xor_sync(0xffffffffu, mine, 1), pick);
-      if (two) *reinterpret_cast<uint32_t *>(o) = both;
-      else if (one) *reinterpret_cast<uint16_t *>(o) = (uint16_t)both;
+      *reinterpret_cast<uint32_t *>(o + (j % 8 ? m.step[j % 8 / 2 - 1] : 0u)) = both;
+      if (j % 8 == 6) o += m.step[3];
     }
   } else if (c < n_out) {
+    const float low = m.relu ? 0.f : -INFINITY;
     T *o = out + first * stride + c;
 #pragma unroll
     for (int j = 0; j < N; ++j, o += STEP * stride)
-      if (STEP * j + first < tokens) *o = from_f32<T>(w[j]);
+      if (STEP * j + first < tokens) *o = from_f32<T>(GATED ? w[j] : relu_from(w[j], low));
   }
-}
-
-// two-channel stores need even rows and a base on a word
-__device__ __forceinline__ bool i8_pairs(I8Params const &p, I8Ptrs const &a) {
-  return p.s_out % 2 == 0 && (reinterpret_cast<uintptr_t>(a.out) & 3) == 0;
 }
 
 // ---------------------------------------------------------------- CTA pairs
@@ -323,8 +338,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(I8Pair::kThreads, 1)
     const int col0 = ((warp - 2) >> 2) * Cfg::kWarpTokens;
     float *scale = s_scale + (warp - 2) * Cfg::kWarpTokens;
     const uint32_t tempty_leader = mapa_shared(smem_u32(tempty), 0);
-    const float low = p.act == EIR_ACT_RELU ? 0.f : -INFINITY;
-    const bool pairs = i8_pairs(p, a);
+    const I8Store mode = i8_store_mode<GATED, T>(p, a);
     const int row = q * 32 + lane;
     int acc = 0;
     uint32_t acc_phase = 0;
@@ -344,17 +358,29 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(I8Pair::kThreads, 1)
         break;
       }
       tc_fence_after();
+      // the accumulator back to the MMAs once it is in registers. The arrive is relaxed: the
+      // tcgen05 fence orders it after the TMEM reads, and a release would wait
+      // for the tile's global stores too
+      auto release_acc = [&]() {
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive_cluster_relaxed(tempty_leader + 8u * (uint32_t)acc);
+      };
       T *out = static_cast<T *>(a.out) + t0 * p.s_out;
       const uint32_t src = tmem_base + ((uint32_t)(q * 32) << 16) + (uint32_t)(acc * Cfg::kTokens + col0);
+      const int tokens = (int)min((int64_t)Cfg::kWarpTokens, p.m - t0);  // <= 0: none of the tile's
+      uint32_t v[kI8Chunk];
+      if (tokens > 0) tmem_ld_32x32b_x32(src, v);
 #pragma unroll 1
-      for (int ch = 0; ch < Cfg::kWarpTokens && t0 + ch < p.m; ch += kI8Chunk, out += kI8Chunk * p.s_out) {
+      for (int ch = 0; ch < tokens; ch += kI8Chunk, out += kI8Chunk * p.s_out) {
         float z[kI8Chunk];
-        i8_drain(src + ch, scale + ch, h, z);
-        i8_store_chunk<GATED, T>(out, p.s_out, z, c, n_out, (int)min((int64_t)kI8Chunk, p.m - (t0 + ch)), pairs, low);
+        tmem_ld_wait();
+        i8_scale_row(v, scale + ch, h, z);
+        if (ch + kI8Chunk < tokens) tmem_ld_32x32b_x32(src + ch + kI8Chunk, v);  // under this chunk's stores
+        else release_acc();
+        i8_store_chunk<GATED, T>(out, p.s_out, z, c, n_out, tokens - ch, mode);
       }
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive_cluster(tempty_leader + 8u * (uint32_t)acc);
+      if (tokens <= 0) release_acc();
       acc ^= 1;
       if (acc == 0) acc_phase ^= 1u;
     }
@@ -538,24 +564,27 @@ __global__ void __launch_bounds__(192, 2)
   const uint32_t src = tmem_base + ((uint32_t)(q * 32) << 16);
   if (split == 1) {
     if (warp >= 2 && ok) {
-      const bool pairs = i8_pairs(p, a);
+      const I8Store mode = i8_store_mode<GATED, T>(p, a);
       T *out = static_cast<T *>(a.out) + t0 * p.s_out;
 #pragma unroll 1
-      for (int ch = 0; ch < tokens; ch += kI8Chunk, out += kI8Chunk * p.s_out) {
-        float z[kI8Chunk];
-        i8_drain(src + ch, s_scale + ch, h[0], z);
-        i8_store_chunk<GATED, T>(out, p.s_out, z, c, n_out, min(kI8Chunk, tokens - ch), pairs, low);
+      for (int ch = 0; ch < tokens; ch += 16, out += 16 * p.s_out) {
+        uint32_t v[16];
+        float z[16];
+        tmem_ld_32x32b_x16(src + ch, v);
+        tmem_ld_wait();
+        i8_scale_row(v, s_scale + ch, h[0], z);
+        i8_store_chunk<GATED, T>(out, p.s_out, z, c, n_out, tokens - ch, mode);
       }
     }
   } else {
     if (warp >= 2 && ok) {
 #pragma unroll 1
-      for (int ch = 0; ch < tokens; ch += kI8Chunk) {
-        uint32_t v[kI8Chunk];
+      for (int ch = 0; ch < tokens; ch += 16) {
+        uint32_t v[16];
         tmem_ld_32x32b_x16(src + ch, v);
         tmem_ld_wait();
 #pragma unroll
-        for (int i = 0; i < kI8Chunk; ++i) s_acc[(ch + i) * kI8Rows + row] = (int32_t)v[i];
+        for (int i = 0; i < 16; ++i) s_acc[(ch + i) * kI8Rows + row] = (int32_t)v[i];
       }
     }
     __syncwarp();

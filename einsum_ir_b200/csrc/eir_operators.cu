@@ -67,10 +67,12 @@ int workspace(eir_plan *p, void **ws) {
 }
 
 // Tiling of an 8-bit contraction on the tensor cores. Pair tiles once they
-// fill most of the GPU's 74 CTA pairs; else one-CTA tiles of just enough tokens, with
-// the K walk of each tile split over a cluster until two CTAs an SM are in flight.
+// fill most of the GPU's 74 CTA pairs; else one-CTA tiles of just enough
+// tokens, the K walk of each split over a cluster: the largest cluster of
+// which all tiles' clusters fit the GPU at once, two CTAs an SM (measured
+// limits; a second wave costs more than the split gains: 256 tokens x 4096 x
+// 4096, 64 tiles, take 14.4 us unsplit, 12.5 split by 4 and 21.7 split by 8).
 eir::I8TcPlan i8_tiling(eir::I8Params const &p) {
-  const int64_t sms = 148;
   eir::I8TcPlan t;
   t.c_tiles = (p.n + 255) / 256;  // gated: 128 gates and their values a tile
   t.t_tiles = (p.m + 255) / 256;
@@ -78,8 +80,12 @@ eir::I8TcPlan i8_tiling(eir::I8Params const &p) {
   t.tokens = p.m <= 16 ? 16 : p.m <= 32 ? 32 : p.m <= 64 ? 64 : 128;
   t.c_tiles = (p.n + 127) / 128;
   t.t_tiles = (p.m + t.tokens - 1) / t.tokens;
-  const int64_t k_blocks = (p.k + 127) / 128;
-  while (t.split < 8 && 2 * t.split * t.c_tiles * t.t_tiles <= 2 * sms && 2 * t.split <= k_blocks) t.split *= 2;
+  struct {
+    int split, tiles;
+  } const fits[] = {{8, 32}, {4, 66}, {3, 90}, {2, 148}};
+  for (auto const &f : fits) {
+    if (t.split == 1 && t.c_tiles * t.t_tiles <= f.tiles && (p.k + 127) / 128 >= 2 * f.split) t.split = f.split;
+  }
   return t;
 }
 
@@ -320,7 +326,13 @@ int eir_contract_int8(eir_plan *p, void const *left, void const *right, float co
   uint32_t *err = nullptr;
   int rc = eir::api_device(&num_sms, &err);
   if (rc != EIR_SUCCESS) return rc;
+  // one token: the row kernel, but for large layers that TMA can stream in
+  // place (4096 x 4096: 4.4 us against 6.0; 8192 x 28672: 40.6 against 37.9)
   I8Operand ops[2] = {i8_operand(left, p->i8.m, p->i8.k, p->i8.s_l), i8_operand(right, p->i8.n, p->i8.k, p->i8.s_r)};
+  if (p->i8.m == 1 && (ops[0].copy || ops[1].copy || p->i8.n * p->i8.k < ((int64_t)1 << 26))) {
+    ProfScope prof(p, st);
+    return launched(eir::launch_i8_row(p->i8, a, num_sms, st), "8-bit contraction launch");
+  }
   const int64_t ld = packed_stride(p->i8.k);
   for (int i = 0; i < 2; ++i) {
     I8Operand &o = ops[i];

@@ -87,6 +87,8 @@ cudaError_t launch_quantize(QuantizeParams const &p, void const *x, int8_t *q, f
 cudaError_t launch_i8_simt(I8Params const &p, I8Ptrs const &a, cudaStream_t st);
 cudaError_t launch_i8_tc(I8TcPlan const &tp, CUtensorMap const &map_channels, CUtensorMap const &map_tokens,
                          I8Params const &p, I8Ptrs const &a, uint32_t *err, cudaStream_t st);
+// one token (m = 1), any stride and alignment
+cudaError_t launch_i8_row(I8Params const &p, I8Ptrs const &a, int num_sms, cudaStream_t st);
 // token rows of one TMA box of the tiling `tp`
 int i8_box_tokens(I8TcPlan const &tp);
 // rows of k bytes, `stride` apart, into rows `ld` bytes apart

@@ -162,8 +162,8 @@ int eir_norm_plan_create(eir_norm_desc const *d, eir_plan **out) {
     n.s_dsum = d->stride_dsum;
     n.s_dx = d->stride_dx;
     p->empty = d->rows == 0;
-    // partial rows of the weight gradient: at most one per CTA of the backward kernel
-    p->ws_bytes = eir::norm_backward_ctas(n, eir::kMaxSms) * d->cols * 4;
+    // partial rows of the weight gradient
+    p->ws_bytes = eir::norm_backward_parts(n, eir::kMaxSms) * d->cols * 4;
     p->text = std::string("norm ") + type_text(n.dt) + " -> " + type_text(n.dt_out) + " rows=" +
               std::to_string(n.rows) + " cols=" + std::to_string(n.cols);
   });
@@ -213,7 +213,7 @@ int eir_norm_backward(eir_plan *p, void const *dy, void const *h, void const *we
   if (rc != EIR_SUCCESS) return rc;
   num_sms = std::min(num_sms, eir::kMaxSms);
   eir::NormGradPtrs a{dy, h, weight, dsum, rstd, dx, dweight, nullptr};
-  const int64_t ctas = eir::norm_backward_ctas(n, num_sms);
+  const int64_t parts = eir::norm_backward_parts(n, num_sms);
   if (dweight != nullptr) {
     void *ws = nullptr;
     rc = workspace(p, &ws);
@@ -225,7 +225,7 @@ int eir_norm_backward(eir_plan *p, void const *dy, void const *h, void const *we
     rc = launched(eir::launch_norm_backward(n, a, num_sms, st), "norm backward launch");
   }
   if (rc != EIR_SUCCESS || dweight == nullptr) return rc;
-  return launched(eir::launch_norm_dweight(n, a.part, ctas, dweight, st), "norm weight gradient launch");
+  return launched(eir::launch_norm_dweight(n, a.part, parts, dweight, st), "norm weight gradient launch");
 }
 
 // ---------------------------------------------------------------- quantize

@@ -6,145 +6,615 @@
 // s = m rstd / 127, so the integers need no rstd and the row's two statistics
 // (sum of squares, maximum) come from one pass. Backward: g = w dy,
 // dx = rstd (g - h rstd^2 mean(g h)) + dsum, dw = sum over rows of dy h rstd.
-// All sums in FP32. Bound by memory: each input is read once from HBM and each
-// output written once; the second pass over a row hits L2.
+// Sums are held in FP32.
+//
+// All three are bound by HBM. A row stays on the SM between the statistics and
+// the output, so each input is read once and each output written once. Up to
+// kPer elements a thread and 1024 threads it stays in registers: a warp a row for
+// narrow rows, a block above, in 16-byte pieces; blocks are persistent, and where
+// the rows lie on the pieces' grid they load their next row before they reduce the present
+// one. Wider rows stay in shared memory, and rows too wide for that are read twice.
+#include <algorithm>
 #include "eir_launch.h"
 #include "eir_common.cuh"
-#include "op_common.cuh"
 #include "op_params.h"
+#include "row_vec.cuh"
 
 namespace eir {
 
-constexpr int kRowThreads = 256;
-
-// one CTA a row: a pass for the statistics, a pass for the output
+// elements of a thread whose row stays in registers: FP32 rows take twice the
+// registers an element
 template <typename T>
-__global__ void __launch_bounds__(kRowThreads) norm_kernel(const NormParams p, const NormPtrs a) {
-  __shared__ uint32_t red[64];
+constexpr int kPer = sizeof(T) == 4 ? 8 : 16;  // norm and quantize
+template <typename T, typename G>
+constexpr int kPerBack = sizeof(T) + sizeof(G) == 8 ? 4 : 8;  // backward
+
+// Sum of v and maximum of m over a row's threads: a warp (`warps` = 1), or the
+// block, with one barrier (`red`: 64 words, other ones at the next call).
+template <bool SUM, bool MAX>
+__device__ __forceinline__ void row_sum_max(float &v, uint32_t &m, uint32_t *red, int warps) {
+  if (SUM) v = warp_sum(v);
+  if (MAX) m = __reduce_max_sync(0xffffffffu, m);
+  if (warps == 1) return;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (lane == 0) {
+    if (SUM) red[warp] = __float_as_uint(v);
+    if (MAX) red[32 + warp] = m;
+  }
+  __syncthreads();
+  if (SUM) v = warp_sum(lane < warps ? __uint_as_float(red[lane]) : 0.f);
+  if (MAX) m = __reduce_max_sync(0xffffffffu, lane < warps ? red[32 + lane] : 0u);
+}
+
+// ---------------------------------------------------------------- norm and quantize
+
+// One piece of the forward pass. OUT: int8_t, float or __nv_bfloat16; QUANT:
+// quantize (no sum of squares, residual or weight; NormParams' and NormPtrs' fields of the
+// same meaning); GRID: every row lies on the pieces' grid and has whole pieces
+template <typename T, typename OUT, bool QUANT, bool GRID>
+struct NormRow {
+  static constexpr int V = 16 / (int)sizeof(T);
+  static constexpr bool kInt8 = sizeof(OUT) == 1;
+  using Piece = RowPiece<T, V>;
+  NormParams const &p;
+  NormPtrs const &a;
+  RowBounds bx, br;
+  bool w_grid;
+
+  __device__ __forceinline__ NormRow(NormParams const &p_, NormPtrs const &a_) : p(p_), a(a_) {
+    if (!GRID) {
+      bx = row_bounds(a.x, p.rows, p.cols, p.s_x, sizeof(T));
+      br = row_bounds(a.res, p.rows, p.cols, p.s_res, sizeof(T));
+    }
+    w_grid = GRID || row_vec_ok(a.w, 0, 1, p.dt_w == EIR_FP32 ? 4 : 2, V);
+  }
+  __device__ __forceinline__ bool residual() const { return !QUANT && a.res != nullptr; }
+  __device__ __forceinline__ void load(int64_t row, int64_t c, Piece &x, Piece &r) const {
+    T const *px = static_cast<T const *>(a.x) + row * p.s_x, *pr = static_cast<T const *>(a.res) + row * p.s_res;
+    if (GRID) {
+      if (c < p.cols) x.template load<true>(px + c);
+      else x.zero();
+      if (residual() && c < p.cols) r.template load<true>(pr + c);
+    } else {
+      x.load_any(px, c, p.cols, bx.begin, bx.end);
+      if (residual()) r.load_any(pr, c, p.cols, br.begin, br.end);
+    }
+  }
+  template <typename D>
+  __device__ __forceinline__ void put(RowPiece<D, V> const &v, D *row, int64_t c) const {
+    if (!GRID) v.store_any(row, c, p.cols);
+    else if (c < p.cols) v.store(row + c);
+  }
+  // h (times the weight for 8-bit output) of a piece and its part of the
+  // statistics; stores the sum if `keep`. Every lane of a warp calls it
+  __device__ __forceinline__ void take(int64_t row, int64_t c, Piece const &x, Piece const &r, float (&h)[V],
+                                       float &ss, uint32_t &mx, bool keep = true) const {
+#pragma unroll
+    for (int e = 0; e < V; ++e) h[e] = x.get(e);
+    if (residual() && c < p.cols) {
+#pragma unroll
+      for (int e = 0; e < V; ++e) h[e] += r.get(e);
+    }
+    if (!QUANT) {
+#pragma unroll
+      for (int e = 0; e < V; ++e) ss += h[e] * h[e];
+      if (a.sum && keep) {
+        Piece s;
+        s.set(h);
+        put<T>(s, static_cast<T *>(a.sum) + row * p.s_sum, c);
+      }
+      if (kInt8 && a.w && c < p.cols) {
+        float w[V];
+        load_shared_any<V>(a.w, p.dt_w, c, p.cols, w_grid, w);
+#pragma unroll
+        for (int e = 0; e < V; ++e) h[e] = __fmul_rn(h[e], w[e]);
+      }
+    }
+    if (kInt8) {
+#pragma unroll
+      for (int e = 0; e < V; ++e) mx = max(mx, abs_bits(h[e]));
+    }
+  }
+  __device__ __forceinline__ void give(int64_t row, int64_t c, float const (&h)[V], float rstd,
+                                       QuantScale const &q) const {
+    OUT *out = static_cast<OUT *>(a.out) + row * p.s_out;
+    RowPiece<OUT, V> o;
+    if constexpr (kInt8) {
+      o.zero();
+#pragma unroll
+      for (int e = 0; e < V; ++e) o.w[e / 4] |= (uint32_t)(quant_one(h[e], q) & 0xff) << (8 * (e % 4));
+    } else {
+      float w[V], y[V];
+#pragma unroll
+      for (int e = 0; e < V; ++e) w[e] = 1.f;
+      if (a.w && c < p.cols) load_shared_any<V>(a.w, p.dt_w, c, p.cols, w_grid, w);
+#pragma unroll
+      for (int e = 0; e < V; ++e) y[e] = h[e] * rstd * w[e];
+      o.set(y);
+    }
+    put<OUT>(o, out, c);
+  }
+  __device__ __forceinline__ float rstd_of(float ss) const {
+    return QUANT ? 1.f : __frsqrt_rn(ss / (float)p.cols + p.eps);
+  }
+  __device__ __forceinline__ void row_values(int64_t row, float rstd, QuantScale const &q) const {
+    if (kInt8) a.scale[row] = q.scale;
+    if (!QUANT && a.rstd) a.rstd[row] = rstd;
+  }
+};
+
+template <typename T, typename OUT, bool QUANT, bool GRID>
+__global__ void __launch_bounds__(1024) norm_kernel(const NormParams p, const NormPtrs a, int row_warps) {
+  using Row = NormRow<T, OUT, QUANT, GRID>;
+  constexpr int V = Row::V, N = kPer<T> / V;
+  __shared__ uint32_t red[2][64];
   pdl_launch_dependents();
   pdl_wait();
-  for (int64_t row = blockIdx.x; row < p.rows; row += gridDim.x) {
-    T const *x = static_cast<T const *>(a.x) + row * p.s_x;
-    T const *r = a.res ? static_cast<T const *>(a.res) + row * p.s_res : nullptr;
-    T *sum = a.sum ? static_cast<T *>(a.sum) + row * p.s_sum : nullptr;
+  const Row op(p, a);
+  const int threads = row_warps * 32, tid = row_warps == 1 ? threadIdx.x & 31 : threadIdx.x;
+  const int64_t rows_at_once = row_warps == 1 ? (int64_t)gridDim.x * (blockDim.x >> 5) : gridDim.x;
+  int64_t row = row_warps == 1 ? (int64_t)blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5) : blockIdx.x;
+  auto column = [&](int j) { return (int64_t)(j * threads + tid) * V; };
+  typename Row::Piece x[N], r[N];
+  auto fetch = [&](int64_t at) {
+#pragma unroll
+    for (int j = 0; j < N; ++j) op.load(at, column(j), x[j], r[j]);
+  };
+  if (GRID && row < p.rows) fetch(row);
+  for (int turn = 0; row < p.rows; row += rows_at_once, turn ^= 1) {
+    if (!GRID) fetch(row);
+    float h[N][V];
     float ss = 0.f;
     uint32_t mx = 0;
-    for (int64_t c = threadIdx.x; c < p.cols; c += kRowThreads) {
-      float h = to_f32(x[c]);
-      if (r) h += to_f32(r[c]);
-      ss += h * h;
-      const float w = a.w ? ld_any(a.w, p.dt_w, c) : 1.f;
-      mx = max(mx, abs_bits(__fmul_rn(h, w)));
-    }
-    block_sum_max<kRowThreads / 32>(ss, mx, red);
-    const float rstd = rsqrtf(ss / (float)p.cols + p.eps);
+#pragma unroll
+    for (int j = 0; j < N; ++j) op.take(row, column(j), x[j], r[j], h[j], ss, mx);
+    if (GRID && row + rows_at_once < p.rows) fetch(row + rows_at_once);
+    row_sum_max<!QUANT, Row::kInt8>(ss, mx, red[turn], row_warps);
+    const float rstd = op.rstd_of(ss);
     const QuantScale q = quant_scale(mx, rstd);
-    for (int64_t c = threadIdx.x; c < p.cols; c += kRowThreads) {
-      float h = to_f32(x[c]);
-      if (r) h += to_f32(r[c]);
-      const float w = a.w ? ld_any(a.w, p.dt_w, c) : 1.f;
-      if (sum) sum[c] = from_f32<T>(h);
-      if (p.dt_out == EIR_INT8)
-        static_cast<int8_t *>(a.out)[row * p.s_out + c] = (int8_t)quant_one(__fmul_rn(h, w), q);
-      else
-        st_any(a.out, p.dt_out, row * p.s_out + c, h * rstd * w);
-    }
-    if (threadIdx.x == 0) {
-      if (a.rstd) a.rstd[row] = rstd;
-      if (p.dt_out == EIR_INT8) a.scale[row] = q.scale;
-    }
+#pragma unroll
+    for (int j = 0; j < N; ++j) op.give(row, column(j), h[j], rstd, q);
+    if (tid == 0) op.row_values(row, rstd, q);
   }
 }
 
-// a CTA walks rows blockIdx.x, + gridDim.x, ...; its thread t owns the columns
-// t, t + 256, ... of every row and adds their dy h rstd into its partial row
-// of the weight gradient (same thread, same order: no atomics)
-template <typename T>
-__global__ void __launch_bounds__(kRowThreads) norm_backward_kernel(const NormParams p, const NormGradPtrs a) {
-  __shared__ uint32_t red[64];
+// wide rows: h in shared memory (CACHED), or read again
+template <typename T, typename OUT, bool QUANT, bool CACHED>
+__global__ void __launch_bounds__(1024) norm_wide_kernel(const NormParams p, const NormPtrs a) {
+  using Row = NormRow<T, OUT, QUANT, false>;
+  constexpr int V = Row::V;
+  __shared__ uint32_t red[2][64];
+  extern __shared__ float4 held[];  // [piece][V / 4][thread]
   pdl_launch_dependents();
   pdl_wait();
-  float *part = a.part ? a.part + (int64_t)blockIdx.x * p.cols : nullptr;
-  for (int64_t row = blockIdx.x; row < p.rows; row += gridDim.x) {
-    T const *h = static_cast<T const *>(a.h) + row * p.s_h;
-    const float rstd = a.rstd[row];
-    float gh = 0.f;
-    uint32_t unused = 0;
-    for (int64_t c = threadIdx.x; c < p.cols; c += kRowThreads) {
-      const float w = a.w ? ld_any(a.w, p.dt_w, c) : 1.f;
-      gh += w * ld_any(a.dy, p.dt_grad, row * p.s_dy + c) * to_f32(h[c]);
-    }
-    block_sum_max<kRowThreads / 32>(gh, unused, red);
-    const float k = rstd * rstd * (gh / (float)p.cols);
-    for (int64_t c = threadIdx.x; c < p.cols; c += kRowThreads) {
-      const float w = a.w ? ld_any(a.w, p.dt_w, c) : 1.f;
-      const float dy = ld_any(a.dy, p.dt_grad, row * p.s_dy + c), hv = to_f32(h[c]);
-      float d = rstd * (w * dy - hv * k);
-      if (a.dsum) d += ld_any(a.dsum, p.dt_grad, row * p.s_dsum + c);
-      if (part) part[c] = (row == blockIdx.x ? 0.f : part[c]) + dy * (hv * rstd);
-      st_any(a.dx, p.dt_grad, row * p.s_dx + c, d);
-    }
-  }
-}
-
-// dw[c] = sum of the partial rows, in their order
-__global__ void __launch_bounds__(kRowThreads) norm_dweight_kernel(int64_t cols, float const *__restrict__ part,
-                                                                   int64_t n_part, float *__restrict__ dw) {
-  pdl_launch_dependents();
-  pdl_wait();
-  const int64_t c = (int64_t)blockIdx.x * kRowThreads + threadIdx.x;
-  if (c >= cols) return;
-  float s = 0.f;
-  for (int64_t i = 0; i < n_part; ++i) s += part[i * cols + c];
-  dw[c] = s;
-}
-
-template <typename T>
-__global__ void __launch_bounds__(kRowThreads) quantize_kernel(const QuantizeParams p, void const *xv,
-                                                               int8_t *__restrict__ out, float *scale) {
-  __shared__ uint32_t red[64];
-  pdl_launch_dependents();
-  pdl_wait();
-  for (int64_t row = blockIdx.x; row < p.rows; row += gridDim.x) {
-    T const *x = static_cast<T const *>(xv) + row * p.s_x;
+  const Row op(p, a);
+  const int threads = blockDim.x, pieces = (int)((p.cols + (int64_t)threads * V - 1) / ((int64_t)threads * V));
+  int turn = 0;
+  for (int64_t row = blockIdx.x; row < p.rows; row += gridDim.x, turn ^= 1) {
+    float ss = 0.f;
     uint32_t mx = 0;
-    float unused = 0.f;
-    for (int64_t c = threadIdx.x; c < p.cols; c += kRowThreads) mx = max(mx, abs_bits(to_f32(x[c])));
-    block_sum_max<kRowThreads / 32>(unused, mx, red);
-    const QuantScale q = quant_scale(mx, 1.f);
-    for (int64_t c = threadIdx.x; c < p.cols; c += kRowThreads)
-      out[row * p.s_out + c] = (int8_t)quant_one(to_f32(x[c]), q);
-    if (threadIdx.x == 0) scale[row] = q.scale;
+    // (the sum may take x's place: a row that is read twice stores it the second time)
+    auto piece = [&](int j, float (&h)[V], bool keep) {
+      typename Row::Piece x, r;
+      const int64_t c = ((int64_t)j * threads + threadIdx.x) * V;
+      op.load(row, c, x, r);
+      op.take(row, c, x, r, h, ss, mx, keep);
+    };
+#pragma unroll 2
+    for (int j = 0; j < pieces; ++j) {
+      float h[V];
+      piece(j, h, CACHED);
+      if (CACHED) {
+#pragma unroll
+        for (int i = 0; i < V / 4; ++i)
+          held[(j * (V / 4) + i) * threads + threadIdx.x] = make_float4(h[4 * i], h[4 * i + 1], h[4 * i + 2], h[4 * i + 3]);
+      }
+    }
+    row_sum_max<!QUANT, Row::kInt8>(ss, mx, red[turn], threads >> 5);
+    const float rstd = op.rstd_of(ss);
+    const QuantScale q = quant_scale(mx, rstd);
+#pragma unroll 2
+    for (int j = 0; j < pieces; ++j) {
+      float h[V];
+      if (CACHED) {
+#pragma unroll
+        for (int i = 0; i < V / 4; ++i) {
+          const float4 f = held[(j * (V / 4) + i) * threads + threadIdx.x];
+          h[4 * i] = f.x;
+          h[4 * i + 1] = f.y;
+          h[4 * i + 2] = f.z;
+          h[4 * i + 3] = f.w;
+        }
+      } else {
+        piece(j, h, true);
+      }
+      op.give(row, ((int64_t)j * threads + threadIdx.x) * V, h, rstd, q);
+    }
+    if (threadIdx.x == 0) op.row_values(row, rstd, q);
   }
 }
 
-static dim3 row_grid(int64_t rows, int num_sms) {
-  const int64_t most = (int64_t)num_sms * 8;
-  return dim3((unsigned)(rows < most ? rows : most));
+// ---------------------------------------------------------------- backward
+
+// One piece of the backward pass; GRID as above
+template <typename T, typename G, bool GRID>
+struct NormBackRow {
+  static constexpr int V = 16 / (int)(sizeof(T) > sizeof(G) ? sizeof(T) : sizeof(G));
+  using PieceH = RowPiece<T, V>;
+  using PieceG = RowPiece<G, V>;
+  NormParams const &p;
+  NormGradPtrs const &a;
+  RowBounds bh, bd, bs;
+  bool w_grid;
+
+  __device__ __forceinline__ NormBackRow(NormParams const &p_, NormGradPtrs const &a_) : p(p_), a(a_) {
+    if (!GRID) {
+      bh = row_bounds(a.h, p.rows, p.cols, p.s_h, sizeof(T));
+      bd = row_bounds(a.dy, p.rows, p.cols, p.s_dy, sizeof(G));
+      bs = row_bounds(a.dsum, p.rows, p.cols, p.s_dsum, sizeof(G));
+    }
+    w_grid = GRID || row_vec_ok(a.w, 0, 1, p.dt_w == EIR_FP32 ? 4 : 2, V);
+  }
+  template <typename D>
+  __device__ __forceinline__ void get(RowPiece<D, V> &v, void const *base, int64_t stride, RowBounds const &b,
+                                      int64_t row, int64_t c) const {
+    D const *at = static_cast<D const *>(base) + row * stride;
+    if (!GRID) v.load_any(at, c, p.cols, b.begin, b.end);
+    else if (c < p.cols) v.template load<true>(at + c);
+    else v.zero();
+  }
+  __device__ __forceinline__ void load(int64_t row, int64_t c, PieceH &h, PieceG &dy) const {
+    get<T>(h, a.h, p.s_h, bh, row, c);
+    get<G>(dy, a.dy, p.s_dy, bd, row, c);
+  }
+  __device__ __forceinline__ void load_sum(int64_t row, int64_t c, PieceG &s) const {
+    if (a.dsum) get<G>(s, a.dsum, p.s_dsum, bs, row, c);
+  }
+  // g = w dy and u = h rstd of a piece
+  __device__ __forceinline__ void take(int64_t c, PieceH const &h, PieceG const &dy, float rstd, float (&g)[V],
+                                       float (&u)[V]) const {
+    float w[V];
+#pragma unroll
+    for (int e = 0; e < V; ++e) w[e] = 1.f;
+    if (a.w && c < p.cols) load_shared_any<V>(a.w, p.dt_w, c, p.cols, w_grid, w);
+#pragma unroll
+    for (int e = 0; e < V; ++e) {
+      u[e] = h.get(e) * rstd;
+      g[e] = w[e] * dy.get(e);
+    }
+  }
+  // dx = rstd (g - u mean(g u)) + dsum; every lane of a warp calls it
+  __device__ __forceinline__ void give(int64_t row, int64_t c, float const (&g)[V], float const (&u)[V],
+                                       PieceG const &s, float rstd, float mean) const {
+    float d[V];
+#pragma unroll
+    for (int e = 0; e < V; ++e) {
+      d[e] = rstd * (g[e] - u[e] * mean);
+      if (a.dsum) d[e] += s.get(e);
+    }
+    PieceG o;
+    o.set(d);
+    G *out = static_cast<G *>(a.dx) + row * p.s_dx;
+    if (!GRID) o.store_any(out, c, p.cols);
+    else if (c < p.cols) o.store(out + c);
+  }
+};
+
+// A row's threads hold h and dy between the two uses, and the weight gradient
+// of their columns over all rows that they see; it is written as one partial row a
+// block (a warp where a warp owns a row) and summed by norm_dweight_kernel: no
+// atomics, so the order is fixed.
+template <typename T, typename G, bool GRID>
+__global__ void __launch_bounds__(1024) norm_backward_kernel(const NormParams p, const NormGradPtrs a, int row_warps) {
+  using Row = NormBackRow<T, G, GRID>;
+  constexpr int V = Row::V, N = kPerBack<T, G> / V;
+  __shared__ uint32_t red[2][64];
+  pdl_launch_dependents();
+  pdl_wait();
+  const Row op(p, a);
+  const int threads = row_warps * 32, tid = row_warps == 1 ? threadIdx.x & 31 : threadIdx.x;
+  const int64_t rows_at_once = row_warps == 1 ? (int64_t)gridDim.x * (blockDim.x >> 5) : gridDim.x;
+  const int64_t first = row_warps == 1 ? (int64_t)blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5) : blockIdx.x;
+  auto column = [&](int j) { return (int64_t)(j * threads + tid) * V; };
+  typename Row::PieceH h[N];
+  typename Row::PieceG dy[N], ds[N];
+  float rstd = 0.f;
+  auto fetch = [&](int64_t r) {
+    rstd = a.rstd[r];
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+      op.load(r, column(j), h[j], dy[j]);
+      op.load_sum(r, column(j), ds[j]);
+    }
+  };
+  float dw[N][V];
+#pragma unroll
+  for (int j = 0; j < N; ++j)
+#pragma unroll
+    for (int e = 0; e < V; ++e) dw[j][e] = 0.f;
+  int64_t row = first;
+  if (GRID && row < p.rows) fetch(row);
+  for (int turn = 0; row < p.rows; row += rows_at_once, turn ^= 1) {
+    if (!GRID) fetch(row);
+    const float unit = rstd;
+    float g[N][V], u[N][V];
+    float gu = 0.f;
+    typename Row::PieceG s[N];
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+      op.take(column(j), h[j], dy[j], unit, g[j], u[j]);
+#pragma unroll
+      for (int e = 0; e < V; ++e) {
+        dw[j][e] += dy[j].get(e) * u[j][e];
+        gu += g[j][e] * u[j][e];
+      }
+      s[j] = ds[j];
+    }
+    if (GRID && row + rows_at_once < p.rows) fetch(row + rows_at_once);
+    uint32_t unused = 0;
+    row_sum_max<true, false>(gu, unused, red[turn], row_warps);
+    const float mean = gu / (float)p.cols;
+#pragma unroll
+    for (int j = 0; j < N; ++j) op.give(row, column(j), g[j], u[j], s[j], unit, mean);
+  }
+  if (a.part != nullptr) {
+    float *part = a.part + first * p.cols;
+#pragma unroll
+    for (int j = 0; j < N; ++j)
+#pragma unroll
+      for (int e = 0; e < V; ++e)
+        if (column(j) + e < p.cols) part[column(j) + e] = dw[j][e];
+  }
+}
+
+// wide rows: h and dy stay in shared memory as they were read, and so does the block's
+// weight gradient (CACHED); else h and dy are read again, and the weight gradient is added up in the
+// block's partial row (always by the same thread)
+template <typename T, typename G, bool CACHED>
+__global__ void __launch_bounds__(512) norm_backward_wide_kernel(const NormParams p, const NormGradPtrs a) {
+  using Row = NormBackRow<T, G, false>;
+  constexpr int V = Row::V;
+  __shared__ uint32_t red[2][64];
+  extern __shared__ uint32_t held_words[];  // pieces of h, pieces of dy, weight gradients: [piece][word][thread]
+  pdl_launch_dependents();
+  pdl_wait();
+  const Row op(p, a);
+  const int threads = blockDim.x, pieces = (int)((p.cols + (int64_t)threads * V - 1) / ((int64_t)threads * V));
+  uint32_t *held_h = held_words + threadIdx.x;
+  uint32_t *held_d = held_h + (int64_t)pieces * Row::PieceH::kWords * threads;
+  float *held_w = reinterpret_cast<float *>(held_d + (int64_t)pieces * Row::PieceG::kWords * threads);
+  float *part = a.part ? a.part + (int64_t)blockIdx.x * p.cols : nullptr;
+  auto column = [&](int j) { return ((int64_t)j * threads + threadIdx.x) * V; };
+  if (CACHED) {
+    for (int i = 0; i < pieces * V; ++i) held_w[i * threads] = 0.f;
+  }
+  int turn = 0;
+  for (int64_t row = blockIdx.x; row < p.rows; row += gridDim.x, turn ^= 1) {
+    const float rstd = a.rstd[row];
+    float gu = 0.f;
+#pragma unroll 2
+    for (int j = 0; j < pieces; ++j) {
+      typename Row::PieceH h;
+      typename Row::PieceG dy;
+      float g[V], u[V];
+      op.load(row, column(j), h, dy);
+      op.take(column(j), h, dy, rstd, g, u);
+#pragma unroll
+      for (int e = 0; e < V; ++e) gu += g[e] * u[e];
+      if (CACHED) {
+#pragma unroll
+        for (int i = 0; i < Row::PieceH::kWords; ++i) held_h[(j * Row::PieceH::kWords + i) * threads] = h.w[i];
+#pragma unroll
+        for (int i = 0; i < Row::PieceG::kWords; ++i) held_d[(j * Row::PieceG::kWords + i) * threads] = dy.w[i];
+      }
+    }
+    uint32_t unused = 0;
+    row_sum_max<true, false>(gu, unused, red[turn], threads >> 5);
+    const float mean = gu / (float)p.cols;
+#pragma unroll 2
+    for (int j = 0; j < pieces; ++j) {
+      const int64_t c = column(j);
+      typename Row::PieceH h;
+      typename Row::PieceG dy, s;
+      float g[V], u[V];
+      op.load_sum(row, c, s);
+      if (CACHED) {
+#pragma unroll
+        for (int i = 0; i < Row::PieceH::kWords; ++i) h.w[i] = held_h[(j * Row::PieceH::kWords + i) * threads];
+#pragma unroll
+        for (int i = 0; i < Row::PieceG::kWords; ++i) dy.w[i] = held_d[(j * Row::PieceG::kWords + i) * threads];
+      } else {
+        op.load(row, c, h, dy);
+      }
+      op.take(c, h, dy, rstd, g, u);
+      if (part) {
+#pragma unroll
+        for (int e = 0; e < V; ++e) {
+          const float d = dy.get(e) * u[e];
+          if (CACHED) held_w[(j * V + e) * threads] += d;
+          else if (c + e < p.cols) part[c + e] = (row == blockIdx.x ? 0.f : part[c + e]) + d;
+        }
+      }
+      op.give(row, c, g, u, s, rstd, mean);
+    }
+  }
+  if (CACHED && part) {
+    for (int j = 0; j < pieces; ++j)
+#pragma unroll
+      for (int e = 0; e < V; ++e)
+        if (column(j) + e < p.cols) part[column(j) + e] = held_w[(j * V + e) * threads];
+  }
+}
+
+// dw[c] = sum of the partial rows: 32 columns a block, thread row y adds the
+// rows y, y + 32, ..., and the 32 sums are added in order
+__global__ void __launch_bounds__(1024) norm_dweight_kernel(int64_t cols, float const *__restrict__ part,
+                                                            int64_t n_part, float *__restrict__ dw) {
+  __shared__ float sums[32][33];
+  pdl_launch_dependents();
+  pdl_wait();
+  const int x = threadIdx.x & 31, y = threadIdx.x >> 5;
+  const int64_t c = (int64_t)blockIdx.x * 32 + x;
+  float s = 0.f;
+  if (c < cols) {
+#pragma unroll 8
+    for (int64_t i = y; i < n_part; i += 32) s += part[i * cols + c];
+  }
+  sums[y][x] = s;
+  __syncthreads();
+  // the warp y adds column y's partial sums
+  s = warp_sum(sums[x][y]);
+  if (x == 0 && (int64_t)blockIdx.x * 32 + y < cols) dw[(int64_t)blockIdx.x * 32 + y] = s;
+}
+
+// ---------------------------------------------------------------- launchers
+
+// threads of a row in warps: one, or a power of two from 4 on
+static int row_warps(int64_t cols, int per) {
+  if (cols <= 32 * per) return 1;
+  int w = 4;
+  while (w < 32 && (int64_t)w * 32 * per < cols) w *= 2;
+  return w;
+}
+
+// block and grid: persistent blocks of up to 1024 threads an SM (64 registers a thread)
+struct RowGrid {
+  int warps;      // of a row
+  int threads;    // of a block
+  int64_t grid;
+  int64_t units;  // rows in flight: blocks, or warps
+};
+static RowGrid row_grid(int64_t rows, int64_t cols, int per, int num_sms) {
+  RowGrid g;
+  g.warps = row_warps(cols, per);
+  g.threads = g.warps == 1 ? 128 : g.warps * 32;
+  const int64_t blocks = g.warps == 1 ? (rows + 3) / 4 : rows;
+  g.grid = std::min<int64_t>(blocks, (int64_t)num_sms * (1024 / g.threads));
+  g.units = g.warps == 1 ? g.grid * 4 : g.grid;
+  return g;
+}
+
+constexpr int kSmemMost = 227 * 1024 - 1024;  // dynamic, beside the reductions' words
+
+// wide rows: threads of a block, bytes that it holds (0: the row is read twice), and the grid
+struct WideGrid {
+  int threads;
+  int64_t bytes;
+  int64_t grid;
+};
+static WideGrid wide_grid(int64_t rows, int64_t cols, int threads, int v, int per_col, int num_sms) {
+  WideGrid g;
+  g.threads = threads;
+  g.bytes = (cols + (int64_t)threads * v - 1) / ((int64_t)threads * v) * threads * v * per_col;
+  if (g.bytes > kSmemMost) g.bytes = 0;
+  const int64_t fit = g.bytes ? std::max<int64_t>(1, std::min<int64_t>(1024 / threads, kSmemMost / g.bytes)) : 1024 / threads;
+  g.grid = std::min<int64_t>(rows, num_sms * fit);
+  return g;
+}
+
+template <typename... KArgs, typename... Args>
+static cudaError_t launch_wide(void (*kern)(KArgs...), WideGrid const &g, cudaStream_t st, Args const &...args) {
+  if (g.bytes > 48 * 1024 - 1024) {
+    cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)g.bytes);
+    if (e != cudaSuccess) return e;
+  }
+  return launch_kernel(kern, dim3((unsigned)g.grid), dim3(g.threads), (size_t)g.bytes, st, args...);
+}
+
+template <typename T, typename OUT, bool QUANT>
+static cudaError_t launch_norm_out(NormParams const &p, NormPtrs const &a, int num_sms, cudaStream_t st) {
+  constexpr int V = 16 / sizeof(T);
+  if (p.cols > 1024 * kPer<T>) {
+    const WideGrid g = wide_grid(p.rows, p.cols, 1024, V, 4, num_sms);
+    return launch_wide(g.bytes ? norm_wide_kernel<T, OUT, QUANT, true> : norm_wide_kernel<T, OUT, QUANT, false>, g, st, p, a);
+  }
+  const bool grid = p.cols % V == 0 && row_vec_ok(a.x, p.s_x, p.rows, sizeof(T), V) &&
+                    row_vec_ok(a.res, p.s_res, p.rows, sizeof(T), V) &&
+                    row_vec_ok(a.sum, p.s_sum, p.rows, sizeof(T), V) &&
+                    row_vec_ok(a.out, p.s_out, p.rows, sizeof(OUT), V) &&
+                    row_vec_ok(a.w, 0, 1, p.dt_w == EIR_FP32 ? 4 : 2, V);
+  const RowGrid g = row_grid(p.rows, p.cols, kPer<T>, num_sms);
+  auto kern = grid ? norm_kernel<T, OUT, QUANT, true> : norm_kernel<T, OUT, QUANT, false>;
+  return launch_kernel(kern, dim3((unsigned)g.grid), dim3(g.threads), 0, st, p, a, g.warps);
+}
+
+template <typename T>
+static cudaError_t launch_norm_t(NormParams const &p, NormPtrs const &a, int num_sms, cudaStream_t st) {
+  if (p.dt_out == EIR_FP32) return launch_norm_out<T, float, false>(p, a, num_sms, st);
+  if (p.dt_out == EIR_BF16) return launch_norm_out<T, __nv_bfloat16, false>(p, a, num_sms, st);
+  return launch_norm_out<T, int8_t, false>(p, a, num_sms, st);
 }
 
 cudaError_t launch_norm(NormParams const &p, NormPtrs const &a, int num_sms, cudaStream_t st) {
-  auto kern = p.dt == EIR_FP32 ? norm_kernel<float> : norm_kernel<__nv_bfloat16>;
-  return launch_kernel(kern, row_grid(p.rows, num_sms), dim3(kRowThreads), 0, st, p, a);
-}
-
-int64_t norm_backward_ctas(NormParams const &p, int num_sms) { return row_grid(p.rows, num_sms).x; }
-
-cudaError_t launch_norm_backward(NormParams const &p, NormGradPtrs const &a, int num_sms, cudaStream_t st) {
-  auto kern = p.dt == EIR_FP32 ? norm_backward_kernel<float> : norm_backward_kernel<__nv_bfloat16>;
-  return launch_kernel(kern, row_grid(p.rows, num_sms), dim3(kRowThreads), 0, st, p, a);
-}
-
-cudaError_t launch_norm_dweight(NormParams const &p, float const *part, int64_t n_part, float *dw,
-                                cudaStream_t st) {
-  return launch_kernel(norm_dweight_kernel, dim3((unsigned)((p.cols + kRowThreads - 1) / kRowThreads)),
-                       dim3(kRowThreads), 0, st, p.cols, part, n_part, dw);
+  return p.dt == EIR_FP32 ? launch_norm_t<float>(p, a, num_sms, st) : launch_norm_t<__nv_bfloat16>(p, a, num_sms, st);
 }
 
 cudaError_t launch_quantize(QuantizeParams const &p, void const *x, int8_t *q, float *scale, int num_sms,
                             cudaStream_t st) {
-  auto kern = p.dt == EIR_FP32 ? quantize_kernel<float> : quantize_kernel<__nv_bfloat16>;
-  return launch_kernel(kern, row_grid(p.rows, num_sms), dim3(kRowThreads), 0, st, p, x, q, scale);
+  NormParams n;
+  n.rows = p.rows;
+  n.cols = p.cols;
+  n.dt = p.dt;
+  n.dt_out = EIR_INT8;
+  n.s_x = p.s_x;
+  n.s_out = p.s_out;
+  const NormPtrs a{x, nullptr, nullptr, nullptr, q, scale, nullptr};
+  return p.dt == EIR_FP32 ? launch_norm_out<float, int8_t, true>(n, a, num_sms, st)
+                          : launch_norm_out<__nv_bfloat16, int8_t, true>(n, a, num_sms, st);
+}
+
+// the backward kernel's grid and how many partial rows of the weight gradient it writes
+struct BackGrid {
+  bool wide;
+  RowGrid row;
+  WideGrid span;
+  int64_t parts;
+};
+static BackGrid back_grid(NormParams const &p, int num_sms) {
+  const int e = (p.dt == EIR_FP32 ? 4 : 2) + (p.dt_grad == EIR_FP32 ? 4 : 2);
+  const int per = e == 8 ? kPerBack<float, float> : kPerBack<__nv_bfloat16, __nv_bfloat16>;
+  BackGrid g{};
+  g.wide = p.cols > 1024 * per;
+  if (g.wide) {
+    g.span = wide_grid(p.rows, p.cols, 512, e == 4 ? 8 : 4, e + 4, num_sms);
+    g.parts = g.span.grid;
+  } else {
+    g.row = row_grid(p.rows, p.cols, per, num_sms);
+    g.parts = g.row.units;
+  }
+  return g;
+}
+
+int64_t norm_backward_parts(NormParams const &p, int num_sms) { return back_grid(p, num_sms).parts; }
+
+template <typename T, typename G>
+static cudaError_t launch_norm_backward_t(NormParams const &p, NormGradPtrs const &a, int num_sms, cudaStream_t st) {
+  constexpr int V = NormBackRow<T, G, false>::V;
+  const BackGrid g = back_grid(p, num_sms);
+  if (g.wide)
+    return launch_wide(g.span.bytes ? norm_backward_wide_kernel<T, G, true> : norm_backward_wide_kernel<T, G, false>,
+                       g.span, st, p, a);
+  const bool grid = p.cols % V == 0 && row_vec_ok(a.h, p.s_h, p.rows, sizeof(T), V) &&
+                    row_vec_ok(a.dy, p.s_dy, p.rows, sizeof(G), V) &&
+                    row_vec_ok(a.dsum, p.s_dsum, p.rows, sizeof(G), V) &&
+                    row_vec_ok(a.dx, p.s_dx, p.rows, sizeof(G), V) &&
+                    row_vec_ok(a.w, 0, 1, p.dt_w == EIR_FP32 ? 4 : 2, V);
+  auto kern = grid ? norm_backward_kernel<T, G, true> : norm_backward_kernel<T, G, false>;
+  return launch_kernel(kern, dim3((unsigned)g.row.grid), dim3(g.row.threads), 0, st, p, a, g.row.warps);
+}
+
+cudaError_t launch_norm_backward(NormParams const &p, NormGradPtrs const &a, int num_sms, cudaStream_t st) {
+  if (p.dt == EIR_FP32)
+    return p.dt_grad == EIR_FP32 ? launch_norm_backward_t<float, float>(p, a, num_sms, st)
+                                 : launch_norm_backward_t<float, __nv_bfloat16>(p, a, num_sms, st);
+  return p.dt_grad == EIR_FP32 ? launch_norm_backward_t<__nv_bfloat16, float>(p, a, num_sms, st)
+                               : launch_norm_backward_t<__nv_bfloat16, __nv_bfloat16>(p, a, num_sms, st);
+}
+
+cudaError_t launch_norm_dweight(NormParams const &p, float const *part, int64_t n_part, float *dw,
+                                cudaStream_t st) {
+  return launch_kernel(norm_dweight_kernel, dim3((unsigned)((p.cols + 31) / 32)), dim3(1024), 0, st, p.cols, part,
+                       n_part, dw);
 }
 
 }  // namespace eir

@@ -42,29 +42,6 @@ __device__ __forceinline__ float warp_sum(float v) {
 // that an integer maximum carries a NaN through
 __device__ __forceinline__ uint32_t abs_bits(float v) { return __float_as_uint(v) & 0x7fffffffu; }
 
-// sum of v and maximum of m over the block; every thread gets both. `red`: 2 x 32 words
-template <int WARPS>
-__device__ __forceinline__ void block_sum_max(float &v, uint32_t &m, uint32_t *red) {
-  v = warp_sum(v);
-  m = __reduce_max_sync(0xffffffffu, m);
-  if (WARPS == 1) return;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  __syncthreads();  // `red` may hold an earlier result
-  if (lane == 0) {
-    red[warp] = __float_as_uint(v);
-    red[32 + warp] = m;
-  }
-  __syncthreads();
-  float s = 0.f;
-  uint32_t t = 0;
-  if (lane < WARPS) {
-    s = __uint_as_float(red[lane]);
-    t = red[32 + lane];
-  }
-  v = warp_sum(s);
-  m = __reduce_max_sync(0xffffffffu, t);
-}
-
 // A row's 8-bit scaling from the bits of its largest magnitude: the factor
 // 127 / m of round(v * factor), and the scale m * unit / 127 of the integers.
 struct QuantScale {

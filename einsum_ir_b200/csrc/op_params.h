@@ -77,8 +77,8 @@ struct LogprobGradPtrs {
 };
 
 cudaError_t launch_norm(NormParams const &p, NormPtrs const &a, int num_sms, cudaStream_t st);
-// CTAs of the backward kernel, and so partial rows of the weight gradient
-int64_t norm_backward_ctas(NormParams const &p, int num_sms);
+// partial rows of the weight gradient that the backward kernel writes
+int64_t norm_backward_parts(NormParams const &p, int num_sms);
 cudaError_t launch_norm_backward(NormParams const &p, NormGradPtrs const &a, int num_sms, cudaStream_t st);
 cudaError_t launch_norm_dweight(NormParams const &p, float const *part, int64_t n_part, float *dw,
                                 cudaStream_t st);

@@ -118,6 +118,38 @@ def test_norm_in_place_sum(cuda, cols):
         assert torch.equal(q, quantized32(h)[0])
 
 
+@pytest.mark.parametrize("offset", [0, 1])
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("rows,cols", [(3, 8200), (300, 8193), (2, 57345), (5, 65537), (150, 70000)])
+def test_norm_wide_rows(cuda, rows, cols, dtype, offset):
+    """rows held in shared memory and rows read twice, in place and not, and their backward pass"""
+    g = gen(rows + cols)
+    w = rows_of(g, 1, cols, BF16)[0]
+    for which in range(3):
+        x, res = rows_of(g, rows, cols, dtype, 0, offset), rows_of(g, rows, cols, dtype, 0, offset)
+        want = norm64(x, res, w, 1e-5)
+        h = x.float() + res.float()
+        s = (torch.empty_like(x), x, res)[which]
+        q, scale, rstd = (torch.empty((rows, cols), device="cuda", dtype=torch.int8), torch.empty(rows, device="cuda"),
+                          torch.empty(rows, device="cuda"))
+        op.NormPlan(rows, cols, CODE[dtype], dtype_weight=cabi.BF16, dtype_out=cabi.INT8, eps=1e-5).norm(
+            x, q, weight=w, residual=res, sum=s, scale=scale, rstd=rstd)
+        assert torch.equal(s, h.to(dtype))
+        assert torch.equal(q, quantized32(h * w.float())[0])
+        close(rstd, want["rstd"], want["rstd"] * (cols / 32 + 16) * U)
+        dy = rows_of(g, rows, cols, dtype, 0, offset)
+        dx, dw = torch.empty_like(dy), torch.empty(cols, device="cuda")
+        back = dy.clone() if which else dy
+        op.NormPlan(rows, cols, CODE[dtype], dtype_weight=cabi.BF16).backward(
+            back, s, rstd, back if which else dx, weight=w, dsum=dy, dweight=dw)
+        got = back if which else dx
+        want_x, want_w = norm_backward64(dy, s, w, rstd, dy)
+        r, gd, hd = rstd.double()[:, None], (dy.double() * w.double()).abs(), s.double().abs()
+        parts = r * (gd + hd * r.square() * (gd * hd).mean(1, keepdim=True)) + dy.double().abs()
+        close(got, want_x, parts * ((cols / 32 + 16) * U) + round_tol(want_x, dtype))
+        close(dw, want_w, (dy.double() * hd * r).abs().sum(0) * ((rows + 16) * U))
+
+
 @pytest.mark.parametrize("cols", [48, 4096, 20001])
 def test_norm_special_rows(cuda, cols):
     """zeros, tiny values, infinities and NaN, each in a row of its own"""

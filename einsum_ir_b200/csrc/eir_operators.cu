@@ -213,7 +213,7 @@ int eir_norm_backward(eir_plan *p, void const *dy, void const *h, void const *we
   if (rc != EIR_SUCCESS) return rc;
   num_sms = std::min(num_sms, eir::kMaxSms);
   eir::NormGradPtrs a{dy, h, weight, dsum, rstd, dx, dweight, nullptr};
-  const int64_t parts = eir::norm_backward_parts(n, num_sms);
+  int64_t parts = 0;
   if (dweight != nullptr) {
     void *ws = nullptr;
     rc = workspace(p, &ws);
@@ -222,7 +222,7 @@ int eir_norm_backward(eir_plan *p, void const *dy, void const *h, void const *we
   }
   {
     ProfScope prof(p, st);
-    rc = launched(eir::launch_norm_backward(n, a, num_sms, st), "norm backward launch");
+    rc = launched(eir::launch_norm_backward(n, a, err, num_sms, st, &parts), "norm backward launch");
   }
   if (rc != EIR_SUCCESS || dweight == nullptr) return rc;
   return launched(eir::launch_norm_dweight(n, a.part, parts, dweight, st), "norm weight gradient launch");

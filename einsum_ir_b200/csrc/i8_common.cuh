@@ -14,18 +14,7 @@ __device__ __forceinline__ float i8_scaled(int32_t acc, float sa, float sb, floa
 }
 // two of them in packed FP32 arithmetic (the same roundings)
 __device__ __forceinline__ float2 scaled2(int32_t a0, int32_t a1, float2 sa, float sb, float bias) {
-  float2 z;
-  asm("{\n\t.reg .b64 s, b, a, f, r;\n\t"
-      "mov.b64 s, {%4, %5};\n\t"
-      "mov.b64 b, {%6, %6};\n\t"
-      "mul.rn.f32x2 f, s, b;\n\t"
-      "mov.b64 a, {%2, %3};\n\t"
-      "mov.b64 b, {%7, %7};\n\t"
-      "fma.rn.f32x2 r, a, f, b;\n\t"
-      "mov.b64 {%0, %1}, r;\n\t}"
-      : "=f"(z.x), "=f"(z.y)
-      : "f"((float)a0), "f"((float)a1), "f"(sa.x), "f"(sa.y), "f"(sb), "f"(bias));
-  return z;
+  return fma2(make_float2((float)a0, (float)a1), mul2(sa, make_float2(sb, sb)), make_float2(bias, bias));
 }
 // silu(z) = z / (1 + e^-z) with the hardware's exponential and reciprocal: off
 // by about (|z| + 4) 2^-24 of itself, under the rounding of the sum that gave z

@@ -5,7 +5,8 @@
 // y = h rstd w. With 8-bit output v = h w, m = max|v|: y / s = v 127 / m for
 // s = m rstd / 127, so the integers need no rstd and the row's two statistics
 // (sum of squares, maximum) come from one pass. Backward: g = w dy,
-// dx = rstd (g - h rstd^2 mean(g h)) + dsum, dw = sum over rows of dy h rstd.
+// dx = rstd (g - h rstd^2 mean(g h)) + dsum, dw = sum over rows of dy h rstd
+// (computed with dy rstd in place of dy, which saves a product an element).
 // Sums are held in FP32.
 //
 // All three are bound by HBM. A row stays on the SM between the statistics and
@@ -24,8 +25,8 @@ namespace eir {
 
 // elements of a thread whose row stays in registers: FP32 rows take twice the
 // registers an element
-template <typename T>
-constexpr int kPer = sizeof(T) == 4 ? 8 : 16;  // norm and quantize
+template <typename T, bool QUANT>
+constexpr int kPer = (sizeof(T) == 4 ? 8 : 16) * (QUANT ? 2 : 1);  // norm; quantize
 template <typename T, typename G>
 constexpr int kPerBack = sizeof(T) + sizeof(G) == 8 ? 4 : 8;  // backward
 
@@ -146,7 +147,7 @@ struct NormRow {
 template <typename T, typename OUT, bool QUANT, bool GRID>
 __global__ void __launch_bounds__(1024) norm_kernel(const NormParams p, const NormPtrs a, int row_warps) {
   using Row = NormRow<T, OUT, QUANT, GRID>;
-  constexpr int V = Row::V, N = kPer<T> / V;
+  constexpr int V = Row::V, N = kPer<T, QUANT> / V;
   __shared__ uint32_t red[2][64];
   pdl_launch_dependents();
   pdl_wait();
@@ -163,17 +164,28 @@ __global__ void __launch_bounds__(1024) norm_kernel(const NormParams p, const No
   if (GRID && row < p.rows) fetch(row);
   for (int turn = 0; row < p.rows; row += rows_at_once, turn ^= 1) {
     if (!GRID) fetch(row);
-    float h[N][V];
+    // norm holds the row as h; quantize as it was read, in half the registers or the same
+    float h[QUANT ? 1 : N][V];
+    typename Row::Piece held[QUANT ? N : 1];
     float ss = 0.f;
     uint32_t mx = 0;
 #pragma unroll
-    for (int j = 0; j < N; ++j) op.take(row, column(j), x[j], r[j], h[j], ss, mx);
+    for (int j = 0; j < N; ++j) {
+      op.take(row, column(j), x[j], r[j], h[QUANT ? 0 : j], ss, mx);
+      if (QUANT) held[j] = x[j];
+    }
     if (GRID && row + rows_at_once < p.rows) fetch(row + rows_at_once);
     row_sum_max<!QUANT, Row::kInt8>(ss, mx, red[turn], row_warps);
     const float rstd = op.rstd_of(ss);
     const QuantScale q = quant_scale(mx, rstd);
 #pragma unroll
-    for (int j = 0; j < N; ++j) op.give(row, column(j), h[j], rstd, q);
+    for (int j = 0; j < N; ++j) {
+      if (QUANT) {
+#pragma unroll
+        for (int e = 0; e < V; ++e) h[0][e] = held[j].get(e);
+      }
+      op.give(row, column(j), h[QUANT ? 0 : j], rstd, q);
+    }
     if (tid == 0) op.row_values(row, rstd, q);
   }
 }
@@ -270,27 +282,43 @@ struct NormBackRow {
   __device__ __forceinline__ void load_sum(int64_t row, int64_t c, PieceG &s) const {
     if (a.dsum) get<G>(s, a.dsum, p.s_dsum, bs, row, c);
   }
-  // g = w dy and u = h rstd of a piece
-  __device__ __forceinline__ void take(int64_t c, PieceH const &h, PieceG const &dy, float rstd, float (&g)[V],
-                                       float (&u)[V]) const {
-    float w[V];
+  // With e = dy rstd and g = w e: held = g + dsum, and the piece's part of sum g h
+  // (GH) and of the weight gradients e h (DW)
+  __device__ __forceinline__ void weight(int64_t c, float (&w)[V]) const {
 #pragma unroll
     for (int e = 0; e < V; ++e) w[e] = 1.f;
     if (a.w && c < p.cols) load_shared_any<V>(a.w, p.dt_w, c, p.cols, w_grid, w);
-#pragma unroll
-    for (int e = 0; e < V; ++e) {
-      u[e] = h.get(e) * rstd;
-      g[e] = w[e] * dy.get(e);
-    }
   }
-  // dx = rstd (g - u mean(g u)) + dsum; every lane of a warp calls it
-  __device__ __forceinline__ void give(int64_t row, int64_t c, float const (&g)[V], float const (&u)[V],
-                                       PieceG const &s, float rstd, float mean) const {
+  template <bool GH, bool DW>
+  __device__ __forceinline__ void take(float const (&w)[V], PieceH const &h, PieceG const &dy, PieceG const &s,
+                                       float rstd, float (&held)[V], float &gh, float (&dw)[V]) const {
+    float2 sum = make_float2(0.f, 0.f);
+#pragma unroll
+    for (int e = 0; e < V; e += 2) {
+      const float2 hv = h.get2(e), d = mul2(dy.get2(e), make_float2(rstd, rstd));
+      float2 g = mul2(make_float2(w[e], w[e + 1]), d);
+      if (GH) sum = fma2(g, hv, sum);
+      if (DW) {
+        const float2 t = fma2(d, hv, make_float2(dw[e], dw[e + 1]));
+        dw[e] = t.x;
+        dw[e + 1] = t.y;
+      }
+      if (a.dsum) g = add2(g, s.get2(e));
+      held[e] = g.x;
+      held[e + 1] = g.y;
+    }
+    if (GH) gh += sum.x + sum.y;
+  }
+  // the factor of h in dx = g - h rstd^2 mean(g h) + dsum
+  __device__ __forceinline__ float factor(float rstd, float gh) const { return rstd * rstd * (gh / (float)p.cols); }
+  // every lane of a warp calls it
+  __device__ __forceinline__ void give(int64_t row, int64_t c, float const (&held)[V], PieceH const &h, float k) const {
     float d[V];
 #pragma unroll
-    for (int e = 0; e < V; ++e) {
-      d[e] = rstd * (g[e] - u[e] * mean);
-      if (a.dsum) d[e] += s.get(e);
+    for (int e = 0; e < V; e += 2) {
+      const float2 t = fma2(h.get2(e), make_float2(-k, -k), make_float2(held[e], held[e + 1]));
+      d[e] = t.x;
+      d[e + 1] = t.y;
     }
     PieceG o;
     o.set(d);
@@ -337,27 +365,24 @@ __global__ void __launch_bounds__(1024) norm_backward_kernel(const NormParams p,
   for (int turn = 0; row < p.rows; row += rows_at_once, turn ^= 1) {
     if (!GRID) fetch(row);
     const float unit = rstd;
-    float g[N][V], u[N][V];
-    float gu = 0.f;
-    typename Row::PieceG s[N];
+    float held[N][V];
+    typename Row::PieceH hr[N];
+    float gh = 0.f;
 #pragma unroll
     for (int j = 0; j < N; ++j) {
-      op.take(column(j), h[j], dy[j], unit, g[j], u[j]);
-#pragma unroll
-      for (int e = 0; e < V; ++e) {
-        dw[j][e] += dy[j].get(e) * u[j][e];
-        gu += g[j][e] * u[j][e];
-      }
-      s[j] = ds[j];
+      float w[V];
+      op.weight(column(j), w);
+      op.template take<true, true>(w, h[j], dy[j], ds[j], unit, held[j], gh, dw[j]);
+      hr[j] = h[j];
     }
     if (GRID && row + rows_at_once < p.rows) fetch(row + rows_at_once);
     uint32_t unused = 0;
-    row_sum_max<true, false>(gu, unused, red[turn], row_warps);
-    const float mean = gu / (float)p.cols;
+    row_sum_max<true, false>(gh, unused, red[turn], row_warps);
+    const float k = op.factor(unit, gh);
 #pragma unroll
-    for (int j = 0; j < N; ++j) op.give(row, column(j), g[j], u[j], s[j], unit, mean);
+    for (int j = 0; j < N; ++j) op.give(row, column(j), held[j], hr[j], k);
   }
-  if (a.part != nullptr) {
+  if (a.part != nullptr && first < p.rows) {
     float *part = a.part + first * p.cols;
 #pragma unroll
     for (int j = 0; j < N; ++j)
@@ -367,22 +392,141 @@ __global__ void __launch_bounds__(1024) norm_backward_kernel(const NormParams p,
   }
 }
 
-// wide rows: h and dy stay in shared memory as they were read, and so does the block's
-// weight gradient (CACHED); else h and dy are read again, and the weight gradient is added up in the
-// block's partial row (always by the same thread)
+// Rows on the pieces' grid, wider than a warp: whole rows of h, dy and dsum are
+// copied (cp.async.bulk) into a ring of stages in shared memory, so that the bytes in flight do
+// not depend on the registers of the threads that work on a row. The barrier of the row's sum
+// says that its stage has been read; one thread then refills it. N: pieces of a
+// thread.
+constexpr int kBackThreads = 512;  // of a block, at most
+// blocks an SM of that many threads, by a thread's elements
+__host__ __device__ constexpr int back_blocks(int per) { return per > 8 ? 1 : 2; }
+struct BackRing {
+  int threads;
+  int stages;
+  int64_t stage_bytes;
+};
+
+__device__ __forceinline__ void bulk_load(void *dst, void const *src, uint32_t bytes, uint64_t *bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
+                   smem_u32(dst)),
+               "l"(src), "r"(bytes), "r"(smem_u32(bar))
+               : "memory");
+}
+
+template <typename T, typename G, int N>
+__global__ void __launch_bounds__(kBackThreads, back_blocks(N * NormBackRow<T, G, true>::V))
+    norm_backward_ring_kernel(const NormParams p, const NormGradPtrs a, const BackRing ring, uint32_t *err) {
+  using Row = NormBackRow<T, G, true>;
+  constexpr int V = Row::V, kMostStages = 8;
+  extern __shared__ __align__(128) uint8_t stages[];
+  __shared__ uint32_t red[2][64];
+  __shared__ uint64_t full[kMostStages];
+  __shared__ int never;  // the bounded waits' abort word: a block's threads tell one another through `red`
+  const int warps = ring.threads >> 5, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < ring.stages; ++s) mbar_init(&full[s], 1);
+    never = 0;
+    fence_barrier_init();
+  }
+  __syncthreads();
+  pdl_launch_dependents();
+  pdl_wait();
+  const uint32_t bytes_h = (uint32_t)(p.cols * sizeof(T)), bytes_g = (uint32_t)(p.cols * sizeof(G));
+  auto copy_row = [&](int64_t row, int stage) {
+    uint8_t *to = stages + stage * ring.stage_bytes;
+    mbar_arrive_expect_tx(&full[stage], bytes_h + bytes_g * (a.dsum ? 2 : 1));
+    bulk_load(to, static_cast<T const *>(a.h) + row * p.s_h, bytes_h, &full[stage]);
+    bulk_load(to + bytes_h, static_cast<G const *>(a.dy) + row * p.s_dy, bytes_g, &full[stage]);
+    if (a.dsum)
+      bulk_load(to + bytes_h + bytes_g, static_cast<G const *>(a.dsum) + row * p.s_dsum, bytes_g, &full[stage]);
+  };
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < ring.stages; ++s)
+      if (blockIdx.x + (int64_t)s * gridDim.x < p.rows) copy_row(blockIdx.x + (int64_t)s * gridDim.x, s);
+  }
+  const Row op(p, a);
+  const float inv_cols = 1.f / (float)p.cols;
+  auto column = [&](int j) { return (j * ring.threads + (int)threadIdx.x) * V; };
+  float dw[N][V];
+#pragma unroll
+  for (int j = 0; j < N; ++j)
+#pragma unroll
+    for (int e = 0; e < V; ++e) dw[j][e] = 0.f;
+  int stage = 0, turn = 0;
+  uint32_t phase = 0;
+  float next = a.rstd[blockIdx.x];
+  for (int64_t row = blockIdx.x; row < p.rows; row += gridDim.x, turn ^= 1) {
+    const float unit = next;
+    if (row + gridDim.x < p.rows) next = a.rstd[row + gridDim.x];
+    const bool late = !mbar_wait_bounded(&full[stage], phase, &never);
+    uint8_t const *at = stages + stage * ring.stage_bytes;
+    float held[N][V];
+    typename Row::PieceH h[N];
+    float gh = 0.f;
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+      const int c = column(j);
+      typename Row::PieceG dy, s;
+      if (c >= p.cols) continue;
+      float w[V];
+      op.weight(c, w);
+      h[j].template load<false>(at + c * sizeof(T));
+      dy.template load<false>(at + bytes_h + c * sizeof(G));
+      if (a.dsum) s.template load<false>(at + bytes_h + bytes_g + c * sizeof(G));
+      op.template take<true, true>(w, h[j], dy, s, unit, held[j], gh, dw[j]);
+    }
+    gh = warp_sum(gh);
+    const bool warp_late = __any_sync(0xffffffffu, late);
+    if (lane == 0) {
+      red[turn][warp] = __float_as_uint(gh);
+      red[turn][32 + warp] = warp_late;
+    }
+    __syncthreads();
+    // all threads leave together where a wait has given up
+    if (__any_sync(0xffffffffu, lane < warps && red[turn][32 + lane] != 0)) {
+      if (threadIdx.x == 0) {
+        record_error(err, kErrTimeoutProducer);
+        for (int i = 0; i < 1000; ++i) __nanosleep(1000);  // copies under way land before the block ends
+      }
+      break;
+    }
+    if (threadIdx.x == 0 && row + (int64_t)ring.stages * gridDim.x < p.rows)
+      copy_row(row + (int64_t)ring.stages * gridDim.x, stage);
+    gh = warp_sum(lane < warps ? __uint_as_float(red[turn][lane]) : 0.f);
+    const float k = unit * unit * (gh * inv_cols);
+#pragma unroll
+    for (int j = 0; j < N; ++j) op.give(row, column(j), held[j], h[j], k);
+    if (++stage == ring.stages) {
+      stage = 0;
+      phase ^= 1u;
+    }
+  }
+  if (a.part != nullptr) {
+    float *part = a.part + (int64_t)blockIdx.x * p.cols;
+#pragma unroll
+    for (int j = 0; j < N; ++j)
+#pragma unroll
+      for (int e = 0; e < V; ++e)
+        if (column(j) + e < p.cols) part[column(j) + e] = dw[j][e];
+  }
+}
+
+// wide rows: h, g + dsum and the block's weight gradient stay in shared memory
+// (CACHED); else the row is read again, and the weight gradient is added up in the block's
+// partial row (always by the same thread)
 template <typename T, typename G, bool CACHED>
 __global__ void __launch_bounds__(512) norm_backward_wide_kernel(const NormParams p, const NormGradPtrs a) {
   using Row = NormBackRow<T, G, false>;
-  constexpr int V = Row::V;
+  constexpr int V = Row::V, W = Row::PieceH::kWords;
   __shared__ uint32_t red[2][64];
-  extern __shared__ uint32_t held_words[];  // pieces of h, pieces of dy, weight gradients: [piece][word][thread]
+  extern __shared__ uint32_t held_words[];  // h as read, g + dsum, weight gradients: [piece][word][thread]
   pdl_launch_dependents();
   pdl_wait();
   const Row op(p, a);
   const int threads = blockDim.x, pieces = (int)((p.cols + (int64_t)threads * V - 1) / ((int64_t)threads * V));
   uint32_t *held_h = held_words + threadIdx.x;
-  uint32_t *held_d = held_h + (int64_t)pieces * Row::PieceH::kWords * threads;
-  float *held_w = reinterpret_cast<float *>(held_d + (int64_t)pieces * Row::PieceG::kWords * threads);
+  float *held_g = reinterpret_cast<float *>(held_h + pieces * W * threads);
+  float *held_w = held_g + pieces * V * threads;
   float *part = a.part ? a.part + (int64_t)blockIdx.x * p.cols : nullptr;
   auto column = [&](int j) { return ((int64_t)j * threads + threadIdx.x) * V; };
   if (CACHED) {
@@ -391,51 +535,60 @@ __global__ void __launch_bounds__(512) norm_backward_wide_kernel(const NormParam
   int turn = 0;
   for (int64_t row = blockIdx.x; row < p.rows; row += gridDim.x, turn ^= 1) {
     const float rstd = a.rstd[row];
-    float gu = 0.f;
+    float gh = 0.f;
 #pragma unroll 2
     for (int j = 0; j < pieces; ++j) {
       typename Row::PieceH h;
-      typename Row::PieceG dy;
-      float g[V], u[V];
+      typename Row::PieceG dy, s;
+      float g[V], dw[V];
       op.load(row, column(j), h, dy);
-      op.take(column(j), h, dy, rstd, g, u);
+      if (CACHED) {
+        op.load_sum(row, column(j), s);
 #pragma unroll
-      for (int e = 0; e < V; ++e) gu += g[e] * u[e];
+        for (int e = 0; e < V; ++e) dw[e] = held_w[(j * V + e) * threads];
+      }
+      float w[V];
+      op.weight(column(j), w);
+      op.template take<true, CACHED>(w, h, dy, s, rstd, g, gh, dw);
       if (CACHED) {
 #pragma unroll
-        for (int i = 0; i < Row::PieceH::kWords; ++i) held_h[(j * Row::PieceH::kWords + i) * threads] = h.w[i];
+        for (int e = 0; e < V; ++e) held_w[(j * V + e) * threads] = dw[e];
 #pragma unroll
-        for (int i = 0; i < Row::PieceG::kWords; ++i) held_d[(j * Row::PieceG::kWords + i) * threads] = dy.w[i];
+        for (int i = 0; i < W; ++i) held_h[(j * W + i) * threads] = h.w[i];
+#pragma unroll
+        for (int e = 0; e < V; ++e) held_g[(j * V + e) * threads] = g[e];
       }
     }
     uint32_t unused = 0;
-    row_sum_max<true, false>(gu, unused, red[turn], threads >> 5);
-    const float mean = gu / (float)p.cols;
+    row_sum_max<true, false>(gh, unused, red[turn], threads >> 5);
+    const float k = op.factor(rstd, gh);
 #pragma unroll 2
     for (int j = 0; j < pieces; ++j) {
       const int64_t c = column(j);
       typename Row::PieceH h;
-      typename Row::PieceG dy, s;
-      float g[V], u[V];
-      op.load_sum(row, c, s);
+      float g[V];
       if (CACHED) {
 #pragma unroll
-        for (int i = 0; i < Row::PieceH::kWords; ++i) h.w[i] = held_h[(j * Row::PieceH::kWords + i) * threads];
+        for (int i = 0; i < W; ++i) h.w[i] = held_h[(j * W + i) * threads];
 #pragma unroll
-        for (int i = 0; i < Row::PieceG::kWords; ++i) dy.w[i] = held_d[(j * Row::PieceG::kWords + i) * threads];
+        for (int e = 0; e < V; ++e) g[e] = held_g[(j * V + e) * threads];
       } else {
+        typename Row::PieceG dy, s;
+        float dw[V], again = 0.f;
         op.load(row, c, h, dy);
-      }
-      op.take(c, h, dy, rstd, g, u);
-      if (part) {
+        op.load_sum(row, c, s);
 #pragma unroll
-        for (int e = 0; e < V; ++e) {
-          const float d = dy.get(e) * u[e];
-          if (CACHED) held_w[(j * V + e) * threads] += d;
-          else if (c + e < p.cols) part[c + e] = (row == blockIdx.x ? 0.f : part[c + e]) + d;
+        for (int e = 0; e < V; ++e) dw[e] = part && row != blockIdx.x && c + e < p.cols ? part[c + e] : 0.f;
+        float w[V];
+        op.weight(c, w);
+        op.template take<false, true>(w, h, dy, s, rstd, g, again, dw);
+        if (part) {
+#pragma unroll
+          for (int e = 0; e < V; ++e)
+            if (c + e < p.cols) part[c + e] = dw[e];
         }
       }
-      op.give(row, c, g, u, s, rstd, mean);
+      op.give(row, c, g, h, k);
     }
   }
   if (CACHED && part) {
@@ -469,13 +622,8 @@ __global__ void __launch_bounds__(1024) norm_dweight_kernel(int64_t cols, float 
 
 // ---------------------------------------------------------------- launchers
 
-// threads of a row in warps: one, or a power of two from 4 on
-static int row_warps(int64_t cols, int per) {
-  if (cols <= 32 * per) return 1;
-  int w = 4;
-  while (w < 32 && (int64_t)w * 32 * per < cols) w *= 2;
-  return w;
-}
+// warps of a row
+static int row_warps(int64_t cols, int per) { return (int)((cols + 32 * per - 1) / (32 * per)); }
 
 // block and grid: persistent blocks of up to 1024 threads an SM (64 registers a thread)
 struct RowGrid {
@@ -524,7 +672,7 @@ static cudaError_t launch_wide(void (*kern)(KArgs...), WideGrid const &g, cudaSt
 template <typename T, typename OUT, bool QUANT>
 static cudaError_t launch_norm_out(NormParams const &p, NormPtrs const &a, int num_sms, cudaStream_t st) {
   constexpr int V = 16 / sizeof(T);
-  if (p.cols > 1024 * kPer<T>) {
+  if (p.cols > 1024 * kPer<T, QUANT>) {
     const WideGrid g = wide_grid(p.rows, p.cols, 1024, V, 4, num_sms);
     return launch_wide(g.bytes ? norm_wide_kernel<T, OUT, QUANT, true> : norm_wide_kernel<T, OUT, QUANT, false>, g, st, p, a);
   }
@@ -533,7 +681,7 @@ static cudaError_t launch_norm_out(NormParams const &p, NormPtrs const &a, int n
                     row_vec_ok(a.sum, p.s_sum, p.rows, sizeof(T), V) &&
                     row_vec_ok(a.out, p.s_out, p.rows, sizeof(OUT), V) &&
                     row_vec_ok(a.w, 0, 1, p.dt_w == EIR_FP32 ? 4 : 2, V);
-  const RowGrid g = row_grid(p.rows, p.cols, kPer<T>, num_sms);
+  const RowGrid g = row_grid(p.rows, p.cols, kPer<T, QUANT>, num_sms);
   auto kern = grid ? norm_kernel<T, OUT, QUANT, true> : norm_kernel<T, OUT, QUANT, false>;
   return launch_kernel(kern, dim3((unsigned)g.grid), dim3(g.threads), 0, st, p, a, g.warps);
 }
@@ -563,52 +711,72 @@ cudaError_t launch_quantize(QuantizeParams const &p, void const *x, int8_t *q, f
                           : launch_norm_out<__nv_bfloat16, int8_t, true>(n, a, num_sms, st);
 }
 
-// the backward kernel's grid and how many partial rows of the weight gradient it writes
-struct BackGrid {
-  bool wide;
-  RowGrid row;
-  WideGrid span;
-  int64_t parts;
-};
-static BackGrid back_grid(NormParams const &p, int num_sms) {
-  const int e = (p.dt == EIR_FP32 ? 4 : 2) + (p.dt_grad == EIR_FP32 ? 4 : 2);
-  const int per = e == 8 ? kPerBack<float, float> : kPerBack<__nv_bfloat16, __nv_bfloat16>;
-  BackGrid g{};
-  g.wide = p.cols > 1024 * per;
-  if (g.wide) {
-    g.span = wide_grid(p.rows, p.cols, 512, e == 4 ? 8 : 4, e + 4, num_sms);
-    g.parts = g.span.grid;
-  } else {
-    g.row = row_grid(p.rows, p.cols, per, num_sms);
-    g.parts = g.row.units;
-  }
-  return g;
+// Backward: the ring takes rows on the pieces' grid that are wider than a warp and of
+// which two stages fit; *per: elements of a thread in a row
+static bool back_ring(NormParams const &p, int row_bytes, int num_sms, BackRing *r, int *per, int64_t *grid) {
+  if (p.cols <= 32 * 8 || p.rows < 2) return false;
+  *per = p.cols <= kBackThreads * 8 ? 8 : 16;
+  r->threads = (int)((p.cols + *per - 1) / *per + 31) / 32 * 32;
+  if (r->threads > kBackThreads) return false;
+  r->stage_bytes = (p.cols * row_bytes + 127) / 128 * 128;
+  int64_t blocks = std::min(8, back_blocks(*per) * kBackThreads / r->threads);
+  while (blocks > 1 && (2 * r->stage_bytes + 2048) * blocks > kSmemMost) --blocks;
+  r->stages = (int)std::min<int64_t>(8, (kSmemMost / blocks - 2048) / r->stage_bytes);
+  *grid = std::min<int64_t>(p.rows, num_sms * blocks);
+  return r->stages >= 2;
 }
 
-int64_t norm_backward_parts(NormParams const &p, int num_sms) { return back_grid(p, num_sms).parts; }
+int64_t norm_backward_parts(NormParams const &p, int num_sms) {
+  return std::min<int64_t>(p.rows, (int64_t)num_sms * 32);
+}
+
+template <typename T, typename G, int N>
+static cudaError_t launch_back_ring(NormParams const &p, NormGradPtrs const &a, BackRing const &r, int64_t grid,
+                                    uint32_t *err, cudaStream_t st) {
+  auto kern = norm_backward_ring_kernel<T, G, N>;
+  const size_t bytes = (size_t)(r.stages * r.stage_bytes);
+  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
+  if (e != cudaSuccess) return e;
+  return launch_kernel(kern, dim3((unsigned)grid), dim3(r.threads), bytes, st, p, a, r, err);
+}
 
 template <typename T, typename G>
-static cudaError_t launch_norm_backward_t(NormParams const &p, NormGradPtrs const &a, int num_sms, cudaStream_t st) {
+static cudaError_t launch_norm_backward_t(NormParams const &p, NormGradPtrs const &a, uint32_t *err, int num_sms,
+                                          cudaStream_t st, int64_t *parts) {
   constexpr int V = NormBackRow<T, G, false>::V;
-  const BackGrid g = back_grid(p, num_sms);
-  if (g.wide)
-    return launch_wide(g.span.bytes ? norm_backward_wide_kernel<T, G, true> : norm_backward_wide_kernel<T, G, false>,
-                       g.span, st, p, a);
-  const bool grid = p.cols % V == 0 && row_vec_ok(a.h, p.s_h, p.rows, sizeof(T), V) &&
-                    row_vec_ok(a.dy, p.s_dy, p.rows, sizeof(G), V) &&
-                    row_vec_ok(a.dsum, p.s_dsum, p.rows, sizeof(G), V) &&
+  const bool grid = p.cols % V == 0 && row_vec_ok(a.h, p.s_h, p.rows, sizeof(T), 16 / sizeof(T)) &&
+                    row_vec_ok(a.dy, p.s_dy, p.rows, sizeof(G), 16 / sizeof(G)) &&
+                    row_vec_ok(a.dsum, p.s_dsum, p.rows, sizeof(G), 16 / sizeof(G)) &&
                     row_vec_ok(a.dx, p.s_dx, p.rows, sizeof(G), V) &&
                     row_vec_ok(a.w, 0, 1, p.dt_w == EIR_FP32 ? 4 : 2, V);
+  BackRing r{};
+  int per = 0;
+  // bulk copies take whole 16-byte units
+  if (grid && p.cols * sizeof(T) % 16 == 0 && p.cols * sizeof(G) % 16 == 0 &&
+      back_ring(p, sizeof(T) + sizeof(G) * (a.dsum ? 2 : 1), num_sms, &r, &per, parts)) {
+    return per == 8 ? launch_back_ring<T, G, 8 / V>(p, a, r, *parts, err, st)
+                    : launch_back_ring<T, G, 16 / V>(p, a, r, *parts, err, st);
+  }
+  if (p.cols > 1024 * kPerBack<T, G>) {
+    const WideGrid g = wide_grid(p.rows, p.cols, 512, V, sizeof(T) + 8, num_sms);
+    *parts = g.grid;
+    return launch_wide(g.bytes ? norm_backward_wide_kernel<T, G, true> : norm_backward_wide_kernel<T, G, false>, g, st,
+                       p, a);
+  }
+  const RowGrid g = row_grid(p.rows, p.cols, kPerBack<T, G>, num_sms);
+  *parts = std::min(g.units, p.rows);
   auto kern = grid ? norm_backward_kernel<T, G, true> : norm_backward_kernel<T, G, false>;
-  return launch_kernel(kern, dim3((unsigned)g.row.grid), dim3(g.row.threads), 0, st, p, a, g.row.warps);
+  return launch_kernel(kern, dim3((unsigned)g.grid), dim3(g.threads), 0, st, p, a, g.warps);
 }
 
-cudaError_t launch_norm_backward(NormParams const &p, NormGradPtrs const &a, int num_sms, cudaStream_t st) {
+cudaError_t launch_norm_backward(NormParams const &p, NormGradPtrs const &a, uint32_t *err, int num_sms,
+                                 cudaStream_t st, int64_t *parts) {
   if (p.dt == EIR_FP32)
-    return p.dt_grad == EIR_FP32 ? launch_norm_backward_t<float, float>(p, a, num_sms, st)
-                                 : launch_norm_backward_t<float, __nv_bfloat16>(p, a, num_sms, st);
-  return p.dt_grad == EIR_FP32 ? launch_norm_backward_t<__nv_bfloat16, float>(p, a, num_sms, st)
-                               : launch_norm_backward_t<__nv_bfloat16, __nv_bfloat16>(p, a, num_sms, st);
+    return p.dt_grad == EIR_FP32 ? launch_norm_backward_t<float, float>(p, a, err, num_sms, st, parts)
+                                 : launch_norm_backward_t<float, __nv_bfloat16>(p, a, err, num_sms, st, parts);
+  return p.dt_grad == EIR_FP32
+             ? launch_norm_backward_t<__nv_bfloat16, float>(p, a, err, num_sms, st, parts)
+             : launch_norm_backward_t<__nv_bfloat16, __nv_bfloat16>(p, a, err, num_sms, st, parts);
 }
 
 cudaError_t launch_norm_dweight(NormParams const &p, float const *part, int64_t n_part, float *dw,

@@ -147,6 +147,7 @@ struct RowPiece {
     if constexpr (sizeof(T) == 4) return __uint_as_float(w[i]);
     else return __uint_as_float(i & 1 ? w[i >> 1] & 0xffff0000u : w[i >> 1] << 16);
   }
+  __device__ __forceinline__ float2 get2(int i) const { return make_float2(get(i), get(i + 1)); }
   // all elements from FP32, each rounded once
   __device__ __forceinline__ void set(float const (&f)[V]) {
     if constexpr (sizeof(T) == 4) {

@@ -187,7 +187,7 @@ int eir_norm(eir_plan *p, void const *x, void const *residual, void const *weigh
   const eir::NormPtrs a{x, residual, weight, sum, out, scale, rstd};
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   ProfScope prof(p, st);
-  return launched(eir::launch_norm(n, a, num_sms, st), "norm launch");
+  return launched(eir::launch_norm(n, a, err, num_sms, st), "norm launch");
 }
 
 int eir_norm_backward(eir_plan *p, void const *dy, void const *h, void const *weight, float const *rstd,
@@ -262,7 +262,7 @@ int eir_quantize(eir_plan *p, void const *x, void *q, float *scale, void *stream
   if (rc != EIR_SUCCESS) return rc;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   ProfScope prof(p, st);
-  return launched(eir::launch_quantize(p->quant, x, static_cast<int8_t *>(q), scale, num_sms, st),
+  return launched(eir::launch_quantize(p->quant, x, static_cast<int8_t *>(q), scale, err, num_sms, st),
                   "quantize launch");
 }
 

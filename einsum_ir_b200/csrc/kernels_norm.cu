@@ -27,8 +27,7 @@ namespace eir {
 // registers an element
 template <typename T, bool QUANT>
 constexpr int kPer = (sizeof(T) == 4 ? 8 : 16) * (QUANT ? 2 : 1);  // norm; quantize
-template <typename T, typename G>
-constexpr int kPerBack = sizeof(T) + sizeof(G) == 8 ? 4 : 8;  // backward
+constexpr int kPerBack = 8;  // backward, of a warp's row
 
 // Sum of v and maximum of m over a row's threads: a warp (`warps` = 1), or the
 // block, with one barrier (`red`: 64 words, other ones at the next call).
@@ -46,6 +45,128 @@ __device__ __forceinline__ void row_sum_max(float &v, uint32_t &m, uint32_t *red
   if (SUM) v = warp_sum(lane < warps ? __uint_as_float(red[lane]) : 0.f);
   if (MAX) m = __reduce_max_sync(0xffffffffu, lane < warps ? red[32 + lane] : 0u);
 }
+
+// ---------------------------------------------------------------- a ring of rows in shared memory
+
+// Rows of up to three tensors are copied (cp.async.bulk) into a ring of stages, so
+// that the bytes in flight do not depend on the registers of the threads that work on a row. A
+// copy takes the 16-byte units that cover a row; of the units that reach outside the tensor (its first and
+// last row may have one), only the row's own bytes are read, by the thread. In its
+// slot a row starts as far off a 16-byte boundary as it does in memory.
+constexpr int kMostStages = 8;
+struct RingShape {
+  int threads;  // that work on rows: whole warps
+  int stages;
+  int64_t stage_bytes;
+};
+__host__ __device__ constexpr int64_t ring_slot(int64_t bytes) { return ((bytes + 15) / 16 + 4) * 16; }
+
+__device__ __forceinline__ void bulk_load(void *dst, uintptr_t src, uint32_t bytes, uint64_t *bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
+                   smem_u32(dst)),
+               "l"(src), "r"(bytes), "r"(smem_u32(bar))
+               : "memory");
+}
+
+struct RingTensor {  // in shared memory: only the copying thread needs all of it
+  uintptr_t begin, end;  // its bytes; none: absent
+  int64_t stride;        // of a row, in bytes
+  int64_t bytes;         // of a row
+  int64_t slot;          // its place in a stage
+  __device__ __forceinline__ void set(void const *p, int64_t rows, int64_t cols, int64_t row_stride, int esize,
+                                      int64_t at) {
+    begin = reinterpret_cast<uintptr_t>(p);
+    stride = row_stride * esize;
+    bytes = cols * esize;
+    end = p == nullptr ? begin : begin + (uintptr_t)((rows - 1) * stride + bytes);
+    slot = at;
+  }
+  __device__ __forceinline__ int64_t next_slot() const { return slot + (end > begin ? ring_slot(bytes) : 0); }
+  // how far into its slot a row lies
+  __device__ __forceinline__ uint32_t off(int64_t row) const {
+    return ((uint32_t)begin + (uint32_t)row * (uint32_t)stride) & 15u;
+  }
+  // bytes that arrive by bulk copy; the others are stored here
+  __device__ __forceinline__ uint32_t span(int64_t row, uint8_t *stage, uintptr_t &a0, uintptr_t &a1) const {
+    const uintptr_t r0 = begin + (uintptr_t)(row * stride), r1 = r0 + (uintptr_t)bytes;
+    a0 = r0 & ~(uintptr_t)15;
+    a1 = (r1 + 15) & ~(uintptr_t)15;
+    uint8_t *to = stage + slot;
+    const uintptr_t base = a0;
+    if (a0 < begin) a0 += 16;
+    if (a1 > end) a1 -= 16;
+    for (uintptr_t q = r0; q < a0 && q < r1; ++q) to[q - base] = *reinterpret_cast<uint8_t const *>(q);
+    for (uintptr_t q = a1 > r0 ? a1 : r0; q < r1; ++q) to[q - base] = *reinterpret_cast<uint8_t const *>(q);
+    return a1 > a0 ? (uint32_t)(a1 - a0) : 0u;
+  }
+  __device__ __forceinline__ void copy(int64_t row, uint8_t *stage, uintptr_t a0, uint32_t n, uint64_t *bar) const {
+    const uintptr_t base = (begin + (uintptr_t)(row * stride)) & ~(uintptr_t)15;
+    if (n) bulk_load(stage + slot + (a0 - base), a0, n, bar);
+  }
+};
+
+template <int TENSORS>
+__device__ __forceinline__ void ring_copy(RingTensor (&t)[TENSORS], int64_t row, uint8_t *stage, uint64_t *bar) {
+  uintptr_t a0[TENSORS], a1;
+  uint32_t n[TENSORS], total = 0;
+#pragma unroll
+  for (int i = 0; i < TENSORS; ++i) {
+    n[i] = 0;
+    if (t[i].end > t[i].begin) n[i] = t[i].span(row, stage, a0[i], a1);
+    total += n[i];
+  }
+  mbar_arrive_expect_tx(bar, total);
+#pragma unroll
+  for (int i = 0; i < TENSORS; ++i)
+    if (t[i].end > t[i].begin) t[i].copy(row, stage, a0[i], n[i], bar);
+}
+
+// The ring's shared words, and the thread that fills it: a warp of its own beside the
+// `warps` that work on rows (in one of those the copies delay every row: 8192 x 4096 BF16
+// backward 69 us)
+template <int TENSORS>
+struct RowRing {
+  uint64_t full[kMostStages], empty[kMostStages];
+  RingTensor t[TENSORS];
+  int abort;
+
+  __device__ __forceinline__ void init(RingShape const &ring) {
+    for (int s = 0; s < ring.stages; ++s) {
+      mbar_init(&full[s], 1);
+      mbar_init(&empty[s], ring.threads >> 5);
+    }
+    abort = 0;
+    fence_barrier_init();
+  }
+  __device__ __forceinline__ void fill(RingShape const &ring, uint8_t *stages, int64_t rows, uint32_t *err) {
+    volatile int *stop = &abort;
+    int stage = 0;
+    uint32_t phase = 0;
+    for (int64_t row = blockIdx.x; row < rows; row += gridDim.x) {
+      if (!mbar_wait_bounded(&empty[stage], phase ^ 1u, stop)) {
+        if (!*stop) record_error(err, kErrTimeoutProducer);
+        *stop = 1;
+        for (int i = 0; i < 1000; ++i) __nanosleep(1000);  // copies under way land before the block ends
+        return;
+      }
+      ring_copy(t, row, stages + stage * ring.stage_bytes, &full[stage]);
+      if (++stage == ring.stages) {
+        stage = 0;
+        phase ^= 1u;
+      }
+    }
+  }
+  // false: the wait has given up
+  __device__ __forceinline__ bool wait(int stage, uint32_t phase, uint32_t *err) {
+    volatile int *stop = &abort;
+    if (mbar_wait_bounded(&full[stage], phase, stop)) return true;
+    if (!*stop) record_error(err, kErrTimeoutEpilogue);
+    *stop = 1;
+    return false;
+  }
+};
+// a barrier of the `threads` that work on rows
+__device__ __forceinline__ void ring_sync(int threads) { asm volatile("bar.sync 1, %0;" ::"r"(threads) : "memory"); }
 
 // ---------------------------------------------------------------- norm and quantize
 
@@ -190,6 +311,75 @@ __global__ void __launch_bounds__(1024) norm_kernel(const NormParams p, const No
   }
 }
 
+// rows off the pieces' grid, a block a row: they come through the ring, since what is
+// shifted into place cannot wait in registers
+template <typename T, typename OUT, bool QUANT>
+__global__ void __launch_bounds__(1024)
+    norm_ring_kernel(const NormParams p, const NormPtrs a, const RingShape ring, uint32_t *err) {
+  using Row = NormRow<T, OUT, QUANT, false>;
+  constexpr int V = Row::V, N = kPer<T, false> / V;
+  extern __shared__ __align__(128) uint8_t stages[];
+  __shared__ uint32_t red[2][96];
+  __shared__ RowRing<2> rr;
+  const int warps = ring.threads >> 5, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (threadIdx.x == 0) {
+    rr.t[0].set(a.x, p.rows, p.cols, p.s_x, sizeof(T), 0);
+    rr.t[1].set(QUANT ? nullptr : a.res, p.rows, p.cols, p.s_res, sizeof(T), rr.t[0].next_slot());
+    rr.init(ring);
+  }
+  __syncthreads();
+  pdl_launch_dependents();
+  pdl_wait();
+  if (warp == warps) {
+    if (lane == 0) rr.fill(ring, stages, p.rows, err);
+    return;
+  }
+  const Row op(p, a);
+  const uint32_t slot = (uint32_t)ring_slot(p.cols * sizeof(T));
+  auto column = [&](int j) { return (j * ring.threads + (int)threadIdx.x) * V; };
+  int stage = 0, turn = 0;
+  uint32_t phase = 0;
+  for (int64_t row = blockIdx.x; row < p.rows; row += gridDim.x, turn ^= 1) {
+    const bool late = !rr.wait(stage, phase, err);
+    uint8_t const *at = stages + stage * ring.stage_bytes;
+    const uint32_t off_x = rr.t[0].off(row), off_r = rr.t[1].off(row);
+    float h[N][V];
+    float ss = 0.f;
+    uint32_t mx = 0;
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+      typename Row::Piece x, r;
+      x.load_slot(at, off_x, column(j), p.cols);
+      if (op.residual()) r.load_slot(at + slot, off_r, column(j), p.cols);
+      op.take(row, column(j), x, r, h[j], ss, mx);
+    }
+    __syncwarp();
+    if (lane == 0) mbar_arrive(&rr.empty[stage]);  // the row is in registers
+    if (!QUANT) ss = warp_sum(ss);
+    mx = __reduce_max_sync(0xffffffffu, mx);
+    const bool warp_late = __any_sync(0xffffffffu, late);
+    if (lane == 0) {
+      red[turn][warp] = __float_as_uint(ss);
+      red[turn][32 + warp] = mx;
+      red[turn][64 + warp] = warp_late;
+    }
+    ring_sync(ring.threads);
+    // all threads leave together where a wait has given up
+    if (__any_sync(0xffffffffu, lane < warps && red[turn][64 + lane] != 0)) break;
+    if (!QUANT) ss = warp_sum(lane < warps ? __uint_as_float(red[turn][lane]) : 0.f);
+    mx = __reduce_max_sync(0xffffffffu, lane < warps ? red[turn][32 + lane] : 0u);
+    const float rstd = op.rstd_of(ss);
+    const QuantScale q = quant_scale(mx, rstd);
+#pragma unroll
+    for (int j = 0; j < N; ++j) op.give(row, column(j), h[j], rstd, q);
+    if (threadIdx.x == 0) op.row_values(row, rstd, q);
+    if (++stage == ring.stages) {
+      stage = 0;
+      phase ^= 1u;
+    }
+  }
+}
+
 // wide rows: h in shared memory (CACHED), or read again
 template <typename T, typename OUT, bool QUANT, bool CACHED>
 __global__ void __launch_bounds__(1024) norm_wide_kernel(const NormParams p, const NormPtrs a) {
@@ -328,22 +518,20 @@ struct NormBackRow {
   }
 };
 
-// A row's threads hold h and dy between the two uses, and the weight gradient
-// of their columns over all rows that they see; it is written as one partial row a
-// block (a warp where a warp owns a row) and summed by norm_dweight_kernel: no
-// atomics, so the order is fixed.
+// Narrow rows: a warp a row, the next one loaded early. The weight gradient of the
+// warp's columns stays in registers over all rows that it sees and is written as one
+// partial row, summed by norm_dweight_kernel: no atomics, so the order is fixed. (So too below, a
+// block a partial row.)
 template <typename T, typename G, bool GRID>
-__global__ void __launch_bounds__(1024) norm_backward_kernel(const NormParams p, const NormGradPtrs a, int row_warps) {
+__global__ void __launch_bounds__(128) norm_backward_kernel(const NormParams p, const NormGradPtrs a) {
   using Row = NormBackRow<T, G, GRID>;
-  constexpr int V = Row::V, N = kPerBack<T, G> / V;
-  __shared__ uint32_t red[2][64];
+  constexpr int V = Row::V, N = kPerBack / V;
   pdl_launch_dependents();
   pdl_wait();
   const Row op(p, a);
-  const int threads = row_warps * 32, tid = row_warps == 1 ? threadIdx.x & 31 : threadIdx.x;
-  const int64_t rows_at_once = row_warps == 1 ? (int64_t)gridDim.x * (blockDim.x >> 5) : gridDim.x;
-  const int64_t first = row_warps == 1 ? (int64_t)blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5) : blockIdx.x;
-  auto column = [&](int j) { return (int64_t)(j * threads + tid) * V; };
+  const int lane = threadIdx.x & 31;
+  const int64_t at_once = (int64_t)gridDim.x * 4, first = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5);
+  auto column = [&](int j) { return (int64_t)(j * 32 + lane) * V; };
   typename Row::PieceH h[N];
   typename Row::PieceG dy[N], ds[N];
   float rstd = 0.f;
@@ -360,10 +548,8 @@ __global__ void __launch_bounds__(1024) norm_backward_kernel(const NormParams p,
   for (int j = 0; j < N; ++j)
 #pragma unroll
     for (int e = 0; e < V; ++e) dw[j][e] = 0.f;
-  int64_t row = first;
-  if (GRID && row < p.rows) fetch(row);
-  for (int turn = 0; row < p.rows; row += rows_at_once, turn ^= 1) {
-    if (!GRID) fetch(row);
+  if (first < p.rows) fetch(first);
+  for (int64_t row = first; row < p.rows; row += at_once) {
     const float unit = rstd;
     float held[N][V];
     typename Row::PieceH hr[N];
@@ -375,10 +561,8 @@ __global__ void __launch_bounds__(1024) norm_backward_kernel(const NormParams p,
       op.template take<true, true>(w, h[j], dy[j], ds[j], unit, held[j], gh, dw[j]);
       hr[j] = h[j];
     }
-    if (GRID && row + rows_at_once < p.rows) fetch(row + rows_at_once);
-    uint32_t unused = 0;
-    row_sum_max<true, false>(gh, unused, red[turn], row_warps);
-    const float k = op.factor(unit, gh);
+    if (row + at_once < p.rows) fetch(row + at_once);
+    const float k = op.factor(unit, warp_sum(gh));
 #pragma unroll
     for (int j = 0; j < N; ++j) op.give(row, column(j), held[j], hr[j], k);
   }
@@ -392,59 +576,35 @@ __global__ void __launch_bounds__(1024) norm_backward_kernel(const NormParams p,
   }
 }
 
-// Rows on the pieces' grid, wider than a warp: whole rows of h, dy and dsum are
-// copied (cp.async.bulk) into a ring of stages in shared memory, so that the bytes in flight do
-// not depend on the registers of the threads that work on a row. The barrier of the row's sum
-// says that its stage has been read; one thread then refills it. N: pieces of a
-// thread.
+// Blocks a row, over the ring. N: pieces of a thread.
 constexpr int kBackThreads = 512;  // of a block, at most
 // blocks an SM of that many threads, by a thread's elements
 __host__ __device__ constexpr int back_blocks(int per) { return per > 8 ? 1 : 2; }
-struct BackRing {
-  int threads;
-  int stages;
-  int64_t stage_bytes;
-};
 
-__device__ __forceinline__ void bulk_load(void *dst, void const *src, uint32_t bytes, uint64_t *bar) {
-  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
-                   smem_u32(dst)),
-               "l"(src), "r"(bytes), "r"(smem_u32(bar))
-               : "memory");
-}
-
-template <typename T, typename G, int N>
-__global__ void __launch_bounds__(kBackThreads, back_blocks(N * NormBackRow<T, G, true>::V))
-    norm_backward_ring_kernel(const NormParams p, const NormGradPtrs a, const BackRing ring, uint32_t *err) {
-  using Row = NormBackRow<T, G, true>;
-  constexpr int V = Row::V, kMostStages = 8;
+template <typename T, typename G, int N, bool GRID>
+__global__ void __launch_bounds__(kBackThreads + 32, back_blocks(N * NormBackRow<T, G, GRID>::V))
+    norm_backward_ring_kernel(const NormParams p, const NormGradPtrs a, const RingShape ring, uint32_t *err) {
+  using Row = NormBackRow<T, G, GRID>;
+  constexpr int V = Row::V;
   extern __shared__ __align__(128) uint8_t stages[];
   __shared__ uint32_t red[2][64];
-  __shared__ uint64_t full[kMostStages];
-  __shared__ int never;  // the bounded waits' abort word: a block's threads tell one another through `red`
+  __shared__ RowRing<3> rr;
   const int warps = ring.threads >> 5, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
-    for (int s = 0; s < ring.stages; ++s) mbar_init(&full[s], 1);
-    never = 0;
-    fence_barrier_init();
+    rr.t[0].set(a.h, p.rows, p.cols, p.s_h, sizeof(T), 0);
+    rr.t[1].set(a.dy, p.rows, p.cols, p.s_dy, sizeof(G), rr.t[0].next_slot());
+    rr.t[2].set(a.dsum, p.rows, p.cols, p.s_dsum, sizeof(G), rr.t[1].next_slot());
+    rr.init(ring);
   }
   __syncthreads();
   pdl_launch_dependents();
   pdl_wait();
-  const uint32_t bytes_h = (uint32_t)(p.cols * sizeof(T)), bytes_g = (uint32_t)(p.cols * sizeof(G));
-  auto copy_row = [&](int64_t row, int stage) {
-    uint8_t *to = stages + stage * ring.stage_bytes;
-    mbar_arrive_expect_tx(&full[stage], bytes_h + bytes_g * (a.dsum ? 2 : 1));
-    bulk_load(to, static_cast<T const *>(a.h) + row * p.s_h, bytes_h, &full[stage]);
-    bulk_load(to + bytes_h, static_cast<G const *>(a.dy) + row * p.s_dy, bytes_g, &full[stage]);
-    if (a.dsum)
-      bulk_load(to + bytes_h + bytes_g, static_cast<G const *>(a.dsum) + row * p.s_dsum, bytes_g, &full[stage]);
-  };
-  if (threadIdx.x == 0) {
-    for (int s = 0; s < ring.stages; ++s)
-      if (blockIdx.x + (int64_t)s * gridDim.x < p.rows) copy_row(blockIdx.x + (int64_t)s * gridDim.x, s);
+  if (warp == warps) {
+    if (lane == 0) rr.fill(ring, stages, p.rows, err);
+    return;
   }
   const Row op(p, a);
+  const uint32_t slot_h = (uint32_t)ring_slot(p.cols * sizeof(T)), slot_g = (uint32_t)ring_slot(p.cols * sizeof(G));
   const float inv_cols = 1.f / (float)p.cols;
   auto column = [&](int j) { return (j * ring.threads + (int)threadIdx.x) * V; };
   float dw[N][V];
@@ -458,8 +618,10 @@ __global__ void __launch_bounds__(kBackThreads, back_blocks(N * NormBackRow<T, G
   for (int64_t row = blockIdx.x; row < p.rows; row += gridDim.x, turn ^= 1) {
     const float unit = next;
     if (row + gridDim.x < p.rows) next = a.rstd[row + gridDim.x];
-    const bool late = !mbar_wait_bounded(&full[stage], phase, &never);
-    uint8_t const *at = stages + stage * ring.stage_bytes;
+    const bool late = !rr.wait(stage, phase, err);
+    uint8_t const *at = stages + stage * ring.stage_bytes, *dy_at = at + slot_h, *sum_at = dy_at + slot_g;
+    const uint32_t off_h = GRID ? 0 : rr.t[0].off(row), off_d = GRID ? 0 : rr.t[1].off(row);
+    const uint32_t off_s = GRID ? 0 : rr.t[2].off(row);
     float held[N][V];
     typename Row::PieceH h[N];
     float gh = 0.f;
@@ -467,31 +629,31 @@ __global__ void __launch_bounds__(kBackThreads, back_blocks(N * NormBackRow<T, G
     for (int j = 0; j < N; ++j) {
       const int c = column(j);
       typename Row::PieceG dy, s;
-      if (c >= p.cols) continue;
+      if (GRID && c >= p.cols) continue;
       float w[V];
       op.weight(c, w);
-      h[j].template load<false>(at + c * sizeof(T));
-      dy.template load<false>(at + bytes_h + c * sizeof(G));
-      if (a.dsum) s.template load<false>(at + bytes_h + bytes_g + c * sizeof(G));
+      if (GRID) {
+        h[j].template load<false>(at + c * (int)sizeof(T));
+        dy.template load<false>(dy_at + c * (int)sizeof(G));
+        if (a.dsum) s.template load<false>(sum_at + c * (int)sizeof(G));
+      } else {
+        h[j].load_slot(at, off_h, c, p.cols);
+        dy.load_slot(dy_at, off_d, c, p.cols);
+        if (a.dsum) s.load_slot(sum_at, off_s, c, p.cols);
+      }
       op.template take<true, true>(w, h[j], dy, s, unit, held[j], gh, dw[j]);
     }
+    __syncwarp();
+    if (lane == 0) mbar_arrive(&rr.empty[stage]);  // the row is in registers
     gh = warp_sum(gh);
     const bool warp_late = __any_sync(0xffffffffu, late);
     if (lane == 0) {
       red[turn][warp] = __float_as_uint(gh);
       red[turn][32 + warp] = warp_late;
     }
-    __syncthreads();
+    ring_sync(ring.threads);
     // all threads leave together where a wait has given up
-    if (__any_sync(0xffffffffu, lane < warps && red[turn][32 + lane] != 0)) {
-      if (threadIdx.x == 0) {
-        record_error(err, kErrTimeoutProducer);
-        for (int i = 0; i < 1000; ++i) __nanosleep(1000);  // copies under way land before the block ends
-      }
-      break;
-    }
-    if (threadIdx.x == 0 && row + (int64_t)ring.stages * gridDim.x < p.rows)
-      copy_row(row + (int64_t)ring.stages * gridDim.x, stage);
+    if (__any_sync(0xffffffffu, lane < warps && red[turn][32 + lane] != 0)) break;
     gh = warp_sum(lane < warps ? __uint_as_float(red[turn][lane]) : 0.f);
     const float k = unit * unit * (gh * inv_cols);
 #pragma unroll
@@ -622,23 +784,18 @@ __global__ void __launch_bounds__(1024) norm_dweight_kernel(int64_t cols, float 
 
 // ---------------------------------------------------------------- launchers
 
-// warps of a row
-static int row_warps(int64_t cols, int per) { return (int)((cols + 32 * per - 1) / (32 * per)); }
-
 // block and grid: persistent blocks of up to 1024 threads an SM (64 registers a thread)
 struct RowGrid {
   int warps;      // of a row
-  int threads;    // of a block
+  int threads;    // of a block: four rows of a warp, or a row
   int64_t grid;
-  int64_t units;  // rows in flight: blocks, or warps
 };
 static RowGrid row_grid(int64_t rows, int64_t cols, int per, int num_sms) {
   RowGrid g;
-  g.warps = row_warps(cols, per);
+  g.warps = (int)((cols + 32 * per - 1) / (32 * per));
   g.threads = g.warps == 1 ? 128 : g.warps * 32;
   const int64_t blocks = g.warps == 1 ? (rows + 3) / 4 : rows;
   g.grid = std::min<int64_t>(blocks, (int64_t)num_sms * (1024 / g.threads));
-  g.units = g.warps == 1 ? g.grid * 4 : g.grid;
   return g;
 }
 
@@ -669,8 +826,28 @@ static cudaError_t launch_wide(void (*kern)(KArgs...), WideGrid const &g, cudaSt
   return launch_kernel(kern, dim3((unsigned)g.grid), dim3(g.threads), (size_t)g.bytes, st, args...);
 }
 
+// stages of a ring for `blocks` blocks an SM at most (fewer where two stages a block do not
+// fit otherwise); 0 stages: too wide
+static int64_t ring_fit(int64_t stage_bytes, int64_t blocks, RingShape *r) {
+  r->stage_bytes = stage_bytes;
+  while (blocks > 1 && (2 * stage_bytes + 2048) * blocks > kSmemMost) --blocks;
+  r->stages = (int)std::min<int64_t>(kMostStages, (kSmemMost / blocks - 2048) / stage_bytes);
+  if (r->stages < 2) r->stages = 0;
+  return blocks;
+}
+
+template <typename... KArgs, typename... Args>
+static cudaError_t launch_ring(void (*kern)(KArgs...), RingShape const &r, int64_t grid, cudaStream_t st,
+                               Args const &...args) {
+  const size_t bytes = (size_t)(r.stages * r.stage_bytes);
+  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
+  if (e != cudaSuccess) return e;
+  return launch_kernel(kern, dim3((unsigned)grid), dim3(r.threads + 32), bytes, st, args...);
+}
+
 template <typename T, typename OUT, bool QUANT>
-static cudaError_t launch_norm_out(NormParams const &p, NormPtrs const &a, int num_sms, cudaStream_t st) {
+static cudaError_t launch_norm_out(NormParams const &p, NormPtrs const &a, uint32_t *err, int num_sms,
+                                   cudaStream_t st) {
   constexpr int V = 16 / sizeof(T);
   if (p.cols > 1024 * kPer<T, QUANT>) {
     const WideGrid g = wide_grid(p.rows, p.cols, 1024, V, 4, num_sms);
@@ -682,23 +859,32 @@ static cudaError_t launch_norm_out(NormParams const &p, NormPtrs const &a, int n
                     row_vec_ok(a.out, p.s_out, p.rows, sizeof(OUT), V) &&
                     row_vec_ok(a.w, 0, 1, p.dt_w == EIR_FP32 ? 4 : 2, V);
   const RowGrid g = row_grid(p.rows, p.cols, kPer<T, QUANT>, num_sms);
+  if (!grid && g.warps > 1 && p.cols <= (1024 - 32) * kPer<T, false>) {
+    RingShape r;
+    r.threads = (int)((p.cols + kPer<T, false> - 1) / kPer<T, false> + 31) / 32 * 32;
+    const int64_t blocks = ring_fit(ring_slot(p.cols * sizeof(T)) * (a.res ? 2 : 1), 1024 / (r.threads + 32), &r);
+    if (r.stages > 0)
+      return launch_ring(norm_ring_kernel<T, OUT, QUANT>, r, std::min<int64_t>(p.rows, num_sms * blocks), st, p, a, r,
+                         err);
+  }
   auto kern = grid ? norm_kernel<T, OUT, QUANT, true> : norm_kernel<T, OUT, QUANT, false>;
   return launch_kernel(kern, dim3((unsigned)g.grid), dim3(g.threads), 0, st, p, a, g.warps);
 }
 
 template <typename T>
-static cudaError_t launch_norm_t(NormParams const &p, NormPtrs const &a, int num_sms, cudaStream_t st) {
-  if (p.dt_out == EIR_FP32) return launch_norm_out<T, float, false>(p, a, num_sms, st);
-  if (p.dt_out == EIR_BF16) return launch_norm_out<T, __nv_bfloat16, false>(p, a, num_sms, st);
-  return launch_norm_out<T, int8_t, false>(p, a, num_sms, st);
+static cudaError_t launch_norm_t(NormParams const &p, NormPtrs const &a, uint32_t *err, int num_sms, cudaStream_t st) {
+  if (p.dt_out == EIR_FP32) return launch_norm_out<T, float, false>(p, a, err, num_sms, st);
+  if (p.dt_out == EIR_BF16) return launch_norm_out<T, __nv_bfloat16, false>(p, a, err, num_sms, st);
+  return launch_norm_out<T, int8_t, false>(p, a, err, num_sms, st);
 }
 
-cudaError_t launch_norm(NormParams const &p, NormPtrs const &a, int num_sms, cudaStream_t st) {
-  return p.dt == EIR_FP32 ? launch_norm_t<float>(p, a, num_sms, st) : launch_norm_t<__nv_bfloat16>(p, a, num_sms, st);
+cudaError_t launch_norm(NormParams const &p, NormPtrs const &a, uint32_t *err, int num_sms, cudaStream_t st) {
+  return p.dt == EIR_FP32 ? launch_norm_t<float>(p, a, err, num_sms, st)
+                          : launch_norm_t<__nv_bfloat16>(p, a, err, num_sms, st);
 }
 
-cudaError_t launch_quantize(QuantizeParams const &p, void const *x, int8_t *q, float *scale, int num_sms,
-                            cudaStream_t st) {
+cudaError_t launch_quantize(QuantizeParams const &p, void const *x, int8_t *q, float *scale, uint32_t *err,
+                            int num_sms, cudaStream_t st) {
   NormParams n;
   n.rows = p.rows;
   n.cols = p.cols;
@@ -707,37 +893,12 @@ cudaError_t launch_quantize(QuantizeParams const &p, void const *x, int8_t *q, f
   n.s_x = p.s_x;
   n.s_out = p.s_out;
   const NormPtrs a{x, nullptr, nullptr, nullptr, q, scale, nullptr};
-  return p.dt == EIR_FP32 ? launch_norm_out<float, int8_t, true>(n, a, num_sms, st)
-                          : launch_norm_out<__nv_bfloat16, int8_t, true>(n, a, num_sms, st);
-}
-
-// Backward: the ring takes rows on the pieces' grid that are wider than a warp and of
-// which two stages fit; *per: elements of a thread in a row
-static bool back_ring(NormParams const &p, int row_bytes, int num_sms, BackRing *r, int *per, int64_t *grid) {
-  if (p.cols <= 32 * 8 || p.rows < 2) return false;
-  *per = p.cols <= kBackThreads * 8 ? 8 : 16;
-  r->threads = (int)((p.cols + *per - 1) / *per + 31) / 32 * 32;
-  if (r->threads > kBackThreads) return false;
-  r->stage_bytes = (p.cols * row_bytes + 127) / 128 * 128;
-  int64_t blocks = std::min(8, back_blocks(*per) * kBackThreads / r->threads);
-  while (blocks > 1 && (2 * r->stage_bytes + 2048) * blocks > kSmemMost) --blocks;
-  r->stages = (int)std::min<int64_t>(8, (kSmemMost / blocks - 2048) / r->stage_bytes);
-  *grid = std::min<int64_t>(p.rows, num_sms * blocks);
-  return r->stages >= 2;
+  return p.dt == EIR_FP32 ? launch_norm_out<float, int8_t, true>(n, a, err, num_sms, st)
+                          : launch_norm_out<__nv_bfloat16, int8_t, true>(n, a, err, num_sms, st);
 }
 
 int64_t norm_backward_parts(NormParams const &p, int num_sms) {
   return std::min<int64_t>(p.rows, (int64_t)num_sms * 32);
-}
-
-template <typename T, typename G, int N>
-static cudaError_t launch_back_ring(NormParams const &p, NormGradPtrs const &a, BackRing const &r, int64_t grid,
-                                    uint32_t *err, cudaStream_t st) {
-  auto kern = norm_backward_ring_kernel<T, G, N>;
-  const size_t bytes = (size_t)(r.stages * r.stage_bytes);
-  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
-  if (e != cudaSuccess) return e;
-  return launch_kernel(kern, dim3((unsigned)grid), dim3(r.threads), bytes, st, p, a, r, err);
 }
 
 template <typename T, typename G>
@@ -749,24 +910,29 @@ static cudaError_t launch_norm_backward_t(NormParams const &p, NormGradPtrs cons
                     row_vec_ok(a.dsum, p.s_dsum, p.rows, sizeof(G), 16 / sizeof(G)) &&
                     row_vec_ok(a.dx, p.s_dx, p.rows, sizeof(G), V) &&
                     row_vec_ok(a.w, 0, 1, p.dt_w == EIR_FP32 ? 4 : 2, V);
-  BackRing r{};
-  int per = 0;
-  // bulk copies take whole 16-byte units
-  if (grid && p.cols * sizeof(T) % 16 == 0 && p.cols * sizeof(G) % 16 == 0 &&
-      back_ring(p, sizeof(T) + sizeof(G) * (a.dsum ? 2 : 1), num_sms, &r, &per, parts)) {
-    return per == 8 ? launch_back_ring<T, G, 8 / V>(p, a, r, *parts, err, st)
-                    : launch_back_ring<T, G, 16 / V>(p, a, r, *parts, err, st);
+  if (p.cols <= 32 * kPerBack) {
+    const RowGrid g = row_grid(p.rows, p.cols, kPerBack, num_sms);
+    *parts = std::min(g.grid * 4, p.rows);
+    auto kern = grid ? norm_backward_kernel<T, G, true> : norm_backward_kernel<T, G, false>;
+    return launch_kernel(kern, dim3((unsigned)g.grid), dim3(g.threads), 0, st, p, a);
   }
-  if (p.cols > 1024 * kPerBack<T, G>) {
-    const WideGrid g = wide_grid(p.rows, p.cols, 512, V, sizeof(T) + 8, num_sms);
-    *parts = g.grid;
-    return launch_wide(g.bytes ? norm_backward_wide_kernel<T, G, true> : norm_backward_wide_kernel<T, G, false>, g, st,
-                       p, a);
+  const int per = p.cols <= kBackThreads * 8 ? 8 : 16;
+  RingShape r;
+  r.threads = (int)((p.cols + per - 1) / per + 31) / 32 * 32;
+  if (r.threads <= kBackThreads) {
+    const int64_t bytes = ring_slot(p.cols * sizeof(T)) + ring_slot(p.cols * sizeof(G)) * (a.dsum ? 2 : 1);
+    const int64_t blocks = ring_fit(bytes, std::min(8, back_blocks(per) * (kBackThreads + 32) / (r.threads + 32)), &r);
+    if (r.stages > 0) {
+      *parts = std::min<int64_t>(p.rows, num_sms * blocks);
+      auto kern = per == 8 ? (grid ? norm_backward_ring_kernel<T, G, 8 / V, true> : norm_backward_ring_kernel<T, G, 8 / V, false>)
+                           : (grid ? norm_backward_ring_kernel<T, G, 16 / V, true> : norm_backward_ring_kernel<T, G, 16 / V, false>);
+      return launch_ring(kern, r, *parts, st, p, a, r, err);
+    }
   }
-  const RowGrid g = row_grid(p.rows, p.cols, kPerBack<T, G>, num_sms);
-  *parts = std::min(g.units, p.rows);
-  auto kern = grid ? norm_backward_kernel<T, G, true> : norm_backward_kernel<T, G, false>;
-  return launch_kernel(kern, dim3((unsigned)g.grid), dim3(g.threads), 0, st, p, a, g.warps);
+  const WideGrid g = wide_grid(p.rows, p.cols, 512, V, sizeof(T) + 8, num_sms);
+  *parts = g.grid;
+  return launch_wide(g.bytes ? norm_backward_wide_kernel<T, G, true> : norm_backward_wide_kernel<T, G, false>, g, st, p,
+                     a);
 }
 
 cudaError_t launch_norm_backward(NormParams const &p, NormGradPtrs const &a, uint32_t *err, int num_sms,

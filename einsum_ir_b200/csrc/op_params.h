@@ -76,15 +76,15 @@ struct LogprobGradPtrs {
   void *dx;
 };
 
-cudaError_t launch_norm(NormParams const &p, NormPtrs const &a, int num_sms, cudaStream_t st);
+cudaError_t launch_norm(NormParams const &p, NormPtrs const &a, uint32_t *err, int num_sms, cudaStream_t st);
 // the most partial rows of the weight gradient that the backward kernels write; *parts: how many
 int64_t norm_backward_parts(NormParams const &p, int num_sms);
 cudaError_t launch_norm_backward(NormParams const &p, NormGradPtrs const &a, uint32_t *err, int num_sms,
                                  cudaStream_t st, int64_t *parts);
 cudaError_t launch_norm_dweight(NormParams const &p, float const *part, int64_t n_part, float *dw,
                                 cudaStream_t st);
-cudaError_t launch_quantize(QuantizeParams const &p, void const *x, int8_t *q, float *scale, int num_sms,
-                            cudaStream_t st);
+cudaError_t launch_quantize(QuantizeParams const &p, void const *x, int8_t *q, float *scale, uint32_t *err,
+                            int num_sms, cudaStream_t st);
 cudaError_t launch_i8_simt(I8Params const &p, I8Ptrs const &a, cudaStream_t st);
 cudaError_t launch_i8_tc(I8TcPlan const &tp, CUtensorMap const &map_channels, CUtensorMap const &map_tokens,
                          I8Params const &p, I8Ptrs const &a, uint32_t *err, cudaStream_t st);

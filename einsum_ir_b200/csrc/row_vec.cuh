@@ -104,6 +104,37 @@ struct RowPiece {
     }
   }
 
+  // the same from a copy of the row in shared memory, which starts `off` bytes
+  // after `slot` (16-byte aligned; at least 48 bytes behind the row may be read)
+  __device__ __forceinline__ void load_slot(uint8_t const *slot, uint32_t off, int c, int64_t cols) {
+    uint8_t const *at = slot + c * (int)sizeof(T);
+    if (c >= cols) {
+      zero();
+      return;
+    }
+    if (kBytes < 16) {  // (a piece of a narrower type: its own grid within the row's shift)
+      at += off / kBytes * kBytes;
+      off %= kBytes;
+    }
+    load<false>(at);
+    if (off != 0) {
+      RowPiece hi;
+      uint32_t lo[kWords];
+#pragma unroll
+      for (int i = 0; i < kWords; ++i) lo[i] = w[i];
+      hi.template load<false>(at + kBytes);
+      shifted_words<kWords>(lo, hi.w, off, w);
+    }
+    if (c + V > cols) {
+#pragma unroll
+      for (int e = 0; e < V; ++e) {
+        if (c + e < cols) continue;
+        if constexpr (sizeof(T) == 4) w[e] = 0;
+        else w[e / 2] &= e % 2 ? 0x0000ffffu : 0xffff0000u;
+      }
+    }
+  }
+
   // elements first .. last - 1 of the piece, one by one
   __device__ __forceinline__ void store_some(T *p, int first, int last) const {
 #pragma unroll

@@ -1,149 +1,554 @@
 // Log probabilities of given tokens, log-sum-exp, entropy and top alternatives
 // of rows of logits, and the gradient of the first and third.
 //
-// With m = max x, S = sum e^(x - m), U = sum (x - m) e^(x - m):
-// lse = m + log S, entropy = log S - U / S (no difference of large numbers:
-// U <= 0), log p = (x - m) - log S (exact differences where the logits are
-// large and near one another). Backward: dx = dlogprob (onehot - p) - dentropy p (x - lse + H).
+// One pass over a row, in base 2 (L = log2 e): with a reference R >= about the row's
+// maximum times L, S = sum 2^d and U = sum d 2^d for d = x L - R give
+// lse = (R + log2 S) / L, log p = (d - log2 S) / L and entropy = (log2 S - U / S) / L. Any R will do, so
+// rounding it costs nothing; a thread raises its own when it meets a larger logit and its
+// sums shrink by 2^(R - R'). d is floored at -200, where 2^d is 0 in FP32, so that
+// a ruled-out logit (-infinity) adds 0 d = 0 to U.
+//
+// Bound by HBM (a logit is read once; the one exponential an element takes 73 %
+// of the SM's rate at BF16 and full bandwidth). A piece is 16 bytes of memory on
+// the 16-byte grid, so rows of any alignment stream alike; the elements of
+// the first and last piece that lie outside the row count as ruled out.
+//
+// Top alternatives without a second pass: each thread keeps its largest logit and the
+// piece it came from. The k-th largest of these (ties: the earlier piece) is a
+// lower bound of the row's k-th largest logit, and only the k threads that hold
+// larger ones can hold an alternative: their pieces are read again (k / threads of the row, from
+// L2), and the few candidates above the bound are sorted. Order by one 64-bit key,
+// logit first and lower index second, so that the result does not depend on the order of work.
+//
+// Rows that do not fill the GPU by number are split over a cluster of up to 8 blocks, joined
+// through distributed shared memory.
+//
+// Rows with a NaN or +infinity, with nothing above -1e37, or with more candidates
+// than their buffer holds are redone by logprob_plain_row: a pass for each value.
+//
+// Backward: dx = dlogprob (onehot - p) - dentropy p (x - lse + H).
+#include <algorithm>
 #include "eir_launch.h"
 #include "eir_common.cuh"
-#include "op_common.cuh"
 #include "op_params.h"
+#include "row_vec.cuh"
 
 namespace eir {
 
-constexpr int kLogThreads = 256;
+constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
+constexpr float kLowest = -1e37f;  // logits below count as ruled out in the fast pass
+constexpr int kLogWarps = 16;      // of a block, at most
+constexpr int kCandidates = 1024;
+
+__device__ __forceinline__ float exp2_fast(float x) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+// the larger, NaN if either is
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
 
 // a logit's rank as an unsigned integer: the order of the floats, both zeros
-// alike, NaNs highest
+// alike, NaNs highest; 0 is below every logit's
 __device__ __forceinline__ uint32_t rank_bits(float x) {
   if (x != x) return 0xffffffffu;
   const uint32_t u = __float_as_uint(x + 0.f);
   return (u & 0x80000000u) ? ~u : u | 0x80000000u;
 }
+__device__ __forceinline__ float rank_value(uint32_t r) {
+  if (r == 0xffffffffu) return __uint_as_float(0x7fc00000u);
+  return __uint_as_float((r & 0x80000000u) ? r ^ 0x80000000u : ~r);
+}
 // rank and place in one word: larger logits first, then lower indices
 __device__ __forceinline__ uint64_t rank_key(float x, uint32_t index) {
   return ((uint64_t)rank_bits(x) << 32) | (uint32_t)~index;
 }
+__device__ __forceinline__ uint64_t warp_max_key(uint64_t k) {
+  const uint32_t hi = __reduce_max_sync(0xffffffffu, (uint32_t)(k >> 32));
+  const uint32_t lo = __reduce_max_sync(0xffffffffu, (uint32_t)(k >> 32) == hi ? (uint32_t)k : 0u);
+  return ((uint64_t)hi << 32) | lo;
+}
 
 __device__ __forceinline__ float logit_nan() { return __uint_as_float(0x7fc00000u); }
 
+// A row's sums against the reference R = m L (0 below kLowest, where S = 0)
+struct LogSums {
+  float m, S, U;
+};
+__device__ __forceinline__ float log_ref(float m) { return m < kLowest ? 0.f : m * kLog2e; }
+// log p of a logit (one below kLowest may leave FP32's range in base 2)
+__device__ __forceinline__ float log_prob(float x, LogSums const &v, float log_s) {
+  return x < kLowest ? x - v.m : (fmaf(x, kLog2e, -log_ref(v.m)) - log_s) * kLn2;
+}
+// the sums of both, against the larger maximum
+__device__ __forceinline__ LogSums log_join(LogSums a, LogSums b) {
+  LogSums r;
+  r.m = fmaxf(a.m, b.m);
+  const float R = log_ref(r.m), da = log_ref(a.m) - R, db = log_ref(b.m) - R;
+  // (sums of 0 may stand beside any reference)
+  const float ea = a.S == 0.f ? 0.f : exp2_fast(da), eb = b.S == 0.f ? 0.f : exp2_fast(db);
+  r.S = a.S * ea + b.S * eb;
+  r.U = (a.S == 0.f ? 0.f : ea * (a.U + da * a.S)) + (b.S == 0.f ? 0.f : eb * (b.U + db * b.S));
+  return r;
+}
+__device__ __forceinline__ LogSums log_join_lanes(LogSums v) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    LogSums w;
+    w.m = __shfl_xor_sync(0xffffffffu, v.m, o);
+    w.S = __shfl_xor_sync(0xffffffffu, v.S, o);
+    w.U = __shfl_xor_sync(0xffffffffu, v.U, o);
+    v = log_join(v, w);
+  }
+  return v;
+}
+
+// one row's values, written by one thread
+__device__ __forceinline__ void logprob_row_values(LogprobParams const &p, LogprobPtrs const &a, int64_t row, bool none,
+                                                   float lse, float entropy, float target_logprob) {
+  if (a.lse) a.lse[row] = lse;
+  if (a.entropy) a.entropy[row] = none ? 0.f : entropy;
+  if (a.targets) {
+    const int64_t t = a.targets[row];
+    a.logprob[row] = t < 0 ? 0.f : (t >= p.vocab ? logit_nan() : (none ? -INFINITY : target_logprob));
+  }
+}
+
+// A row by plain passes (all threads of the block): right for every row, a
+// pass over it for each value. red: 3 x 32 words; best: 32 keys.
 template <typename T>
-__global__ void __launch_bounds__(kLogThreads) logprob_kernel(const LogprobParams p, const LogprobPtrs a) {
-  __shared__ float red[3][kLogThreads / 32];
-  __shared__ uint64_t best[kLogThreads / 32];
+__device__ __noinline__ void logprob_plain_row(LogprobParams const &p, LogprobPtrs const &a, int64_t row, float *red,
+                                               uint64_t *best) {
+  const int warps = blockDim.x >> 5, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  T const *x = static_cast<T const *>(a.x) + row * p.s_x;
+  float m = -INFINITY;
+  for (int64_t c = threadIdx.x; c < p.vocab; c += blockDim.x) m = fmaxf(m, to_f32(x[c]));
+  for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+  __syncthreads();
+  if (lane == 0) red[warp] = m;
+  __syncthreads();
+  for (int w = 0; w < warps; ++w) m = fmaxf(m, red[w]);
+  const float ref = m == -INFINITY ? 0.f : m;
+  float S = 0.f, U = 0.f;
+  for (int64_t c = threadIdx.x; c < p.vocab; c += blockDim.x) {
+    const float d = to_f32(x[c]) - ref, e = expf(d);
+    S += e;
+    U += d == -INFINITY ? 0.f : d * e;
+  }
+  S = warp_sum(S);
+  U = warp_sum(U);
+  if (lane == 0) {
+    red[32 + warp] = S;
+    red[64 + warp] = U;
+  }
+  __syncthreads();
+  S = U = 0.f;
+  for (int w = 0; w < warps; ++w) {
+    S += red[32 + w];
+    U += red[64 + w];
+  }
+  const bool none = S == 0.f;
+  const float log_s = logf(S);
+  if (threadIdx.x == 0) {
+    const int64_t t = a.targets ? a.targets[row] : -1;
+    const float xt = t >= 0 && t < p.vocab ? to_f32(x[t]) : 0.f;
+    logprob_row_values(p, a, row, none, none ? -INFINITY : ref + log_s, log_s - U / S, xt - ref - log_s);
+  }
+  uint64_t last = ~0ull;
+  for (int i = 0; i < p.top; ++i) {
+    uint64_t k = 0;
+    for (int64_t c = threadIdx.x; c < p.vocab; c += blockDim.x) {
+      const uint64_t key = rank_key(to_f32(x[c]), (uint32_t)c);
+      if (key < last || i == 0) k = key > k ? key : k;
+    }
+    k = warp_max_key(k);
+    __syncthreads();
+    if (lane == 0) best[warp] = k;
+    __syncthreads();
+    for (int w = 0; w < warps; ++w) k = best[w] > k ? best[w] : k;
+    last = k;
+    if (threadIdx.x == 0) {
+      const uint32_t at = ~(uint32_t)k;
+      if (a.top_index) a.top_index[row * p.top + i] = at;
+      if (a.top_logprob) a.top_logprob[row * p.top + i] = none ? -INFINITY : to_f32(x[at]) - ref - log_s;
+    }
+  }
+  __syncthreads();
+}
+
+// a row's pieces: 16-byte units of memory that hold some of its elements
+template <typename T>
+struct LogitRow {
+  static constexpr int V = 16 / (int)sizeof(T);
+  using Piece = RowPiece<T, V>;
+  uint8_t const *base;  // the first unit
+  int off;              // elements of it before the row
+  int vocab;
+  int pieces;
+  __device__ __forceinline__ LogitRow(T const *x, int64_t n) {
+    const uintptr_t at = reinterpret_cast<uintptr_t>(x);
+    base = reinterpret_cast<uint8_t const *>(at & ~(uintptr_t)15);
+    off = (int)(at & 15) / (int)sizeof(T);
+    vocab = (int)n;
+    pieces = (int)((n + off + V - 1) / V);
+  }
+  __device__ __forceinline__ int first_index(int piece) const { return piece * V - off; }
+  // a piece; elements outside the row are -infinity
+  __device__ __forceinline__ Piece load(int piece) const {
+    Piece v;
+    const int i0 = first_index(piece);
+    if (i0 >= 0 && i0 <= vocab - V) {
+      v.template load<false>(base + (int64_t)piece * 16);
+    } else {
+#pragma unroll
+      for (int i = 0; i < Piece::kWords; ++i) v.w[i] = sizeof(T) == 4 ? 0xff800000u : 0xff80ff80u;
+      T const *x = reinterpret_cast<T const *>(base) + off;
+#pragma unroll
+      for (int e = 0; e < V; ++e) {
+        if (i0 + e < 0 || i0 + e >= vocab) continue;
+        if constexpr (sizeof(T) == 4) v.w[e] = *reinterpret_cast<uint32_t const *>(x + i0 + e);
+        else {
+          const uint32_t b = *reinterpret_cast<unsigned short const *>(x + i0 + e);
+          v.w[e / 2] = e % 2 ? (v.w[e / 2] & 0x0000ffffu) | b << 16 : (v.w[e / 2] & 0xffff0000u) | b;
+        }
+      }
+    }
+    return v;
+  }
+  // the largest element (a NaN counts as absent)
+  static __device__ __forceinline__ float largest(Piece const &v) {
+    if constexpr (sizeof(T) == 4) {
+      return fmaxf(fmaxf(v.get(0), v.get(1)), fmaxf(v.get(2), v.get(3)));
+    } else {
+      __nv_bfloat162 b[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) b[i] = *reinterpret_cast<__nv_bfloat162 const *>(&v.w[i]);
+      const __nv_bfloat162 m = __hmax2(__hmax2(b[0], b[1]), __hmax2(b[2], b[3]));
+      return fmaxf(__low2float(m), __high2float(m));
+    }
+  }
+};
+
+struct LogShared {
+  float red[96];           // (m, S, U) of the warps; the plain row's words
+  uint64_t keys[32 * kLogWarps];  // the threads' largest logits
+  uint64_t chosen[32];     // the k largest of them; the plain row's words
+  uint64_t top[32];        // the block's alternatives
+  uint64_t found[kCandidates];
+  int n_chosen, n_found, odd;
+  LogSums sums;            // of the block
+};
+
+// the `k` largest of `n` keys in shared memory (which it takes out), by one warp, into out[]; 0 where there are
+// fewer. Returns how many
+__device__ __forceinline__ int pick_largest(uint64_t *keys, int n, int k, uint64_t *out) {
+  const int lane = threadIdx.x & 31;
+  int got = 0;
+  for (int i = 0; i < k; ++i) {
+    uint64_t best = 0;
+    int at = -1;
+    for (int j = lane; j < n; j += 32) {
+      const uint64_t key = keys[j];
+      if (key > best) {
+        best = key;
+        at = j;
+      }
+    }
+    const uint64_t most = warp_max_key(best);
+    if (most != 0) ++got;
+    if (at >= 0 && best == most) keys[at] = 0;  // keys are unique
+    if (lane == 0) out[i] = most;
+    __syncwarp();
+  }
+  return got;
+}
+
+template <typename T>
+__global__ void __launch_bounds__(32 * kLogWarps, 2)
+    logprob_kernel(const LogprobParams p, const LogprobPtrs a, uint32_t blocks_a_row) {
+  using Row = LogitRow<T>;
+  constexpr int V = Row::V, AT_ONCE = 4;
+  __shared__ LogShared sh;
   pdl_launch_dependents();
   pdl_wait();
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  for (int64_t row = blockIdx.x; row < p.rows; row += gridDim.x) {
-    T const *x = static_cast<T const *>(a.x) + row * p.s_x;
-    float m = -INFINITY;
-    for (int64_t c = threadIdx.x; c < p.vocab; c += kLogThreads) m = fmaxf(m, to_f32(x[c]));
-    for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-    __syncthreads();
-    if (lane == 0) red[0][warp] = m;
-    __syncthreads();
-    for (int w = 0; w < kLogThreads / 32; ++w) m = fmaxf(m, red[0][w]);
-    const float ref = m == -INFINITY ? 0.f : m;
-    float S = 0.f, U = 0.f;
-    for (int64_t c = threadIdx.x; c < p.vocab; c += kLogThreads) {
-      const float d = to_f32(x[c]) - ref;
-      const float e = expf(d);
-      S += e;
-      U += d == -INFINITY ? 0.f : d * e;
+  const int threads = blockDim.x, warps = threads >> 5, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t rank = blocks_a_row > 1 ? cluster_ctarank() : 0u;
+  for (int64_t row = blockIdx.x / blocks_a_row; row < p.rows; row += gridDim.x / blocks_a_row) {
+    const Row x(static_cast<T const *>(a.x) + row * p.s_x, p.vocab);
+    const int p0 = (int)((int64_t)x.pieces * rank / blocks_a_row);
+    const int p1 = (int)((int64_t)x.pieces * (rank + 1) / blocks_a_row);
+    // ---- the pass
+    LogSums v{-INFINITY, 0.f, 0.f};
+    float2 S2 = make_float2(0.f, 0.f), U2 = make_float2(0.f, 0.f);
+    float R = 0.f, best = -INFINITY;
+    int best_piece = -1;
+    for (int q = p0 + (int)threadIdx.x; q < p1; q += AT_ONCE * threads) {
+      typename Row::Piece c[AT_ONCE];
+#pragma unroll
+      for (int i = 0; i < AT_ONCE; ++i) {
+        if (q + i * threads < p1) {
+          c[i] = x.load(q + i * threads);
+        } else {
+#pragma unroll
+          for (int w = 0; w < Row::Piece::kWords; ++w) c[i].w[w] = sizeof(T) == 4 ? 0xff800000u : 0xff80ff80u;
+        }
+      }
+      float most = -INFINITY;
+#pragma unroll
+      for (int i = 0; i < AT_ONCE; ++i) {
+        const float l = Row::largest(c[i]);
+        if (q + i * threads < p1 && (l > best || best_piece < 0)) {
+          best = l;
+          best_piece = q + i * threads;
+        }
+        most = fmaxf(most, l);
+      }
+      if (most > v.m) {
+        v.m = most;
+        const float to = log_ref(most), d = R - to, e = exp2_fast(d);
+        // (from R = 0 of the start the sums are 0 as yet)
+        U2 = S2.x + S2.y == 0.f ? U2 : make_float2(e * (U2.x + d * S2.x), e * (U2.y + d * S2.y));
+        S2 = S2.x + S2.y == 0.f ? S2 : make_float2(e * S2.x, e * S2.y);
+        R = to;
+      }
+#pragma unroll
+      for (int i = 0; i < AT_ONCE; ++i)
+#pragma unroll
+        for (int e = 0; e < V; e += 2) {
+          float2 d = fma2(c[i].get2(e), make_float2(kLog2e, kLog2e), make_float2(-R, -R));
+          d = make_float2(max_nan(d.x, -200.f), max_nan(d.y, -200.f));
+          const float2 t = make_float2(exp2_fast(d.x), exp2_fast(d.y));
+          S2 = add2(S2, t);
+          U2 = fma2(d, t, U2);
+        }
     }
-    S = warp_sum(S);
-    U = warp_sum(U);
+    v.S = S2.x + S2.y;
+    v.U = U2.x + U2.y;
+    // ---- the block's sums, and the threads' largest logits
+    v = log_join_lanes(v);
     if (lane == 0) {
-      red[1][warp] = S;
-      red[2][warp] = U;
+      sh.red[warp] = v.m;
+      sh.red[32 + warp] = v.S;
+      sh.red[64 + warp] = v.U;
     }
+    if (p.top > 0)  // (the end of the piece stands for the logit's place: a lower bound)
+      sh.keys[threadIdx.x] = best_piece < 0 ? 0 : rank_key(best, (uint32_t)(x.first_index(best_piece) + V - 1));
+    if (threadIdx.x == 0) sh.n_found = 0;
     __syncthreads();
-    S = U = 0.f;
-    for (int w = 0; w < kLogThreads / 32; ++w) {
-      S += red[1][w];
-      U += red[2][w];
-    }
-    const bool none = S == 0.f;
-    const float log_s = logf(S), lse = none ? -INFINITY : ref + log_s;
-    if (threadIdx.x == 0) {
-      if (a.lse) a.lse[row] = lse;
-      if (a.entropy) a.entropy[row] = none ? 0.f : log_s - U / S;
-      if (a.targets) {
-        const int64_t t = a.targets[row];
-        a.logprob[row] = t < 0 ? 0.f : (t >= p.vocab ? logit_nan() : (none ? -INFINITY : to_f32(x[t]) - ref - log_s));
-      }
-    }
-    uint64_t last = ~0ull;  // every key is below
-    for (int i = 0; i < p.top; ++i) {
-      uint64_t k = 0;
-      for (int64_t c = threadIdx.x; c < p.vocab; c += kLogThreads) {
-        const uint64_t key = rank_key(to_f32(x[c]), (uint32_t)c);
-        if (key < last || i == 0) k = key > k ? key : k;
-      }
-      for (int o = 16; o > 0; o >>= 1) {
-        const uint64_t other = __shfl_xor_sync(0xffffffffu, k, o);
-        k = other > k ? other : k;
+    v = log_join_lanes(lane < warps ? LogSums{sh.red[lane], sh.red[32 + lane], sh.red[64 + lane]}
+                                    : LogSums{-INFINITY, 0.f, 0.f});
+    // ---- the block's alternatives
+    bool full = false;
+    if (p.top > 0) {
+      if (warp == 0) {
+        const int n = pick_largest(sh.keys, threads, p.top, sh.chosen);
+        if (lane == 0) sh.n_chosen = n;
       }
       __syncthreads();
-      if (lane == 0) best[warp] = k;
+      const int n = sh.n_chosen;
+      const uint64_t bound = n < p.top ? 0 : sh.chosen[p.top - 1];
+      for (int i = warp; i < n; i += warps) {
+        // the thread that holds chosen[i] read every threads-th piece from `first` on
+        const int end = (int)~(uint32_t)sh.chosen[i];
+        const int first = p0 + ((end - (V - 1) + x.off) / V - p0) % threads;
+        for (int q = first + lane * threads; q < p1; q += 32 * threads) {
+          const typename Row::Piece c = x.load(q);
+#pragma unroll
+          for (int e = 0; e < V; ++e) {
+            const int at = x.first_index(q) + e;
+            const uint64_t key = rank_key(c.get(e), (uint32_t)at);
+            if (at < 0 || at >= x.vocab || key < bound) continue;
+            const int slot = atomicAdd(&sh.n_found, 1);
+            if (slot < kCandidates) sh.found[slot] = key;
+          }
+        }
+      }
       __syncthreads();
-      for (int w = 0; w < kLogThreads / 32; ++w) k = best[w] > k ? best[w] : k;
-      last = k;
+      full = sh.n_found > kCandidates;
+      if (warp == 0 && !full) pick_largest(sh.found, sh.n_found, p.top, sh.top);
+    }
+    // (S is NaN where the row holds a NaN or +infinity)
+    bool odd = full || !(v.S == v.S) || v.m > 1e37f || (v.m < kLowest && v.m != -INFINITY);
+    if (blocks_a_row > 1) {
       if (threadIdx.x == 0) {
-        const uint32_t at = ~(uint32_t)k;
-        if (a.top_index) a.top_index[row * p.top + i] = at;
-        if (a.top_logprob) a.top_logprob[row * p.top + i] = none ? -INFINITY : to_f32(x[at]) - ref - log_s;
+        sh.sums = v;
+        sh.odd = odd;
       }
+      __syncwarp();
+      cluster_sync();  // every block's sums and alternatives are in its shared memory
+      if (rank == 0) {
+        // all blocks' sums (each lane a block's), and the largest of all alternatives
+        LogSums w{-INFINITY, 0.f, 0.f};
+        int any = 0;
+        if (lane < (int)blocks_a_row) {
+          const uint32_t sums = mapa_shared(smem_u32(&sh.sums), lane);
+          w = LogSums{__uint_as_float(ld_cluster_u32(sums)), __uint_as_float(ld_cluster_u32(sums + 4)),
+                      __uint_as_float(ld_cluster_u32(sums + 8))};
+          any = (int)ld_cluster_u32(mapa_shared(smem_u32(&sh.odd), lane));
+        }
+        v = log_join_lanes(w);
+        // a part that is odd by itself (nothing above kLowest) need not be so in the whole row
+        odd = !(v.S == v.S) || v.m > 1e37f || (v.m < kLowest && v.m != -INFINITY);
+        if (p.top > 0) odd = odd || __any_sync(0xffffffffu, any != 0);
+        if (p.top > 0 && !odd && warp == 0) {
+          for (int i = lane; i < p.top * (int)blocks_a_row; i += 32) {
+            const uint32_t key = mapa_shared(smem_u32(&sh.top[i % p.top]), i / p.top);
+            sh.found[i] = (uint64_t)ld_cluster_u32(key) | (uint64_t)ld_cluster_u32(key + 4) << 32;
+          }
+          __syncwarp();
+          pick_largest(sh.found, p.top * (int)blocks_a_row, p.top, sh.chosen);
+        }
+      }
+    }
+    if (rank == 0) {
+      if (odd) {
+        __syncthreads();
+        logprob_plain_row<T>(p, a, row, sh.red, sh.chosen);
+      } else if (warp == 0) {
+        const bool none = v.S == 0.f;
+        const float ref = log_ref(v.m), log_s = log2f(v.S);
+        if (lane == 0) {
+          const int64_t t = a.targets ? a.targets[row] : -1;
+          float xt = 0.f;
+          if (t >= 0 && t < p.vocab) xt = to_f32(static_cast<T const *>(a.x)[row * p.s_x + t]);
+          logprob_row_values(p, a, row, none, none ? -INFINITY : (ref + log_s) * kLn2, (log_s - v.U / v.S) * kLn2,
+                             log_prob(xt, v, log_s));
+        }
+        if (lane < p.top) {
+          const uint64_t key = (blocks_a_row > 1 ? sh.chosen : sh.top)[lane];
+          const float xt = rank_value((uint32_t)(key >> 32));
+          if (a.top_index) a.top_index[row * p.top + lane] = ~(uint32_t)key;
+          if (a.top_logprob)
+            a.top_logprob[row * p.top + lane] = none ? -INFINITY : log_prob(xt, v, log_s);
+        }
+      }
+    }
+    if (blocks_a_row > 1) {
+      __syncwarp();
+      cluster_sync();  // no block goes on while its shared memory is read
+    } else {
+      __syncthreads();
     }
   }
 }
 
-// p = e^(x - lse) of one logit, and its gradient
-__device__ __forceinline__ float logit_grad(float x, float lse, float dlp, float dent, float ent) {
-  const float d = x - lse;
-  const float pr = expf(d);
-  float g = -dlp * pr;
-  if (dent != 0.f && pr != 0.f) g -= dent * pr * (d + ent);
-  return g;
-}
+// ---------------------------------------------------------------- backward
 
-template <typename T>
-__global__ void __launch_bounds__(kLogThreads) logprob_backward_kernel(const LogprobParams p,
-                                                                       const LogprobGradPtrs a) {
+// 16-byte units of the gradient's row a thread at a time. SAME: the logits lie alike on the grid; else they are
+// shifted into place
+template <typename T, bool SAME>
+__global__ void __launch_bounds__(256) logprob_backward_kernel(const LogprobParams p, const LogprobGradPtrs a,
+                                                               int blocks_a_row) {
+  using Row = LogitRow<T>;
+  constexpr int V = Row::V;
   pdl_launch_dependents();
   pdl_wait();
-  for (int64_t row = blockIdx.x; row < p.rows; row += gridDim.x) {
+  const uintptr_t begin = reinterpret_cast<uintptr_t>(a.x);
+  const uintptr_t end = begin + (uintptr_t)(((p.rows - 1) * p.s_x + p.vocab) * (int64_t)sizeof(T));
+  for (int64_t unit = blockIdx.x; unit < p.rows * blocks_a_row; unit += gridDim.x) {
+    const int64_t row = unit / blocks_a_row;
+    const int part = (int)(unit - row * blocks_a_row);
     T const *x = static_cast<T const *>(a.x) + row * p.s_x;
     T *dx = static_cast<T *>(a.dx) + row * p.s_dx;
+    const Row out(dx, p.vocab);
+    const int q0 = (int)((int64_t)out.pieces * part / blocks_a_row);
+    const int q1 = (int)((int64_t)out.pieces * (part + 1) / blocks_a_row);
     const float lse = a.lse[row];
     const int64_t t = a.targets ? a.targets[row] : -1;
     float dlp = t >= 0 ? a.dlogprob[row] : 0.f;
     if (t >= p.vocab) dlp = logit_nan();
-    const float dent = a.dentropy ? a.dentropy[row] : 0.f, ent = a.dentropy ? a.entropy[row] : 0.f;
+    const float dent = a.dentropy ? a.dentropy[row] : 0.f;
+    // dx = -p (dlp + dent (x - lse + H)) = p (k0 + k1 d), d = (x - lse) log2 e
+    const float k0 = -dlp - dent * (a.dentropy ? a.entropy[row] : 0.f), k1 = -dent * kLn2;
     const bool none = lse == -INFINITY;
-    for (int64_t c = threadIdx.x; c < p.vocab; c += kLogThreads) {
-      float g = none ? 0.f : logit_grad(to_f32(x[c]), lse, dlp, dent, ent);
-      if (c == t && !none) g += dlp;
-      dx[c] = from_f32<T>(g);
+#pragma unroll 4
+    for (int q = q0 + (int)threadIdx.x; q < q1; q += 256) {
+      const int i0 = out.first_index(q);
+      typename Row::Piece c, g;
+      if (SAME) c = Row(x, p.vocab).load(q);
+      else if (i0 >= 0 && i0 <= p.vocab - V) c.load_any(x, i0, p.vocab, begin, end);
+      float f[V];
+#pragma unroll
+      for (int e = 0; e < V; e += 2) {
+        float2 xv;
+        if (SAME || (i0 >= 0 && i0 <= p.vocab - V)) {
+          xv = c.get2(e);
+        } else {
+          xv.x = i0 + e >= 0 && i0 + e < p.vocab ? to_f32(x[i0 + e]) : 0.f;
+          xv.y = i0 + e + 1 >= 0 && i0 + e + 1 < p.vocab ? to_f32(x[i0 + e + 1]) : 0.f;
+        }
+        float2 d = mul2(add2(xv, make_float2(-lse, -lse)), make_float2(kLog2e, kLog2e));
+        // (2^-200 is 0 in FP32: a ruled-out logit gets 0, not 0 times infinity)
+        d = make_float2(max_nan(d.x, -200.f), max_nan(d.y, -200.f));
+        const float2 pr = make_float2(exp2_fast(d.x), exp2_fast(d.y));
+        const float2 r = mul2(pr, fma2(d, make_float2(k1, k1), make_float2(k0, k0)));
+        f[e] = none ? 0.f : r.x;
+        f[e + 1] = none ? 0.f : r.y;
+      }
+      if (t >= i0 && t < i0 + V && !none) {
+#pragma unroll
+        for (int e = 0; e < V; ++e)
+          if (t == i0 + e) f[e] += dlp;
+      }
+      g.set(f);
+      if (i0 >= 0 && i0 <= p.vocab - V) g.store(dx + i0);
+      else g.store_some(dx + i0, i0 < 0 ? -i0 : 0, p.vocab - i0 < V ? (int)(p.vocab - i0) : V);
     }
   }
 }
 
-static dim3 logprob_grid(int64_t rows, int num_sms) {
-  const int64_t most = (int64_t)num_sms * 8;
-  return dim3((unsigned)(rows < most ? rows : most));
-}
+// ---------------------------------------------------------------- launchers
 
 cudaError_t launch_logprob(LogprobParams const &p, LogprobPtrs const &a, int num_sms, cudaStream_t st) {
+  const int64_t pieces = (p.vocab * (p.dt == EIR_FP32 ? 4 : 2) + 15) / 16 + 1;
+  // a block a row where the rows fill the SMs; else clusters of up to 8, with
+  // at least 256 pieces a block
+  uint32_t blocks = 1;
+  while (blocks < 8 && p.rows * blocks * 2 <= 2 * num_sms && pieces >= 512 * (int64_t)blocks) blocks *= 2;
+  const int threads = pieces <= 512 ? 128 : blocks > 1 || pieces > 16384 ? 512 : 256;
+  const int64_t fit = (int64_t)num_sms * (1024 / threads);
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(std::min<int64_t>(p.rows, std::max<int64_t>(1, fit / blocks)) * blocks));
+  cfg.blockDim = dim3(threads);
+  cfg.stream = st;
+  cudaLaunchAttribute attr[2];
+  int n = 0;
+  if (pdl_enabled()) {
+    attr[n].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[n++].val.programmaticStreamSerializationAllowed = 1;
+  }
+  if (blocks > 1) {
+    attr[n].id = cudaLaunchAttributeClusterDimension;
+    attr[n].val.clusterDim.x = blocks;
+    attr[n].val.clusterDim.y = attr[n].val.clusterDim.z = 1;
+    ++n;
+  }
+  cfg.attrs = attr;
+  cfg.numAttrs = n;
   auto kern = p.dt == EIR_FP32 ? logprob_kernel<float> : logprob_kernel<__nv_bfloat16>;
-  return launch_kernel(kern, logprob_grid(p.rows, num_sms), dim3(kLogThreads), 0, st, p, a);
+  return cudaLaunchKernelEx(&cfg, kern, p, a, blocks);
+}
+
+template <typename T>
+static cudaError_t launch_logprob_backward_t(LogprobParams const &p, LogprobGradPtrs const &a, int num_sms,
+                                             cudaStream_t st) {
+  const int64_t pieces = (p.vocab * (int64_t)sizeof(T) + 15) / 16 + 1, most = (int64_t)num_sms * 8;
+  int64_t blocks = 1;  // of a row: until the GPU is full, or a thread has four pieces
+  while (p.rows * blocks < most && pieces > 1024 * blocks) blocks *= 2;
+  const bool same = (reinterpret_cast<uintptr_t>(a.x) - reinterpret_cast<uintptr_t>(a.dx)) % 16 == 0 &&
+                    (p.rows == 1 || (p.s_x - p.s_dx) * (int64_t)sizeof(T) % 16 == 0);
+  auto kern = same ? logprob_backward_kernel<T, true> : logprob_backward_kernel<T, false>;
+  return launch_kernel(kern, dim3((unsigned)std::min(p.rows * blocks, most)), dim3(256), 0, st, p, a, (int)blocks);
 }
 
 cudaError_t launch_logprob_backward(LogprobParams const &p, LogprobGradPtrs const &a, int num_sms,
                                     cudaStream_t st) {
-  auto kern = p.dt == EIR_FP32 ? logprob_backward_kernel<float> : logprob_backward_kernel<__nv_bfloat16>;
-  return launch_kernel(kern, logprob_grid(p.rows, num_sms), dim3(kLogThreads), 0, st, p, a);
+  return p.dt == EIR_FP32 ? launch_logprob_backward_t<float>(p, a, num_sms, st)
+                          : launch_logprob_backward_t<__nv_bfloat16>(p, a, num_sms, st);
 }
 
 }  // namespace eir

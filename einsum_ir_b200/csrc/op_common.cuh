@@ -38,6 +38,13 @@ __device__ __forceinline__ float warp_sum(float v) {
   return v;
 }
 
+// a word of another block's shared memory (a shared::cluster address)
+__device__ __forceinline__ uint32_t ld_cluster_u32(uint32_t addr_cluster) {
+  uint32_t v;
+  asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(addr_cluster) : "memory");
+  return v;
+}
+
 // packed FP32 arithmetic: two roundings of one instruction
 __device__ __forceinline__ float2 mul2(float2 a, float2 b) {
   float2 r;

@@ -5,8 +5,8 @@
 // maximum times L, S = sum 2^d and U = sum d 2^d for d = x L - R give
 // lse = (R + log2 S) / L, log p = (d - log2 S) / L and entropy = (log2 S - U / S) / L. Any R will do, so
 // rounding it costs nothing; a thread raises its own when it meets a larger logit and its
-// sums shrink by 2^(R - R'). d is floored at -200, where 2^d is 0 in FP32, so that
-// a ruled-out logit (-infinity) adds 0 d = 0 to U.
+// sums shrink by 2^(R - R'). Logits are floored at -1e37, where 2^d is 0, so that
+// a ruled-out one (-infinity) adds 0 d = 0 to U.
 //
 // Bound by HBM (a logit is read once; the one exponential an element takes 73 %
 // of the SM's rate at BF16 and full bandwidth). A piece is 16 bytes of memory on
@@ -37,8 +37,6 @@ namespace eir {
 
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 constexpr float kLowest = -1e37f;  // logits below count as ruled out in the fast pass
-constexpr int kLogWarps = 16;      // of a block, at most
-constexpr int kCandidates = 1024;
 
 __device__ __forceinline__ float exp2_fast(float x) {
   float r;
@@ -84,26 +82,20 @@ __device__ __forceinline__ float log_ref(float m) { return m < kLowest ? 0.f : m
 __device__ __forceinline__ float log_prob(float x, LogSums const &v, float log_s) {
   return x < kLowest ? x - v.m : (fmaf(x, kLog2e, -log_ref(v.m)) - log_s) * kLn2;
 }
-// the sums of both, against the larger maximum
-__device__ __forceinline__ LogSums log_join(LogSums a, LogSums b) {
-  LogSums r;
-  r.m = fmaxf(a.m, b.m);
-  const float R = log_ref(r.m), da = log_ref(a.m) - R, db = log_ref(b.m) - R;
-  // (sums of 0 may stand beside any reference)
-  const float ea = a.S == 0.f ? 0.f : exp2_fast(da), eb = b.S == 0.f ? 0.f : exp2_fast(db);
-  r.S = a.S * ea + b.S * eb;
-  r.U = (a.S == 0.f ? 0.f : ea * (a.U + da * a.S)) + (b.S == 0.f ? 0.f : eb * (b.U + db * b.S));
-  return r;
+// sums moved to the reference of a larger maximum (sums of 0 may stand beside any reference)
+__device__ __forceinline__ LogSums log_rebase(LogSums v, float m) {
+  const float d = log_ref(v.m) - log_ref(m), e = exp2_fast(d);
+  if (v.S == 0.f) return LogSums{m, 0.f, 0.f};
+  return LogSums{m, e * v.S, e * (v.U + d * v.S)};
 }
+// the sums of the warp's lanes
 __device__ __forceinline__ LogSums log_join_lanes(LogSums v) {
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    LogSums w;
-    w.m = __shfl_xor_sync(0xffffffffu, v.m, o);
-    w.S = __shfl_xor_sync(0xffffffffu, v.S, o);
-    w.U = __shfl_xor_sync(0xffffffffu, v.U, o);
-    v = log_join(v, w);
-  }
+  // (signed integers in the order of the floats; a NaN is no maximum here, but stays in S)
+  const int b = __float_as_int(v.m == v.m ? v.m : -INFINITY);
+  const int most = __reduce_max_sync(0xffffffffu, b ^ ((b >> 31) & 0x7fffffff));
+  v = log_rebase(v, __int_as_float(most ^ ((most >> 31) & 0x7fffffff)));
+  v.S = warp_sum(v.S);
+  v.U = warp_sum(v.U);
   return v;
 }
 
@@ -219,6 +211,27 @@ struct LogitRow {
     }
     return v;
   }
+  static __device__ __forceinline__ Piece none() {
+    Piece v;
+#pragma unroll
+    for (int i = 0; i < Piece::kWords; ++i) v.w[i] = sizeof(T) == 4 ? 0xff800000u : 0xff80ff80u;
+    return v;
+  }
+  // the piece with its elements not below kLowest (NaNs stay), so that none is infinitely far below the reference
+  static __device__ __forceinline__ Piece floored(Piece v) {
+    if constexpr (sizeof(T) == 4) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) v.w[i] = __float_as_uint(max_nan(v.get(i), kLowest));
+    } else {
+      const __nv_bfloat162 low = __float2bfloat162_rn(kLowest);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const __nv_bfloat162 b = __hmax2_nan(*reinterpret_cast<__nv_bfloat162 const *>(&v.w[i]), low);
+        v.w[i] = *reinterpret_cast<uint32_t const *>(&b);
+      }
+    }
+    return v;
+  }
   // the largest element (a NaN counts as absent)
   static __device__ __forceinline__ float largest(Piece const &v) {
     if constexpr (sizeof(T) == 4) {
@@ -233,49 +246,60 @@ struct LogitRow {
   }
 };
 
+template <int THREADS>
 struct LogShared {
+  static constexpr int kCandidates = THREADS < 64 ? 256 : 4 * THREADS;  // (a merge of 8 blocks takes 8 x 32)
   float red[96];           // (m, S, U) of the warps; the plain row's words
-  uint64_t keys[32 * kLogWarps];  // the threads' largest logits
-  uint64_t chosen[32];     // the k largest of them; the plain row's words
+  uint64_t keys[THREADS];  // the threads' largest logits
+  uint64_t plain[32];      // the plain row's words
   uint64_t top[32];        // the block's alternatives
   uint64_t found[kCandidates];
-  int n_chosen, n_found, odd;
+  int n_found, odd;
   LogSums sums;            // of the block
 };
 
-// the `k` largest of `n` keys in shared memory (which it takes out), by one warp, into out[]; 0 where there are
-// fewer. Returns how many
-__device__ __forceinline__ int pick_largest(uint64_t *keys, int n, int k, uint64_t *out) {
+// the largest of the warp's keys below `last`, PER of them a lane; 0: none
+template <int PER>
+__device__ __forceinline__ uint64_t next_largest(uint64_t const (&keys)[PER], uint64_t last) {
+  uint64_t best = 0;
+#pragma unroll
+  for (int i = 0; i < PER; ++i)
+    if (keys[i] < last && keys[i] > best) best = keys[i];
+  return warp_max_key(best);
+}
+// the `k` largest of `n` keys in shared memory by one warp, into lane i's answer (0 where there are fewer)
+__device__ __forceinline__ uint64_t pick_largest(uint64_t const *keys, int n, int k) {
   const int lane = threadIdx.x & 31;
-  int got = 0;
+  uint64_t last = ~0ull, mine = 0;
+  if (n <= 64) {
+    const uint64_t two[2] = {lane < n ? keys[lane] : 0, lane + 32 < n ? keys[lane + 32] : 0};
+    for (int i = 0; i < k; ++i) {
+      last = next_largest<2>(two, last);
+      if (lane == i) mine = last;
+    }
+    return mine;
+  }
   for (int i = 0; i < k; ++i) {
     uint64_t best = 0;
-    int at = -1;
-    for (int j = lane; j < n; j += 32) {
-      const uint64_t key = keys[j];
-      if (key > best) {
-        best = key;
-        at = j;
-      }
-    }
-    const uint64_t most = warp_max_key(best);
-    if (most != 0) ++got;
-    if (at >= 0 && best == most) keys[at] = 0;  // keys are unique
-    if (lane == 0) out[i] = most;
-    __syncwarp();
+    for (int j = lane; j < n; j += 32)
+      if (keys[j] < last && keys[j] > best) best = keys[j];
+    last = warp_max_key(best);
+    if (lane == i) mine = last;
   }
-  return got;
+  return mine;
 }
 
-template <typename T>
-__global__ void __launch_bounds__(32 * kLogWarps, 2)
+template <typename T, int THREADS>
+__global__ void __launch_bounds__(THREADS, 1024 / THREADS)
     logprob_kernel(const LogprobParams p, const LogprobPtrs a, uint32_t blocks_a_row) {
   using Row = LogitRow<T>;
-  constexpr int V = Row::V, AT_ONCE = 4;
-  __shared__ LogShared sh;
+  using Piece = typename Row::Piece;
+  constexpr int V = Row::V, AT_ONCE = 4, threads = THREADS, warps = THREADS / 32;
+  __shared__ LogShared<THREADS> sh;
+  constexpr int kCandidates = LogShared<THREADS>::kCandidates;
   pdl_launch_dependents();
   pdl_wait();
-  const int threads = blockDim.x, warps = threads >> 5, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t rank = blocks_a_row > 1 ? cluster_ctarank() : 0u;
   for (int64_t row = blockIdx.x / blocks_a_row; row < p.rows; row += gridDim.x / blocks_a_row) {
     const Row x(static_cast<T const *>(a.x) + row * p.s_x, p.vocab);
@@ -284,51 +308,61 @@ __global__ void __launch_bounds__(32 * kLogWarps, 2)
     // ---- the pass
     LogSums v{-INFINITY, 0.f, 0.f};
     float2 S2 = make_float2(0.f, 0.f), U2 = make_float2(0.f, 0.f);
-    float R = 0.f, best = -INFINITY;
-    int best_piece = -1;
-    for (int q = p0 + (int)threadIdx.x; q < p1; q += AT_ONCE * threads) {
-      typename Row::Piece c[AT_ONCE];
+    float R = 0.f;
+    int best = p0 + (int)threadIdx.x;  // the piece that holds v.m
+    auto add_pieces = [&](Piece const (&c)[AT_ONCE], int q) {
+      float l[AT_ONCE], most = -INFINITY;
 #pragma unroll
       for (int i = 0; i < AT_ONCE; ++i) {
-        if (q + i * threads < p1) {
-          c[i] = x.load(q + i * threads);
-        } else {
-#pragma unroll
-          for (int w = 0; w < Row::Piece::kWords; ++w) c[i].w[w] = sizeof(T) == 4 ? 0xff800000u : 0xff80ff80u;
-        }
-      }
-      float most = -INFINITY;
-#pragma unroll
-      for (int i = 0; i < AT_ONCE; ++i) {
-        const float l = Row::largest(c[i]);
-        if (q + i * threads < p1 && (l > best || best_piece < 0)) {
-          best = l;
-          best_piece = q + i * threads;
-        }
-        most = fmaxf(most, l);
+        l[i] = Row::largest(c[i]);
+        most = fmaxf(most, l[i]);
       }
       if (most > v.m) {
         v.m = most;
+#pragma unroll
+        for (int i = AT_ONCE - 1; i >= 0; --i)
+          if (l[i] == most) best = q + i * threads;
         const float to = log_ref(most), d = R - to, e = exp2_fast(d);
-        // (from R = 0 of the start the sums are 0 as yet)
-        U2 = S2.x + S2.y == 0.f ? U2 : make_float2(e * (U2.x + d * S2.x), e * (U2.y + d * S2.y));
-        S2 = S2.x + S2.y == 0.f ? S2 : make_float2(e * S2.x, e * S2.y);
+        if (S2.x + S2.y != 0.f) {  // (sums of 0 may stand beside any reference)
+          U2 = make_float2(e * (U2.x + d * S2.x), e * (U2.y + d * S2.y));
+          S2 = make_float2(e * S2.x, e * S2.y);
+        }
         R = to;
       }
 #pragma unroll
-      for (int i = 0; i < AT_ONCE; ++i)
+      for (int i = 0; i < AT_ONCE; ++i) {
+        const Piece f = Row::floored(c[i]);
 #pragma unroll
         for (int e = 0; e < V; e += 2) {
-          float2 d = fma2(c[i].get2(e), make_float2(kLog2e, kLog2e), make_float2(-R, -R));
-          d = make_float2(max_nan(d.x, -200.f), max_nan(d.y, -200.f));
+          const float2 d = fma2(f.get2(e), make_float2(kLog2e, kLog2e), make_float2(-R, -R));
           const float2 t = make_float2(exp2_fast(d.x), exp2_fast(d.y));
           S2 = add2(S2, t);
           U2 = fma2(d, t, U2);
         }
+      }
+    };
+    {
+      int q = p0 + (int)threadIdx.x;
+      Piece c[AT_ONCE];
+      // the first pieces, which may reach outside the row, and the last ones
+      auto any = [&]() {
+#pragma unroll
+        for (int i = 0; i < AT_ONCE; ++i) c[i] = q + i * threads < p1 ? x.load(q + i * threads) : Row::none();
+        add_pieces(c, q);
+        q += AT_ONCE * threads;
+      };
+      if (q < p1) any();
+      for (; q + (AT_ONCE - 1) * threads < p1 - 1; q += AT_ONCE * threads) {
+#pragma unroll
+        for (int i = 0; i < AT_ONCE; ++i) c[i].template load<false>(x.base + (int64_t)(q + i * threads) * 16);
+        add_pieces(c, q);
+      }
+      if (q < p1) any();
     }
     v.S = S2.x + S2.y;
     v.U = U2.x + U2.y;
     // ---- the block's sums, and the threads' largest logits
+    const float own = v.m;
     v = log_join_lanes(v);
     if (lane == 0) {
       sh.red[warp] = v.m;
@@ -336,7 +370,7 @@ __global__ void __launch_bounds__(32 * kLogWarps, 2)
       sh.red[64 + warp] = v.U;
     }
     if (p.top > 0)  // (the end of the piece stands for the logit's place: a lower bound)
-      sh.keys[threadIdx.x] = best_piece < 0 ? 0 : rank_key(best, (uint32_t)(x.first_index(best_piece) + V - 1));
+      sh.keys[threadIdx.x] = best < p1 ? rank_key(own, (uint32_t)(x.first_index(best) + V - 1)) : 0;
     if (threadIdx.x == 0) sh.n_found = 0;
     __syncthreads();
     v = log_join_lanes(lane < warps ? LogSums{sh.red[lane], sh.red[32 + lane], sh.red[64 + lane]}
@@ -344,19 +378,25 @@ __global__ void __launch_bounds__(32 * kLogWarps, 2)
     // ---- the block's alternatives
     bool full = false;
     if (p.top > 0) {
-      if (warp == 0) {
-        const int n = pick_largest(sh.keys, threads, p.top, sh.chosen);
-        if (lane == 0) sh.n_chosen = n;
+      // every warp finds the k largest of the threads' logits, and reads the pieces of some of these threads
+      uint64_t keys[warps], last = ~0ull, mine = 0;
+#pragma unroll
+      for (int i = 0; i < warps; ++i) keys[i] = sh.keys[32 * i + lane];
+      int n = 0;
+      for (int i = 0; i < p.top; ++i) {
+        last = next_largest<warps>(keys, last);
+        if (last == 0) break;
+        ++n;
+        if (lane == i) mine = last;
       }
-      __syncthreads();
-      const int n = sh.n_chosen;
-      const uint64_t bound = n < p.top ? 0 : sh.chosen[p.top - 1];
+      const uint64_t bound = last;  // 0: fewer threads than alternatives, every logit may be one
       for (int i = warp; i < n; i += warps) {
-        // the thread that holds chosen[i] read every threads-th piece from `first` on
-        const int end = (int)~(uint32_t)sh.chosen[i];
+        // the thread that holds the i-th read every threads-th piece from `first` on
+        const int end = (int)~(uint32_t)__shfl_sync(0xffffffffu, mine, i);
         const int first = p0 + ((end - (V - 1) + x.off) / V - p0) % threads;
         for (int q = first + lane * threads; q < p1; q += 32 * threads) {
-          const typename Row::Piece c = x.load(q);
+          const Piece c = x.load(q);
+          if (rank_key(Row::largest(c), 0) < bound) continue;  // (no index is above 2^32 - 1 - 0)
 #pragma unroll
           for (int e = 0; e < V; ++e) {
             const int at = x.first_index(q) + e;
@@ -369,7 +409,11 @@ __global__ void __launch_bounds__(32 * kLogWarps, 2)
       }
       __syncthreads();
       full = sh.n_found > kCandidates;
-      if (warp == 0 && !full) pick_largest(sh.found, sh.n_found, p.top, sh.top);
+      if (warp == 0 && !full) {
+        const uint64_t t = pick_largest(sh.found, sh.n_found, p.top);
+        sh.top[lane] = t;
+        __syncwarp();
+      }
     }
     // (S is NaN where the row holds a NaN or +infinity)
     bool odd = full || !(v.S == v.S) || v.m > 1e37f || (v.m < kLowest && v.m != -INFINITY);
@@ -400,14 +444,17 @@ __global__ void __launch_bounds__(32 * kLogWarps, 2)
             sh.found[i] = (uint64_t)ld_cluster_u32(key) | (uint64_t)ld_cluster_u32(key + 4) << 32;
           }
           __syncwarp();
-          pick_largest(sh.found, p.top * (int)blocks_a_row, p.top, sh.chosen);
+          const uint64_t t = pick_largest(sh.found, p.top * (int)blocks_a_row, p.top);
+          __syncwarp();
+          sh.found[lane] = t;
+          __syncwarp();
         }
       }
     }
     if (rank == 0) {
       if (odd) {
         __syncthreads();
-        logprob_plain_row<T>(p, a, row, sh.red, sh.chosen);
+        logprob_plain_row<T>(p, a, row, sh.red, sh.plain);
       } else if (warp == 0) {
         const bool none = v.S == 0.f;
         const float ref = log_ref(v.m), log_s = log2f(v.S);
@@ -419,7 +466,7 @@ __global__ void __launch_bounds__(32 * kLogWarps, 2)
                              log_prob(xt, v, log_s));
         }
         if (lane < p.top) {
-          const uint64_t key = (blocks_a_row > 1 ? sh.chosen : sh.top)[lane];
+          const uint64_t key = (blocks_a_row > 1 ? sh.found : sh.top)[lane];
           const float xt = rank_value((uint32_t)(key >> 32));
           if (a.top_index) a.top_index[row * p.top + lane] = ~(uint32_t)key;
           if (a.top_logprob)
@@ -509,10 +556,11 @@ cudaError_t launch_logprob(LogprobParams const &p, LogprobPtrs const &a, int num
   // at least 256 pieces a block
   uint32_t blocks = 1;
   while (blocks < 8 && p.rows * blocks * 2 <= 2 * num_sms && pieces >= 512 * (int64_t)blocks) blocks *= 2;
-  const int threads = pieces <= 512 ? 128 : blocks > 1 || pieces > 16384 ? 512 : 256;
-  const int64_t fit = (int64_t)num_sms * (1024 / threads);
+  // a row's blocks and barriers cost least with few threads, as long as each has some pieces; the rows
+  // that are waiting fill the SMs
+  const int threads = blocks > 1 ? 256 : pieces <= 512 ? 32 : pieces <= 2048 ? 64 : pieces <= 8192 ? 128 : 256;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)(std::min<int64_t>(p.rows, std::max<int64_t>(1, fit / blocks)) * blocks));
+  cfg.gridDim = dim3((unsigned)(p.rows * blocks));
   cfg.blockDim = dim3(threads);
   cfg.stream = st;
   cudaLaunchAttribute attr[2];
@@ -529,7 +577,16 @@ cudaError_t launch_logprob(LogprobParams const &p, LogprobPtrs const &a, int num
   }
   cfg.attrs = attr;
   cfg.numAttrs = n;
-  auto kern = p.dt == EIR_FP32 ? logprob_kernel<float> : logprob_kernel<__nv_bfloat16>;
+  auto pick = [&](auto zero) {
+    using T = decltype(zero);
+    switch (threads) {
+      case 32: return logprob_kernel<T, 32>;
+      case 64: return logprob_kernel<T, 64>;
+      case 128: return logprob_kernel<T, 128>;
+      default: return logprob_kernel<T, 256>;
+    }
+  };
+  auto kern = p.dt == EIR_FP32 ? pick(float{}) : pick(__nv_bfloat16{});
   return cudaLaunchKernelEx(&cfg, kern, p, a, blocks);
 }
 

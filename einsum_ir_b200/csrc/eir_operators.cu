@@ -401,7 +401,7 @@ int eir_logprob(eir_plan *p, void const *logits, int64_t const *targets, float *
   const eir::LogprobPtrs a{logits, targets, logprob, entropy, lse, top_logprob, top_index};
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   ProfScope prof(p, st);
-  return launched(eir::launch_logprob(q, a, num_sms, st), "logprob launch");
+  return launched(eir::launch_logprob(q, a, err, num_sms, st), "logprob launch");
 }
 
 int eir_logprob_backward(eir_plan *p, void const *logits, int64_t const *targets, float const *lse,

@@ -246,6 +246,15 @@ struct LogitRow {
   }
 };
 
+constexpr int kLogStages = 2;  // of a warp, 2 KB each
+
+__device__ __forceinline__ void bulk_copy(void *dst, void const *src, uint32_t bytes, uint64_t *bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
+                   smem_u32(dst)),
+               "l"(src), "r"(bytes), "r"(smem_u32(bar))
+               : "memory");
+}
+
 template <int THREADS>
 struct LogShared {
   static constexpr int kCandidates = THREADS < 64 ? 256 : 4 * THREADS;  // (a merge of 8 blocks takes 8 x 32)
@@ -255,7 +264,10 @@ struct LogShared {
   uint64_t top[32];        // the block's alternatives
   uint64_t found[kCandidates];
   int n_found, odd;
+  volatile int abort;      // a bounded wait has given up
   LogSums sums;            // of the block
+  alignas(8) uint64_t full[THREADS / 32][kLogStages];
+  alignas(128) uint8_t stages[THREADS / 32][kLogStages][2048];
 };
 
 // the largest of the warp's keys below `last`, PER of them a lane; 0: none
@@ -291,195 +303,221 @@ __device__ __forceinline__ uint64_t pick_largest(uint64_t const *keys, int n, in
 
 template <typename T, int THREADS>
 __global__ void __launch_bounds__(THREADS, 1024 / THREADS)
-    logprob_kernel(const LogprobParams p, const LogprobPtrs a, uint32_t blocks_a_row) {
+    logprob_kernel(const LogprobParams p, const LogprobPtrs a, uint32_t blocks_a_row, uint32_t *err) {
   using Row = LogitRow<T>;
   using Piece = typename Row::Piece;
-  constexpr int V = Row::V, AT_ONCE = 4, threads = THREADS, warps = THREADS / 32;
+  constexpr int V = Row::V, AT_ONCE = 4, warps = THREADS / 32, kChunk = 32 * AT_ONCE;
   __shared__ LogShared<THREADS> sh;
   constexpr int kCandidates = LogShared<THREADS>::kCandidates;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (lane == 0) {
+    for (int s = 0; s < kLogStages; ++s) mbar_init(&sh.full[warp][s], 1);
+    fence_barrier_init();
+    if (warp == 0) sh.abort = 0;
+  }
+  __syncthreads();
   pdl_launch_dependents();
   pdl_wait();
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t rank = blocks_a_row > 1 ? cluster_ctarank() : 0u;
-  for (int64_t row = blockIdx.x / blocks_a_row; row < p.rows; row += gridDim.x / blocks_a_row) {
-    const Row x(static_cast<T const *>(a.x) + row * p.s_x, p.vocab);
-    const int p0 = (int)((int64_t)x.pieces * rank / blocks_a_row);
-    const int p1 = (int)((int64_t)x.pieces * (rank + 1) / blocks_a_row);
-    // ---- the pass
-    LogSums v{-INFINITY, 0.f, 0.f};
-    float2 S2 = make_float2(0.f, 0.f), U2 = make_float2(0.f, 0.f);
-    float R = 0.f;
-    int best = p0 + (int)threadIdx.x;  // the piece that holds v.m
-    auto add_pieces = [&](Piece const (&c)[AT_ONCE], int q) {
-      float l[AT_ONCE], most = -INFINITY;
+  // A warp takes every warps-th chunk of its block's part of a row. Chunks that lie inside the row come through
+  // the warp's own stages, copied in bulk ahead of their use; the row's first and last
+  // chunk are read piece by piece
+  const int64_t row = blockIdx.x / blocks_a_row;
+  const Row x(static_cast<T const *>(a.x) + row * p.s_x, p.vocab);
+  const int p0 = (int)((int64_t)x.pieces * rank / blocks_a_row);
+  const int p1 = (int)((int64_t)x.pieces * (rank + 1) / blocks_a_row);
+  const int chunks = (p1 - p0 + kChunk - 1) / kChunk;
+  const int inner0 = p0 == 0 ? 1 : 0, inner1 = (p1 == x.pieces ? p1 - 1 - p0 : p1 - p0) / kChunk;
+  auto inner = [&](int k) { return k >= inner0 && k < inner1; };
+  auto copy = [&](int k, int stage) {
+    mbar_arrive_expect_tx(&sh.full[warp][stage], kChunk * 16);
+    bulk_copy(sh.stages[warp][stage], x.base + (int64_t)(p0 + k * kChunk) * 16, kChunk * 16, &sh.full[warp][stage]);
+  };
+  if (lane == 0) {
+    const int k0 = inner(warp) ? warp : warp + warps;  // the warp's first inner chunk, if it has any
+    for (int s = 0; s < kLogStages; ++s)
+      if (inner(k0 + s * warps)) copy(k0 + s * warps, s);
+  }
+  uint32_t phases = 0;  // of the warp's stages
+  int stage = 0;
+  // ---- the pass
+  LogSums v{-INFINITY, 0.f, 0.f};
+  float2 S2 = make_float2(0.f, 0.f), U2 = make_float2(0.f, 0.f);
+  float R = 0.f;
+  int best = p0 + warp * kChunk + lane;  // the piece that holds v.m
+  auto add_pieces = [&](Piece const (&c)[AT_ONCE], int q) {
+    float l[AT_ONCE], most = -INFINITY;
 #pragma unroll
-      for (int i = 0; i < AT_ONCE; ++i) {
-        l[i] = Row::largest(c[i]);
-        most = fmaxf(most, l[i]);
-      }
-      if (most > v.m) {
-        v.m = most;
-#pragma unroll
-        for (int i = AT_ONCE - 1; i >= 0; --i)
-          if (l[i] == most) best = q + i * threads;
-        const float to = log_ref(most), d = R - to, e = exp2_fast(d);
-        if (S2.x + S2.y != 0.f) {  // (sums of 0 may stand beside any reference)
-          U2 = make_float2(e * (U2.x + d * S2.x), e * (U2.y + d * S2.y));
-          S2 = make_float2(e * S2.x, e * S2.y);
-        }
-        R = to;
-      }
-#pragma unroll
-      for (int i = 0; i < AT_ONCE; ++i) {
-        const Piece f = Row::floored(c[i]);
-#pragma unroll
-        for (int e = 0; e < V; e += 2) {
-          const float2 d = fma2(f.get2(e), make_float2(kLog2e, kLog2e), make_float2(-R, -R));
-          const float2 t = make_float2(exp2_fast(d.x), exp2_fast(d.y));
-          S2 = add2(S2, t);
-          U2 = fma2(d, t, U2);
-        }
-      }
-    };
-    {
-      int q = p0 + (int)threadIdx.x;
-      Piece c[AT_ONCE];
-      // the first pieces, which may reach outside the row, and the last ones
-      auto any = [&]() {
-#pragma unroll
-        for (int i = 0; i < AT_ONCE; ++i) c[i] = q + i * threads < p1 ? x.load(q + i * threads) : Row::none();
-        add_pieces(c, q);
-        q += AT_ONCE * threads;
-      };
-      if (q < p1) any();
-      for (; q + (AT_ONCE - 1) * threads < p1 - 1; q += AT_ONCE * threads) {
-#pragma unroll
-        for (int i = 0; i < AT_ONCE; ++i) c[i].template load<false>(x.base + (int64_t)(q + i * threads) * 16);
-        add_pieces(c, q);
-      }
-      if (q < p1) any();
+    for (int i = 0; i < AT_ONCE; ++i) {
+      l[i] = Row::largest(c[i]);
+      most = fmaxf(most, l[i]);
     }
-    v.S = S2.x + S2.y;
-    v.U = U2.x + U2.y;
-    // ---- the block's sums, and the threads' largest logits
-    const float own = v.m;
-    v = log_join_lanes(v);
-    if (lane == 0) {
-      sh.red[warp] = v.m;
-      sh.red[32 + warp] = v.S;
-      sh.red[64 + warp] = v.U;
+    if (most > v.m) {
+      v.m = most;
+#pragma unroll
+      for (int i = AT_ONCE - 1; i >= 0; --i)
+        if (l[i] == most) best = q + i * 32;
+      const float to = log_ref(most), d = R - to, e = exp2_fast(d);
+      if (S2.x + S2.y != 0.f) {  // (sums of 0 may stand beside any reference)
+        U2 = make_float2(e * (U2.x + d * S2.x), e * (U2.y + d * S2.y));
+        S2 = make_float2(e * S2.x, e * S2.y);
+      }
+      R = to;
     }
-    if (p.top > 0)  // (the end of the piece stands for the logit's place: a lower bound)
-      sh.keys[threadIdx.x] = best < p1 ? rank_key(own, (uint32_t)(x.first_index(best) + V - 1)) : 0;
-    if (threadIdx.x == 0) sh.n_found = 0;
+#pragma unroll
+    for (int i = 0; i < AT_ONCE; ++i) {
+      const Piece f = Row::floored(c[i]);
+#pragma unroll
+      for (int e = 0; e < V; e += 2) {
+        const float2 d = fma2(f.get2(e), make_float2(kLog2e, kLog2e), make_float2(-R, -R));
+        const float2 t = make_float2(exp2_fast(d.x), exp2_fast(d.y));
+        S2 = add2(S2, t);
+        U2 = fma2(d, t, U2);
+      }
+    }
+  };
+  for (int k = warp; k < chunks; k += warps) {
+    const int q = p0 + k * kChunk + lane;
+    Piece c[AT_ONCE];
+    if (inner(k)) {
+      if (!mbar_wait_bounded(&sh.full[warp][stage], (phases >> stage) & 1u, &sh.abort)) {
+        if (!sh.abort) record_error(err, kErrTimeoutProducer);
+        sh.abort = 1;
+      }
+      phases ^= 1u << stage;
+#pragma unroll
+      for (int i = 0; i < AT_ONCE; ++i) c[i].template load<false>(sh.stages[warp][stage] + (i * 32 + lane) * 16);
+      __syncwarp();
+      if (lane == 0 && inner(k + kLogStages * warps)) copy(k + kLogStages * warps, stage);
+      stage = stage + 1 == kLogStages ? 0 : stage + 1;
+    } else {
+#pragma unroll
+      for (int i = 0; i < AT_ONCE; ++i) c[i] = q + 32 * i < p1 ? x.load(q + 32 * i) : Row::none();
+    }
+    add_pieces(c, q);
+  }
+  v.S = S2.x + S2.y;
+  v.U = U2.x + U2.y;
+  // ---- the block's sums, and the threads' largest logits
+  const float own = v.m;
+  v = log_join_lanes(v);
+  if (lane == 0) {
+    sh.red[warp] = v.m;
+    sh.red[32 + warp] = v.S;
+    sh.red[64 + warp] = v.U;
+  }
+  if (p.top > 0)  // (the end of the piece stands for the logit's place: a lower bound)
+    sh.keys[threadIdx.x] = best < p1 ? rank_key(own, (uint32_t)(x.first_index(best) + V - 1)) : 0;
+  if (threadIdx.x == 0) sh.n_found = 0;
+  __syncthreads();
+  v = log_join_lanes(lane < warps ? LogSums{sh.red[lane], sh.red[32 + lane], sh.red[64 + lane]}
+                                  : LogSums{-INFINITY, 0.f, 0.f});
+  // ---- the block's alternatives
+  bool full = false;
+  if (p.top > 0) {
+    // every warp finds the k largest of the threads' logits, and reads the pieces of some of these threads
+    uint64_t keys[warps], last = ~0ull, mine = 0;
+#pragma unroll
+    for (int i = 0; i < warps; ++i) keys[i] = sh.keys[32 * i + lane];
+    int n = 0;
+    for (int i = 0; i < p.top; ++i) {
+      last = next_largest<warps>(keys, last);
+      if (last == 0) break;
+      ++n;
+      if (lane == i) mine = last;
+    }
+    const uint64_t bound = last;  // 0: fewer threads than alternatives, every logit may be one
+    for (int i = warp; i < n; i += warps) {
+      // the pieces of the thread that holds the i-th: one in 32 of its warp's chunks
+      const int end = (int)~(uint32_t)__shfl_sync(0xffffffffu, mine, i);
+      const int piece = (end - (V - 1) + x.off) / V - p0;
+      const int its_warp = piece / kChunk % warps;
+      for (int j = lane;; j += 32) {
+        const int q = p0 + (j / AT_ONCE * warps + its_warp) * kChunk + j % AT_ONCE * 32 + piece % 32;
+        if (q - j % AT_ONCE * 32 >= p1) break;
+        if (q >= p1) continue;
+        const Piece c = x.load(q);
+        if (rank_key(Row::largest(c), 0) < bound) continue;  // (no index is above 2^32 - 1 - 0)
+#pragma unroll
+        for (int e = 0; e < V; ++e) {
+          const int at = x.first_index(q) + e;
+          const uint64_t key = rank_key(c.get(e), (uint32_t)at);
+          if (at < 0 || at >= x.vocab || key < bound) continue;
+          const int slot = atomicAdd(&sh.n_found, 1);
+          if (slot < kCandidates) sh.found[slot] = key;
+        }
+      }
+    }
     __syncthreads();
-    v = log_join_lanes(lane < warps ? LogSums{sh.red[lane], sh.red[32 + lane], sh.red[64 + lane]}
-                                    : LogSums{-INFINITY, 0.f, 0.f});
-    // ---- the block's alternatives
-    bool full = false;
-    if (p.top > 0) {
-      // every warp finds the k largest of the threads' logits, and reads the pieces of some of these threads
-      uint64_t keys[warps], last = ~0ull, mine = 0;
-#pragma unroll
-      for (int i = 0; i < warps; ++i) keys[i] = sh.keys[32 * i + lane];
-      int n = 0;
-      for (int i = 0; i < p.top; ++i) {
-        last = next_largest<warps>(keys, last);
-        if (last == 0) break;
-        ++n;
-        if (lane == i) mine = last;
+    full = sh.n_found > kCandidates;
+    if (warp == 0 && !full) {
+      const uint64_t t = pick_largest(sh.found, sh.n_found, p.top);
+      sh.top[lane] = t;
+      __syncwarp();
+    }
+  }
+  // (S is NaN where the row holds a NaN or +infinity)
+  bool odd = full || !(v.S == v.S) || v.m > 1e37f || (v.m < kLowest && v.m != -INFINITY);
+  if (blocks_a_row > 1) {
+    if (threadIdx.x == 0) {
+      sh.sums = v;
+      sh.odd = odd;
+    }
+    __syncwarp();
+    cluster_sync();  // every block's sums and alternatives are in its shared memory
+    if (rank == 0) {
+      // all blocks' sums (each lane a block's), and the largest of all alternatives
+      LogSums w{-INFINITY, 0.f, 0.f};
+      int any = 0;
+      if (lane < (int)blocks_a_row) {
+        const uint32_t sums = mapa_shared(smem_u32(&sh.sums), lane);
+        w = LogSums{__uint_as_float(ld_cluster_u32(sums)), __uint_as_float(ld_cluster_u32(sums + 4)),
+                    __uint_as_float(ld_cluster_u32(sums + 8))};
+        any = (int)ld_cluster_u32(mapa_shared(smem_u32(&sh.odd), lane));
       }
-      const uint64_t bound = last;  // 0: fewer threads than alternatives, every logit may be one
-      for (int i = warp; i < n; i += warps) {
-        // the thread that holds the i-th read every threads-th piece from `first` on
-        const int end = (int)~(uint32_t)__shfl_sync(0xffffffffu, mine, i);
-        const int first = p0 + ((end - (V - 1) + x.off) / V - p0) % threads;
-        for (int q = first + lane * threads; q < p1; q += 32 * threads) {
-          const Piece c = x.load(q);
-          if (rank_key(Row::largest(c), 0) < bound) continue;  // (no index is above 2^32 - 1 - 0)
-#pragma unroll
-          for (int e = 0; e < V; ++e) {
-            const int at = x.first_index(q) + e;
-            const uint64_t key = rank_key(c.get(e), (uint32_t)at);
-            if (at < 0 || at >= x.vocab || key < bound) continue;
-            const int slot = atomicAdd(&sh.n_found, 1);
-            if (slot < kCandidates) sh.found[slot] = key;
-          }
+      v = log_join_lanes(w);
+      // a part that is odd by itself (nothing above kLowest) need not be so in the whole row
+      odd = !(v.S == v.S) || v.m > 1e37f || (v.m < kLowest && v.m != -INFINITY);
+      if (p.top > 0) odd = odd || __any_sync(0xffffffffu, any != 0);
+      if (p.top > 0 && !odd && warp == 0) {
+        for (int i = lane; i < p.top * (int)blocks_a_row; i += 32) {
+          const uint32_t key = mapa_shared(smem_u32(&sh.top[i % p.top]), i / p.top);
+          sh.found[i] = (uint64_t)ld_cluster_u32(key) | (uint64_t)ld_cluster_u32(key + 4) << 32;
         }
-      }
-      __syncthreads();
-      full = sh.n_found > kCandidates;
-      if (warp == 0 && !full) {
-        const uint64_t t = pick_largest(sh.found, sh.n_found, p.top);
-        sh.top[lane] = t;
+        __syncwarp();
+        const uint64_t t = pick_largest(sh.found, p.top * (int)blocks_a_row, p.top);
+        __syncwarp();
+        sh.found[lane] = t;
         __syncwarp();
       }
     }
-    // (S is NaN where the row holds a NaN or +infinity)
-    bool odd = full || !(v.S == v.S) || v.m > 1e37f || (v.m < kLowest && v.m != -INFINITY);
-    if (blocks_a_row > 1) {
-      if (threadIdx.x == 0) {
-        sh.sums = v;
-        sh.odd = odd;
-      }
-      __syncwarp();
-      cluster_sync();  // every block's sums and alternatives are in its shared memory
-      if (rank == 0) {
-        // all blocks' sums (each lane a block's), and the largest of all alternatives
-        LogSums w{-INFINITY, 0.f, 0.f};
-        int any = 0;
-        if (lane < (int)blocks_a_row) {
-          const uint32_t sums = mapa_shared(smem_u32(&sh.sums), lane);
-          w = LogSums{__uint_as_float(ld_cluster_u32(sums)), __uint_as_float(ld_cluster_u32(sums + 4)),
-                      __uint_as_float(ld_cluster_u32(sums + 8))};
-          any = (int)ld_cluster_u32(mapa_shared(smem_u32(&sh.odd), lane));
-        }
-        v = log_join_lanes(w);
-        // a part that is odd by itself (nothing above kLowest) need not be so in the whole row
-        odd = !(v.S == v.S) || v.m > 1e37f || (v.m < kLowest && v.m != -INFINITY);
-        if (p.top > 0) odd = odd || __any_sync(0xffffffffu, any != 0);
-        if (p.top > 0 && !odd && warp == 0) {
-          for (int i = lane; i < p.top * (int)blocks_a_row; i += 32) {
-            const uint32_t key = mapa_shared(smem_u32(&sh.top[i % p.top]), i / p.top);
-            sh.found[i] = (uint64_t)ld_cluster_u32(key) | (uint64_t)ld_cluster_u32(key + 4) << 32;
-          }
-          __syncwarp();
-          const uint64_t t = pick_largest(sh.found, p.top * (int)blocks_a_row, p.top);
-          __syncwarp();
-          sh.found[lane] = t;
-          __syncwarp();
-        }
-      }
-    }
-    if (rank == 0) {
-      if (odd) {
-        __syncthreads();
-        logprob_plain_row<T>(p, a, row, sh.red, sh.plain);
-      } else if (warp == 0) {
-        const bool none = v.S == 0.f;
-        const float ref = log_ref(v.m), log_s = log2f(v.S);
-        if (lane == 0) {
-          const int64_t t = a.targets ? a.targets[row] : -1;
-          float xt = 0.f;
-          if (t >= 0 && t < p.vocab) xt = to_f32(static_cast<T const *>(a.x)[row * p.s_x + t]);
-          logprob_row_values(p, a, row, none, none ? -INFINITY : (ref + log_s) * kLn2, (log_s - v.U / v.S) * kLn2,
-                             log_prob(xt, v, log_s));
-        }
-        if (lane < p.top) {
-          const uint64_t key = (blocks_a_row > 1 ? sh.found : sh.top)[lane];
-          const float xt = rank_value((uint32_t)(key >> 32));
-          if (a.top_index) a.top_index[row * p.top + lane] = ~(uint32_t)key;
-          if (a.top_logprob)
-            a.top_logprob[row * p.top + lane] = none ? -INFINITY : log_prob(xt, v, log_s);
-        }
-      }
-    }
-    if (blocks_a_row > 1) {
-      __syncwarp();
-      cluster_sync();  // no block goes on while its shared memory is read
-    } else {
+  }
+  if (rank == 0) {
+    if (odd) {
       __syncthreads();
+      logprob_plain_row<T>(p, a, row, sh.red, sh.plain);
+    } else if (warp == 0) {
+      const bool none = v.S == 0.f;
+      const float ref = log_ref(v.m), log_s = log2f(v.S);
+      if (lane == 0) {
+        const int64_t t = a.targets ? a.targets[row] : -1;
+        float xt = 0.f;
+        if (t >= 0 && t < p.vocab) xt = to_f32(static_cast<T const *>(a.x)[row * p.s_x + t]);
+        logprob_row_values(p, a, row, none, none ? -INFINITY : (ref + log_s) * kLn2, (log_s - v.U / v.S) * kLn2,
+                           log_prob(xt, v, log_s));
+      }
+      if (lane < p.top) {
+        const uint64_t key = (blocks_a_row > 1 ? sh.found : sh.top)[lane];
+        const float xt = rank_value((uint32_t)(key >> 32));
+        if (a.top_index) a.top_index[row * p.top + lane] = ~(uint32_t)key;
+        if (a.top_logprob)
+          a.top_logprob[row * p.top + lane] = none ? -INFINITY : log_prob(xt, v, log_s);
+      }
     }
+  }
+  if (blocks_a_row > 1) {
+    __syncwarp();
+    cluster_sync();  // no block ends while its shared memory is read
   }
 }
 
@@ -550,14 +588,16 @@ __global__ void __launch_bounds__(256) logprob_backward_kernel(const LogprobPara
 
 // ---------------------------------------------------------------- launchers
 
-cudaError_t launch_logprob(LogprobParams const &p, LogprobPtrs const &a, int num_sms, cudaStream_t st) {
+cudaError_t launch_logprob(LogprobParams const &p, LogprobPtrs const &a, uint32_t *err, int num_sms,
+                           cudaStream_t st) {
   const int64_t pieces = (p.vocab * (p.dt == EIR_FP32 ? 4 : 2) + 15) / 16 + 1;
   // a block a row where the rows fill the SMs; else clusters of up to 8, with
   // at least 256 pieces a block
   uint32_t blocks = 1;
   while (blocks < 8 && p.rows * blocks * 2 <= 2 * num_sms && pieces >= 512 * (int64_t)blocks) blocks *= 2;
-  // a row's blocks and barriers cost least with few threads, as long as each has some pieces; the rows
-  // that are waiting fill the SMs
+  // Few threads a row make its barriers cheap; as many rows as fit are on an SM at a time, and
+  // the next take the place of the finished ones (persistent blocks that
+  // walked rows ran in step with one another: 67 us against 59 without alternatives, 4096 x 32768 BF16)
   const int threads = blocks > 1 ? 256 : pieces <= 512 ? 32 : pieces <= 2048 ? 64 : pieces <= 8192 ? 128 : 256;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(p.rows * blocks));
@@ -587,7 +627,7 @@ cudaError_t launch_logprob(LogprobParams const &p, LogprobPtrs const &a, int num
     }
   };
   auto kern = p.dt == EIR_FP32 ? pick(float{}) : pick(__nv_bfloat16{});
-  return cudaLaunchKernelEx(&cfg, kern, p, a, blocks);
+  return cudaLaunchKernelEx(&cfg, kern, p, a, blocks, err);
 }
 
 template <typename T>

@@ -95,7 +95,8 @@ int i8_box_tokens(I8TcPlan const &tp);
 // rows of k bytes, `stride` apart, into rows `ld` bytes apart
 cudaError_t launch_i8_pack(int64_t rows, int64_t k, int64_t stride, int8_t const *src, int8_t *dst, int64_t ld,
                            int num_sms, cudaStream_t st);
-cudaError_t launch_logprob(LogprobParams const &p, LogprobPtrs const &a, int num_sms, cudaStream_t st);
+cudaError_t launch_logprob(LogprobParams const &p, LogprobPtrs const &a, uint32_t *err, int num_sms,
+                           cudaStream_t st);
 cudaError_t launch_logprob_backward(LogprobParams const &p, LogprobGradPtrs const &a, int num_sms,
                                     cudaStream_t st);
 

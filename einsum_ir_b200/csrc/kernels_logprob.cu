@@ -529,61 +529,85 @@ template <typename T, bool SAME>
 __global__ void __launch_bounds__(256) logprob_backward_kernel(const LogprobParams p, const LogprobGradPtrs a,
                                                                int blocks_a_row) {
   using Row = LogitRow<T>;
-  constexpr int V = Row::V;
+  using Piece = typename Row::Piece;
+  constexpr int V = Row::V, AT_ONCE = 4;
   pdl_launch_dependents();
   pdl_wait();
   const uintptr_t begin = reinterpret_cast<uintptr_t>(a.x);
   const uintptr_t end = begin + (uintptr_t)(((p.rows - 1) * p.s_x + p.vocab) * (int64_t)sizeof(T));
-  for (int64_t unit = blockIdx.x; unit < p.rows * blocks_a_row; unit += gridDim.x) {
-    const int64_t row = unit / blocks_a_row;
-    const int part = (int)(unit - row * blocks_a_row);
-    T const *x = static_cast<T const *>(a.x) + row * p.s_x;
-    T *dx = static_cast<T *>(a.dx) + row * p.s_dx;
-    const Row out(dx, p.vocab);
-    const int q0 = (int)((int64_t)out.pieces * part / blocks_a_row);
-    const int q1 = (int)((int64_t)out.pieces * (part + 1) / blocks_a_row);
-    const float lse = a.lse[row];
-    const int64_t t = a.targets ? a.targets[row] : -1;
-    float dlp = t >= 0 ? a.dlogprob[row] : 0.f;
-    if (t >= p.vocab) dlp = logit_nan();
-    const float dent = a.dentropy ? a.dentropy[row] : 0.f;
-    // dx = -p (dlp + dent (x - lse + H)) = p (k0 + k1 d), d = (x - lse) log2 e
-    const float k0 = -dlp - dent * (a.dentropy ? a.entropy[row] : 0.f), k1 = -dent * kLn2;
-    const bool none = lse == -INFINITY;
-#pragma unroll 4
-    for (int q = q0 + (int)threadIdx.x; q < q1; q += 256) {
-      const int i0 = out.first_index(q);
-      typename Row::Piece c, g;
-      if (SAME) c = Row(x, p.vocab).load(q);
-      else if (i0 >= 0 && i0 <= p.vocab - V) c.load_any(x, i0, p.vocab, begin, end);
+  const int64_t row = blockIdx.x / (uint32_t)blocks_a_row;
+  const int part = (int)(blockIdx.x % (uint32_t)blocks_a_row);
+  T const *x = static_cast<T const *>(a.x) + row * p.s_x;
+  T *dx = static_cast<T *>(a.dx) + row * p.s_dx;
+  const Row out(dx, p.vocab), in(x, p.vocab);
+  const int q0 = (int)((int64_t)out.pieces * part / blocks_a_row);
+  const int q1 = (int)((int64_t)out.pieces * (part + 1) / blocks_a_row);
+  const float lse = a.lse[row];
+  const int64_t t = a.targets ? a.targets[row] : -1;
+  float dlp = t >= 0 ? a.dlogprob[row] : 0.f;
+  if (t >= p.vocab) dlp = logit_nan();
+  const float dent = a.dentropy ? a.dentropy[row] : 0.f;
+  // dx = -p (dlp + dent (x - lse + H)) = p (k0 + k1 d), d = (x - lse) log2 e
+  const float k0 = -dlp - dent * (a.dentropy ? a.entropy[row] : 0.f), k1 = -dent * kLn2;
+  const bool none = lse == -INFINITY;
+  // the gradients of a piece's logits
+  auto grads = [&](int q, Piece const &c) {
+    const int i0 = out.first_index(q);
+    float f[V];
+#pragma unroll
+    for (int e = 0; e < V; e += 2) {
+      float2 d = mul2(add2(c.get2(e), make_float2(-lse, -lse)), make_float2(kLog2e, kLog2e));
+      // (2^-200 is 0 in FP32: a ruled-out logit gets 0, not 0 times infinity)
+      d = make_float2(max_nan(d.x, -200.f), max_nan(d.y, -200.f));
+      const float2 pr = make_float2(exp2_fast(d.x), exp2_fast(d.y));
+      const float2 r = mul2(pr, fma2(d, make_float2(k1, k1), make_float2(k0, k0)));
+      f[e] = r.x;
+      f[e + 1] = r.y;
+    }
+    if (none) {
+#pragma unroll
+      for (int e = 0; e < V; ++e) f[e] = 0.f;
+    } else if (t >= i0 && t < i0 + V) {
+#pragma unroll
+      for (int e = 0; e < V; ++e)
+        if (t == i0 + e) f[e] += dlp;
+    }
+    Piece g;
+    g.set(f);
+    return g;
+  };
+  const int threads = blockDim.x;
+  int q = q0 + (int)threadIdx.x;
+  auto ragged = [&]() {  // pieces that may reach outside the row, or the tensor
+    const int i0 = out.first_index(q);
+    const bool inside = i0 >= 0 && i0 <= p.vocab - V;
+    Piece c;
+    if (SAME) {
+      c = in.load(q);
+    } else if (inside) {
+      c.load_any(x, i0, p.vocab, begin, end);
+    } else {
       float f[V];
 #pragma unroll
-      for (int e = 0; e < V; e += 2) {
-        float2 xv;
-        if (SAME || (i0 >= 0 && i0 <= p.vocab - V)) {
-          xv = c.get2(e);
-        } else {
-          xv.x = i0 + e >= 0 && i0 + e < p.vocab ? to_f32(x[i0 + e]) : 0.f;
-          xv.y = i0 + e + 1 >= 0 && i0 + e + 1 < p.vocab ? to_f32(x[i0 + e + 1]) : 0.f;
-        }
-        float2 d = mul2(add2(xv, make_float2(-lse, -lse)), make_float2(kLog2e, kLog2e));
-        // (2^-200 is 0 in FP32: a ruled-out logit gets 0, not 0 times infinity)
-        d = make_float2(max_nan(d.x, -200.f), max_nan(d.y, -200.f));
-        const float2 pr = make_float2(exp2_fast(d.x), exp2_fast(d.y));
-        const float2 r = mul2(pr, fma2(d, make_float2(k1, k1), make_float2(k0, k0)));
-        f[e] = none ? 0.f : r.x;
-        f[e + 1] = none ? 0.f : r.y;
-      }
-      if (t >= i0 && t < i0 + V && !none) {
+      for (int e = 0; e < V; ++e) f[e] = i0 + e >= 0 && i0 + e < p.vocab ? to_f32(x[i0 + e]) : 0.f;
+      c.set(f);
+    }
+    const Piece g = grads(q, c);
+    if (inside) g.store(dx + i0);
+    else g.store_some(dx + i0, i0 < 0 ? -i0 : 0, p.vocab - i0 < V ? (int)(p.vocab - i0) : V);
+    q += threads;
+  };
+  if (q < q1) ragged();
+  if (SAME) {
+    for (; q + (AT_ONCE - 1) * threads < q1 - 1; q += AT_ONCE * threads) {
+      Piece c[AT_ONCE];
 #pragma unroll
-        for (int e = 0; e < V; ++e)
-          if (t == i0 + e) f[e] += dlp;
-      }
-      g.set(f);
-      if (i0 >= 0 && i0 <= p.vocab - V) g.store(dx + i0);
-      else g.store_some(dx + i0, i0 < 0 ? -i0 : 0, p.vocab - i0 < V ? (int)(p.vocab - i0) : V);
+      for (int i = 0; i < AT_ONCE; ++i) c[i].template load<false>(in.base + (int64_t)(q + i * threads) * 16);
+#pragma unroll
+      for (int i = 0; i < AT_ONCE; ++i) grads(q + i * 256, c[i]).store(dx + out.first_index(q + i * threads));
     }
   }
+  while (q < q1) ragged();
 }
 
 // ---------------------------------------------------------------- launchers
@@ -637,13 +661,17 @@ cudaError_t launch_logprob(LogprobParams const &p, LogprobPtrs const &a, uint32_
 template <typename T>
 static cudaError_t launch_logprob_backward_t(LogprobParams const &p, LogprobGradPtrs const &a, int num_sms,
                                              cudaStream_t st) {
-  const int64_t pieces = (p.vocab * (int64_t)sizeof(T) + 15) / 16 + 1, most = (int64_t)num_sms * 8;
-  int64_t blocks = 1;  // of a row: until the GPU is full, or a thread has four pieces
-  while (p.rows * blocks < most && pieces > 1024 * blocks) blocks *= 2;
+  // blocks of 4096 pieces, smaller where the GPU would not be full. (Blocks that end make room
+  // for others out of step: persistent ones took 80 us for 2048 x 50021 BF16, these take 72.)
+  const int64_t pieces = (p.vocab * (int64_t)sizeof(T) + 15) / 16 + 1;
+  int64_t blocks = (pieces + 4096 - 1) / 4096;
+  while (p.rows * blocks < (int64_t)num_sms * 8 && pieces > 1024 * blocks) blocks *= 2;
+  blocks = std::max<int64_t>(1, std::min<int64_t>(blocks, INT32_MAX / p.rows));
   const bool same = (reinterpret_cast<uintptr_t>(a.x) - reinterpret_cast<uintptr_t>(a.dx)) % 16 == 0 &&
                     (p.rows == 1 || (p.s_x - p.s_dx) * (int64_t)sizeof(T) % 16 == 0);
   auto kern = same ? logprob_backward_kernel<T, true> : logprob_backward_kernel<T, false>;
-  return launch_kernel(kern, dim3((unsigned)std::min(p.rows * blocks, most)), dim3(256), 0, st, p, a, (int)blocks);
+  return launch_kernel(kern, dim3((unsigned)(p.rows * blocks)), dim3(pieces <= 256 ? 64 : pieces <= 1024 ? 128 : 256), 0,
+                       st, p, a, (int)blocks);
 }
 
 cudaError_t launch_logprob_backward(LogprobParams const &p, LogprobGradPtrs const &a, int num_sms,

@@ -387,6 +387,8 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS)
       phases ^= 1u << stage;
 #pragma unroll
       for (int i = 0; i < AT_ONCE; ++i) c[i].template load<false>(sh.stages[warp][stage] + (i * 32 + lane) * 16);
+      // (without the fence a read that is still queued can meet the next copy's bytes)
+      fence_proxy_async_smem();
       __syncwarp();
       if (lane == 0 && inner(k + kLogStages * warps)) copy(k + kLogStages * warps, stage);
       stage = stage + 1 == kLogStages ? 0 : stage + 1;
@@ -604,7 +606,7 @@ __global__ void __launch_bounds__(256) logprob_backward_kernel(const LogprobPara
 #pragma unroll
       for (int i = 0; i < AT_ONCE; ++i) c[i].template load<false>(in.base + (int64_t)(q + i * threads) * 16);
 #pragma unroll
-      for (int i = 0; i < AT_ONCE; ++i) grads(q + i * 256, c[i]).store(dx + out.first_index(q + i * threads));
+      for (int i = 0; i < AT_ONCE; ++i) grads(q + i * threads, c[i]).store(dx + out.first_index(q + i * threads));
     }
   }
   while (q < q1) ragged();

@@ -496,6 +496,21 @@ def test_logprob_backward(cuda, rows, vocab, pad, offset, dtype):
 
 
 @pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("rows,vocab", [(2, 6528), (74, 4736), (568, 3136), (96, 6117), (30, 10007), (9, 24001), (1, 1500)])
+def test_logprob_backward_every_target(cuda, rows, vocab, dtype):
+    """targets spread over the whole row: the one-hot term lands in its column whatever thread holds it"""
+    g = gen(rows)
+    x = rows_of(g, rows, vocab, dtype)
+    t = torch.linspace(0, vocab - 1, rows, device="cuda").round().long()
+    lse = torch.logsumexp(x.double(), 1).float()
+    dlp = torch.full((rows,), 2.0, device="cuda")
+    dx = torch.empty_like(x)
+    op.LogprobPlan(rows, vocab, CODE[dtype]).backward(x, t, lse, dlp, dx)
+    want = logprob_backward64(x, t, lse, None, dlp, None)
+    close(dx, want, 64 * U + round_tol(want, dtype))
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
 def test_logprob_backward_special_rows_and_in_place(cuda, dtype):
     vocab = 1203
     x = logits_of(gen(6), 6, vocab, dtype)
@@ -526,3 +541,42 @@ def test_row_operators_on_another_stream(cuda):
     s.synchronize()
     check_logprob(x, t, 3, o)
     assert torch.equal(q, quantized32(x)[0])
+
+
+@pytest.mark.parametrize("case", range(6))
+def test_repeats_are_equal(cuda, case):
+    """the same call many times, the GPU full of blocks: bit for bit the same, and right"""
+    g = gen(case)
+    if case < 3:
+        rows, vocab, dtype = [(2144, 9920, BF16), (3000, 5000, F32), (1200, 30011, BF16)][case]
+        x = rows_of(g, rows, vocab, dtype, scale=3.0)
+        first = run_logprob(x, None, 8)
+        check_logprob(x, None, 8, first)
+        again = lambda: run_logprob(x, None, 8)
+    elif case < 5:
+        rows, cols, dtype = [(3000, 4096, BF16), (2500, 2311, F32)][case - 3]
+        h, dy = rows_of(g, rows, cols, dtype, 1), rows_of(g, rows, cols, dtype, 8)
+        rstd = norm64(h, None, None, 1e-5)["rstd"].float()
+        plan = op.NormPlan(rows, cols, CODE[dtype], dtype_out=cabi.INT8, stride_x=cols + 1, stride_dy=cols + 8)
+
+        def again():
+            o = {"dx": torch.empty((rows, cols), device="cuda", dtype=dtype), "dw": torch.empty(cols, device="cuda"),
+                 "q": torch.empty((rows, cols), device="cuda", dtype=torch.int8), "scale": torch.empty(rows, device="cuda")}
+            plan.norm(h, o["q"], scale=o["scale"])
+            plan.backward(dy, h, rstd, o["dx"], dweight=o["dw"])
+            return o
+        first = again()
+        assert torch.equal(first["q"], quantized32(h)[0])
+    else:
+        a, b = codes(g, 300, 2000), codes(g, 1500, 2000)
+        plan = op.Int8ContractPlan(300, 1500, 2000, dtype_out=cabi.FP32)
+
+        def again():
+            y = torch.empty((300, 1500), device="cuda")
+            plan.contract(a, b, None, None, y)
+            return {"y": y}
+        first = again()
+        assert torch.equal(first["y"].double(), contract64(a, b, None, None, None, 0).float().double())
+    for _ in range(60):
+        for k, v in again().items():
+            assert v is None or torch.equal(v, first[k]), k

@@ -1,7 +1,7 @@
 // C-ABI of the row operators and the 8-bit contraction (eir_operators.h):
 // argument checks, workspaces and launches.
 #include <algorithm>
-#include <cstdio>
+#include <mutex>
 #include <new>
 #include <string>
 #include "eir_operators.h"
@@ -48,22 +48,67 @@ int make_plan(eir_plan **out, int what, int family, Fill fill) {
   return EIR_SUCCESS;
 }
 
-// the plan's own workspace on the current device, allocated on first use
-int workspace(eir_plan *p, void **ws) {
+// The workspaces' memory comes from a pool of the library's own per device, so
+// that a plan made for a new shape does not pay for cudaMalloc on its first call
+// (0.5 ms and more; it synchronises the device too). Up to 256 MiB stay with the
+// pool when plans are destroyed.
+int workspace_pool(int dev, cudaMemPool_t *pool) {
+  static std::mutex mu;
+  static cudaMemPool_t pools[64] = {};
+  if (dev < 0 || dev >= 64) return fail(EIR_CUDA_ERROR, "device index out of range");
+  std::lock_guard<std::mutex> lk(mu);
+  if (pools[dev] == nullptr) {
+    cudaMemPoolProps props = {};
+    props.allocType = cudaMemAllocationTypePinned;
+    props.location.type = cudaMemLocationTypeDevice;
+    props.location.id = dev;
+    cudaMemPool_t made = nullptr;
+    cudaError_t e = cudaMemPoolCreate(&made, &props);
+    if (e != cudaSuccess) return eir::api_cuda_fail(e, "cudaMemPoolCreate");
+    uint64_t keep = (uint64_t)256 << 20;
+    e = cudaMemPoolSetAttribute(made, cudaMemPoolAttrReleaseThreshold, &keep);
+    if (e != cudaSuccess) {
+      cudaMemPoolDestroy(made);
+      return eir::api_cuda_fail(e, "cudaMemPoolSetAttribute");
+    }
+    pools[dev] = made;
+  }
+  *pool = pools[dev];
+  return EIR_SUCCESS;
+}
+
+// the plan's own workspace on the current device, allocated on first use in
+// `st`'s order (a plan with a workspace runs on one stream at a time)
+int workspace(eir_plan *p, cudaStream_t st, void **ws) {
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
   if (e != cudaSuccess) return eir::api_cuda_fail(e, "cudaGetDevice");
   if (p->ws == nullptr || p->ws_device != dev) {
-    if (p->ws != nullptr) cudaFree(p->ws);
-    e = cudaMalloc(&p->ws, (size_t)p->ws_bytes);
+    eir::api_free_workspace(p);
+    cudaMemPool_t pool = nullptr;
+    int rc = workspace_pool(dev, &pool);
+    if (rc != EIR_SUCCESS) return rc;
+    e = cudaEventCreateWithFlags(&p->ws_used, cudaEventDisableTiming);
+    if (e != cudaSuccess) return eir::api_cuda_fail(e, "cudaEventCreate(workspace)");
+    e = cudaMallocFromPoolAsync(&p->ws, (size_t)p->ws_bytes, pool, st);
     if (e != cudaSuccess) {
       p->ws = nullptr;
-      return eir::api_cuda_fail(e, "cudaMalloc(workspace)");
+      cudaEventDestroy(p->ws_used);
+      p->ws_used = nullptr;
+      return eir::api_cuda_fail(e, "cudaMallocFromPoolAsync(workspace)");
     }
     p->ws_device = dev;
   }
   *ws = p->ws;
   return EIR_SUCCESS;
+}
+
+// marks the end of the workspace's use, which the plan's destruction waits for
+int workspace_used(eir_plan *p, cudaStream_t st) {
+  cudaStreamCaptureStatus cap = cudaStreamCaptureStatusNone;
+  cudaError_t e = cudaStreamIsCapturing(st, &cap);
+  if (e == cudaSuccess && cap == cudaStreamCaptureStatusNone) e = cudaEventRecord(p->ws_used, st);
+  return e == cudaSuccess ? EIR_SUCCESS : eir::api_cuda_fail(e, "cudaEventRecord(workspace)");
 }
 
 // Tiling of an 8-bit contraction on the tensor cores. Pair tiles once they
@@ -216,7 +261,7 @@ int eir_norm_backward(eir_plan *p, void const *dy, void const *h, void const *we
   int64_t parts = 0;
   if (dweight != nullptr) {
     void *ws = nullptr;
-    rc = workspace(p, &ws);
+    rc = workspace(p, st, &ws);
     if (rc != EIR_SUCCESS) return rc;
     a.part = static_cast<float *>(ws);
   }
@@ -225,7 +270,8 @@ int eir_norm_backward(eir_plan *p, void const *dy, void const *h, void const *we
     rc = launched(eir::launch_norm_backward(n, a, err, num_sms, st, &parts), "norm backward launch");
   }
   if (rc != EIR_SUCCESS || dweight == nullptr) return rc;
-  return launched(eir::launch_norm_dweight(n, a.part, parts, dweight, st), "norm weight gradient launch");
+  rc = launched(eir::launch_norm_dweight(n, a.part, parts, dweight, st), "norm weight gradient launch");
+  return rc == EIR_SUCCESS ? workspace_used(p, st) : rc;
 }
 
 // ---------------------------------------------------------------- quantize
@@ -338,7 +384,7 @@ int eir_contract_int8(eir_plan *p, void const *left, void const *right, float co
     I8Operand &o = ops[i];
     if (!o.copy) continue;
     void *ws = nullptr;
-    rc = workspace(p, &ws);
+    rc = workspace(p, st, &ws);
     if (rc != EIR_SUCCESS) return rc;
     int8_t *to = static_cast<int8_t *>(ws) + (i == 0 ? 0 : p->i8.m * ld);
     rc = launched(eir::launch_i8_pack(o.rows, p->i8.k, i == 0 ? p->i8.s_l : p->i8.s_r, o.ptr, to, ld, num_sms, st),
@@ -352,8 +398,11 @@ int eir_contract_int8(eir_plan *p, void const *left, void const *right, float co
   if (rc != EIR_SUCCESS) return rc;
   rc = i8_map(ops[1], p->i8.k, 128, p->i8.act == EIR_ACT_GATED_SILU, &map_c);
   if (rc != EIR_SUCCESS) return rc;
-  ProfScope prof(p, st);
-  return launched(eir::launch_i8_tc(p->i8_tc, map_c, map_t, p->i8, a, err, st), "8-bit contraction launch");
+  {
+    ProfScope prof(p, st);
+    rc = launched(eir::launch_i8_tc(p->i8_tc, map_c, map_t, p->i8, a, err, st), "8-bit contraction launch");
+  }
+  return rc == EIR_SUCCESS && (ops[0].copy || ops[1].copy) ? workspace_used(p, st) : rc;
 }
 
 // ---------------------------------------------------------------- log probabilities

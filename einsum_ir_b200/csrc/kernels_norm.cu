@@ -353,8 +353,9 @@ __global__ void __launch_bounds__(1024)
       if (op.residual()) r.load_slot(at + slot, off_r, column(j), p.cols);
       op.take(row, column(j), x, r, h[j], ss, mx);
     }
+    fence_proxy_async_smem();  // the row is in registers: its stage may be copied over
     __syncwarp();
-    if (lane == 0) mbar_arrive(&rr.empty[stage]);  // the row is in registers
+    if (lane == 0) mbar_arrive(&rr.empty[stage]);
     if (!QUANT) ss = warp_sum(ss);
     mx = __reduce_max_sync(0xffffffffu, mx);
     const bool warp_late = __any_sync(0xffffffffu, late);
@@ -643,8 +644,9 @@ __global__ void __launch_bounds__(kBackThreads + 32, back_blocks(N * NormBackRow
       }
       op.template take<true, true>(w, h[j], dy, s, unit, held[j], gh, dw[j]);
     }
+    fence_proxy_async_smem();  // the row is in registers: its stage may be copied over
     __syncwarp();
-    if (lane == 0) mbar_arrive(&rr.empty[stage]);  // the row is in registers
+    if (lane == 0) mbar_arrive(&rr.empty[stage]);
     gh = warp_sum(gh);
     const bool warp_late = __any_sync(0xffffffffu, late);
     if (lane == 0) {
@@ -897,8 +899,17 @@ cudaError_t launch_quantize(QuantizeParams const &p, void const *x, int8_t *q, f
                           : launch_norm_out<__nv_bfloat16, int8_t, true>(n, a, err, num_sms, st);
 }
 
+// blocks an SM of the backward ring, if their stages fit
+static int64_t back_ring_blocks(int64_t cols, int *threads) {
+  const int per = cols <= kBackThreads * 8 ? 8 : 16;
+  *threads = (int)((cols + per - 1) / per + 31) / 32 * 32;
+  return *threads > kBackThreads ? 0 : std::min(8, back_blocks(per) * (kBackThreads + 32) / (*threads + 32));
+}
+
 int64_t norm_backward_parts(NormParams const &p, int num_sms) {
-  return std::min<int64_t>(p.rows, (int64_t)num_sms * 32);
+  int threads = 0;  // (narrow rows: 8 blocks of 4 warps an SM; wide ones: 2 blocks)
+  const int64_t an_sm = p.cols <= 32 * kPerBack ? 32 : std::max<int64_t>(2, back_ring_blocks(p.cols, &threads));
+  return std::min<int64_t>(p.rows, num_sms * an_sm);
 }
 
 template <typename T, typename G>
@@ -918,10 +929,10 @@ static cudaError_t launch_norm_backward_t(NormParams const &p, NormGradPtrs cons
   }
   const int per = p.cols <= kBackThreads * 8 ? 8 : 16;
   RingShape r;
-  r.threads = (int)((p.cols + per - 1) / per + 31) / 32 * 32;
-  if (r.threads <= kBackThreads) {
+  const int64_t most = back_ring_blocks(p.cols, &r.threads);
+  if (most > 0) {
     const int64_t bytes = ring_slot(p.cols * sizeof(T)) + ring_slot(p.cols * sizeof(G)) * (a.dsum ? 2 : 1);
-    const int64_t blocks = ring_fit(bytes, std::min(8, back_blocks(per) * (kBackThreads + 32) / (r.threads + 32)), &r);
+    const int64_t blocks = ring_fit(bytes, most, &r);
     if (r.stages > 0) {
       *parts = std::min<int64_t>(p.rows, num_sms * blocks);
       auto kern = per == 8 ? (grid ? norm_backward_ring_kernel<T, G, 8 / V, true> : norm_backward_ring_kernel<T, G, 8 / V, false>)

@@ -111,9 +111,11 @@ int workspace_used(eir_plan *p, cudaStream_t st) {
   return e == cudaSuccess ? EIR_SUCCESS : eir::api_cuda_fail(e, "cudaEventRecord(workspace)");
 }
 
-// Tiling of an 8-bit contraction on the tensor cores. Pair tiles once they
-// fill most of the GPU's 74 CTA pairs; else one-CTA tiles of just enough
-// tokens, the K walk of each split over a cluster: the largest cluster of
+// Tiling of an 8-bit contraction on the tensor cores. Pair tiles once there are
+// 32 of them (of the GPU's 74 CTA pairs), or 16 of a short K walk: one-CTA tiles
+// move twice the operand bytes (512 tokens x 4096 x 2048: 10.1 us against
+// 11.4). Else one-CTA tiles of just enough tokens, the K walk of each split over
+// a cluster, 4 K blocks a CTA at least (the exchange takes 1 to 3 us): the largest cluster of
 // which all tiles' clusters fit the GPU at once, two CTAs an SM (measured
 // limits; a second wave costs more than the split gains: 256 tokens x 4096 x
 // 4096, 64 tiles, take 14.4 us unsplit, 12.5 split by 4 and 21.7 split by 8).
@@ -121,7 +123,7 @@ eir::I8TcPlan i8_tiling(eir::I8Params const &p) {
   eir::I8TcPlan t;
   t.c_tiles = (p.n + 255) / 256;  // gated: 128 gates and their values a tile
   t.t_tiles = (p.m + 255) / 256;
-  if (p.m > 128 && t.c_tiles * t.t_tiles >= 64) return t;
+  if (p.m > 128 && t.c_tiles * t.t_tiles >= (p.k <= 2048 ? 16 : 32)) return t;
   t.tokens = p.m <= 16 ? 16 : p.m <= 32 ? 32 : p.m <= 64 ? 64 : 128;
   t.c_tiles = (p.n + 127) / 128;
   t.t_tiles = (p.m + t.tokens - 1) / t.tokens;
@@ -129,7 +131,7 @@ eir::I8TcPlan i8_tiling(eir::I8Params const &p) {
     int split, tiles;
   } const fits[] = {{8, 32}, {4, 66}, {3, 90}, {2, 148}};
   for (auto const &f : fits) {
-    if (t.split == 1 && t.c_tiles * t.t_tiles <= f.tiles && (p.k + 127) / 128 >= 2 * f.split) t.split = f.split;
+    if (t.split == 1 && t.c_tiles * t.t_tiles <= f.tiles && (p.k + 127) / 128 >= 4 * f.split) t.split = f.split;
   }
   return t;
 }
@@ -380,18 +382,21 @@ int eir_contract_int8(eir_plan *p, void const *left, void const *right, float co
     return launched(eir::launch_i8_row(p->i8, a, num_sms, st), "8-bit contraction launch");
   }
   const int64_t ld = packed_stride(p->i8.k);
-  for (int i = 0; i < 2; ++i) {
-    I8Operand &o = ops[i];
-    if (!o.copy) continue;
+  if (ops[0].copy || ops[1].copy) {
     void *ws = nullptr;
     rc = workspace(p, st, &ws);
     if (rc != EIR_SUCCESS) return rc;
-    int8_t *to = static_cast<int8_t *>(ws) + (i == 0 ? 0 : p->i8.m * ld);
-    rc = launched(eir::launch_i8_pack(o.rows, p->i8.k, i == 0 ? p->i8.s_l : p->i8.s_r, o.ptr, to, ld, num_sms, st),
-                  "8-bit operand copy");
+    eir::I8Pack packs[2] = {};
+    for (int i = 0; i < 2; ++i) {
+      I8Operand &o = ops[i];
+      if (!o.copy) continue;
+      int8_t *to = static_cast<int8_t *>(ws) + (i == 0 ? 0 : p->i8.m * ld);
+      packs[i] = eir::I8Pack{o.rows, i == 0 ? p->i8.s_l : p->i8.s_r, o.ptr, to};
+      o.ptr = to;
+      o.stride = ld;
+    }
+    rc = launched(eir::launch_i8_pack(packs[0], packs[1], p->i8.k, ld, num_sms, st), "8-bit operand copy");
     if (rc != EIR_SUCCESS) return rc;
-    o.ptr = to;
-    o.stride = ld;
   }
   CUtensorMap map_t, map_c;
   rc = i8_map(ops[0], p->i8.k, eir::i8_box_tokens(p->i8_tc), false, &map_t);

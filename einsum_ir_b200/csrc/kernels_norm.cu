@@ -899,9 +899,11 @@ cudaError_t launch_quantize(QuantizeParams const &p, void const *x, int8_t *q, f
                           : launch_norm_out<__nv_bfloat16, int8_t, true>(n, a, err, num_sms, st);
 }
 
+// elements of a thread: 8, 16 or 32
+static int back_per(int64_t cols) { return cols <= kBackThreads * 8 ? 8 : cols <= kBackThreads * 16 ? 16 : 32; }
 // blocks an SM of the backward ring, if their stages fit
 static int64_t back_ring_blocks(int64_t cols, int *threads) {
-  const int per = cols <= kBackThreads * 8 ? 8 : 16;
+  const int per = back_per(cols);
   *threads = (int)((cols + per - 1) / per + 31) / 32 * 32;
   return *threads > kBackThreads ? 0 : std::min(8, back_blocks(per) * (kBackThreads + 32) / (*threads + 32));
 }
@@ -927,7 +929,7 @@ static cudaError_t launch_norm_backward_t(NormParams const &p, NormGradPtrs cons
     auto kern = grid ? norm_backward_kernel<T, G, true> : norm_backward_kernel<T, G, false>;
     return launch_kernel(kern, dim3((unsigned)g.grid), dim3(g.threads), 0, st, p, a);
   }
-  const int per = p.cols <= kBackThreads * 8 ? 8 : 16;
+  const int per = back_per(p.cols);
   RingShape r;
   const int64_t most = back_ring_blocks(p.cols, &r.threads);
   if (most > 0) {
@@ -935,8 +937,12 @@ static cudaError_t launch_norm_backward_t(NormParams const &p, NormGradPtrs cons
     const int64_t blocks = ring_fit(bytes, most, &r);
     if (r.stages > 0) {
       *parts = std::min<int64_t>(p.rows, num_sms * blocks);
-      auto kern = per == 8 ? (grid ? norm_backward_ring_kernel<T, G, 8 / V, true> : norm_backward_ring_kernel<T, G, 8 / V, false>)
-                           : (grid ? norm_backward_ring_kernel<T, G, 16 / V, true> : norm_backward_ring_kernel<T, G, 16 / V, false>);
+      auto kern = grid ? (per == 8    ? norm_backward_ring_kernel<T, G, 8 / V, true>
+                          : per == 16 ? norm_backward_ring_kernel<T, G, 16 / V, true>
+                                      : norm_backward_ring_kernel<T, G, 32 / V, true>)
+                       : (per == 8    ? norm_backward_ring_kernel<T, G, 8 / V, false>
+                          : per == 16 ? norm_backward_ring_kernel<T, G, 16 / V, false>
+                                      : norm_backward_ring_kernel<T, G, 32 / V, false>);
       return launch_ring(kern, r, *parts, st, p, a, r, err);
     }
   }

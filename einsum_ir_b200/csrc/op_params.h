@@ -92,9 +92,13 @@ cudaError_t launch_i8_tc(I8TcPlan const &tp, CUtensorMap const &map_channels, CU
 cudaError_t launch_i8_row(I8Params const &p, I8Ptrs const &a, int num_sms, cudaStream_t st);
 // token rows of one TMA box of the tiling `tp`
 int i8_box_tokens(I8TcPlan const &tp);
-// rows of k bytes, `stride` apart, into rows `ld` bytes apart
-cudaError_t launch_i8_pack(int64_t rows, int64_t k, int64_t stride, int8_t const *src, int8_t *dst, int64_t ld,
-                           int num_sms, cudaStream_t st);
+// rows of k bytes, `stride` apart, into rows `ld` bytes apart, of one or two operands (rows = 0: absent)
+struct I8Pack {
+  int64_t rows, stride;
+  int8_t const *src;
+  int8_t *dst;
+};
+cudaError_t launch_i8_pack(I8Pack const &one, I8Pack const &two, int64_t k, int64_t ld, int num_sms, cudaStream_t st);
 cudaError_t launch_logprob(LogprobParams const &p, LogprobPtrs const &a, uint32_t *err, int num_sms,
                            cudaStream_t st);
 cudaError_t launch_logprob_backward(LogprobParams const &p, LogprobGradPtrs const &a, int num_sms,

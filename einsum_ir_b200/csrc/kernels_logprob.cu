@@ -43,13 +43,6 @@ __device__ __forceinline__ float exp2_fast(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
   return r;
 }
-// the larger, NaN if either is
-__device__ __forceinline__ float max_nan(float a, float b) {
-  float r;
-  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
-  return r;
-}
-
 // a logit's rank as an unsigned integer: the order of the floats, both zeros
 // alike, NaNs highest; 0 is below every logit's
 __device__ __forceinline__ uint32_t rank_bits(float x) {

@@ -211,15 +211,18 @@ struct NormRow {
   // statistics; stores the sum if `keep`. Every lane of a warp calls it
   __device__ __forceinline__ void take(int64_t row, int64_t c, Piece const &x, Piece const &r, float (&h)[V],
                                        float &ss, uint32_t &mx, bool keep = true) const {
+    const bool add = residual() && c < p.cols;
+    float2 sum = make_float2(0.f, 0.f);
 #pragma unroll
-    for (int e = 0; e < V; ++e) h[e] = x.get(e);
-    if (residual() && c < p.cols) {
-#pragma unroll
-      for (int e = 0; e < V; ++e) h[e] += r.get(e);
+    for (int e = 0; e < V; e += 2) {
+      float2 v = x.get2(e);
+      if (add) v = add2(v, r.get2(e));
+      if (!QUANT) sum = fma2(v, v, sum);
+      h[e] = v.x;
+      h[e + 1] = v.y;
     }
     if (!QUANT) {
-#pragma unroll
-      for (int e = 0; e < V; ++e) ss += h[e] * h[e];
+      ss += sum.x + sum.y;
       if (a.sum && keep) {
         Piece s;
         s.set(h);
@@ -229,12 +232,18 @@ struct NormRow {
         float w[V];
         load_shared_any<V>(a.w, p.dt_w, c, p.cols, w_grid, w);
 #pragma unroll
-        for (int e = 0; e < V; ++e) h[e] = __fmul_rn(h[e], w[e]);
+        for (int e = 0; e < V; e += 2) {
+          const float2 v = mul2(make_float2(h[e], h[e + 1]), make_float2(w[e], w[e + 1]));
+          h[e] = v.x;
+          h[e + 1] = v.y;
+        }
       }
     }
     if (kInt8) {
+      float most = __uint_as_float(mx);
 #pragma unroll
-      for (int e = 0; e < V; ++e) mx = max(mx, abs_bits(h[e]));
+      for (int e = 0; e < V; ++e) most = max_nan(most, fabsf(h[e]));
+      mx = __float_as_uint(most);
     }
   }
   __device__ __forceinline__ void give(int64_t row, int64_t c, float const (&h)[V], float rstd,
@@ -243,8 +252,21 @@ struct NormRow {
     RowPiece<OUT, V> o;
     if constexpr (kInt8) {
       o.zero();
+      if (q.finite) {
+        // 1.5 * 2^23 + t rounds t to an integer, ties to even, and holds it in its low byte: a
+        // quarter of the instructions of conversions and masks
+        constexpr float kMagic = 12582912.f;
 #pragma unroll
-      for (int e = 0; e < V; ++e) o.w[e / 4] |= (uint32_t)(quant_one(h[e], q) & 0xff) << (8 * (e % 4));
+        for (int e = 0; e < V; e += 4) {
+          // (__fmul_rn: a packed product and sum would be contracted to one rounding)
+          const float2 t = add2(make_float2(__fmul_rn(h[e], q.inv), __fmul_rn(h[e + 1], q.inv)),
+                                make_float2(kMagic, kMagic));
+          const float2 u = add2(make_float2(__fmul_rn(h[e + 2], q.inv), __fmul_rn(h[e + 3], q.inv)),
+                                make_float2(kMagic, kMagic));
+          o.w[e / 4] = __byte_perm(__byte_perm(__float_as_uint(t.x), __float_as_uint(t.y), 0x0040),
+                                   __byte_perm(__float_as_uint(u.x), __float_as_uint(u.y), 0x0040), 0x5410);
+        }
+      }
     } else {
       float w[V], y[V];
 #pragma unroll

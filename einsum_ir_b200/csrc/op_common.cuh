@@ -71,12 +71,17 @@ __device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
   return r;
 }
 
-// |v| as bits: the order of non-negative floats, with NaNs above infinity, so
-// that an integer maximum carries a NaN through
-__device__ __forceinline__ uint32_t abs_bits(float v) { return __float_as_uint(v) & 0x7fffffffu; }
+// the larger, NaN if either is. Magnitudes as bits keep their order, NaNs above
+// infinity, so that an integer maximum carries a NaN through
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
 
 // A row's 8-bit scaling from the bits of its largest magnitude: the factor
-// 127 / m of round(v * factor), and the scale m * unit / 127 of the integers.
+// 127 / m of round(v * factor), which 127 bounds, and the scale m * unit / 127 of
+// the integers. A row with an infinity or NaN is all zeros, and its scale says so.
 struct QuantScale {
   float inv, scale;
   bool finite;
@@ -90,10 +95,4 @@ __device__ __forceinline__ QuantScale quant_scale(uint32_t max_bits, float unit)
   q.scale = q.finite ? (some ? __fdiv_rn(__fmul_rn(m, unit), 127.f) : 0.f) : __uint_as_float(0x7fc00000u);
   return q;
 }
-// v in 8 bits (|v| <= m, so |v * 127 / m| rounds to 127 at most); a row with
-// an infinity or NaN is all zeros, and its scale says so
-__device__ __forceinline__ int quant_one(float v, QuantScale const &q) {
-  return q.finite ? __float2int_rn(__fmul_rn(v, q.inv)) : 0;
-}
-
 }  // namespace eir

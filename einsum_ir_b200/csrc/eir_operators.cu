@@ -77,13 +77,20 @@ int workspace_pool(int dev, cudaMemPool_t *pool) {
   return EIR_SUCCESS;
 }
 
-// the plan's own workspace on the current device, allocated on first use in
-// `st`'s order (a plan with a workspace runs on one stream at a time)
+// The plan's own workspace on the current device, allocated on first use in
+// `st`'s order; on another stream than the last use's it waits for that. A capture
+// gets the workspace that is there: memory allocated in it would be the graph's own, and an
+// event from outside cannot be waited for (the caller orders a graph's launches).
 int workspace(eir_plan *p, cudaStream_t st, void **ws) {
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
   if (e != cudaSuccess) return eir::api_cuda_fail(e, "cudaGetDevice");
+  cudaStreamCaptureStatus cap = cudaStreamCaptureStatusNone;
+  e = cudaStreamIsCapturing(st, &cap);
+  if (e != cudaSuccess) return eir::api_cuda_fail(e, "cudaStreamIsCapturing");
+  const bool captured = cap != cudaStreamCaptureStatusNone;
   if (p->ws == nullptr || p->ws_device != dev) {
+    if (captured) return bad_argument("a plan with a workspace needs a call on the device before it is captured");
     eir::api_free_workspace(p);
     cudaMemPool_t pool = nullptr;
     int rc = workspace_pool(dev, &pool);
@@ -98,17 +105,25 @@ int workspace(eir_plan *p, cudaStream_t st, void **ws) {
       return eir::api_cuda_fail(e, "cudaMallocFromPoolAsync(workspace)");
     }
     p->ws_device = dev;
+    p->ws_stream = st;
+  } else if (!captured && st != p->ws_stream) {
+    e = cudaStreamWaitEvent(st, p->ws_used, 0);
+    if (e != cudaSuccess) return eir::api_cuda_fail(e, "cudaStreamWaitEvent(workspace)");
   }
   *ws = p->ws;
   return EIR_SUCCESS;
 }
 
-// marks the end of the workspace's use, which the plan's destruction waits for
-int workspace_used(eir_plan *p, cudaStream_t st) {
+// marks the end of the workspace's use, which other streams and the plan's destruction wait
+// for; rc: the launches' status, returned
+int workspace_used(eir_plan *p, cudaStream_t st, int rc) {
   cudaStreamCaptureStatus cap = cudaStreamCaptureStatusNone;
   cudaError_t e = cudaStreamIsCapturing(st, &cap);
-  if (e == cudaSuccess && cap == cudaStreamCaptureStatusNone) e = cudaEventRecord(p->ws_used, st);
-  return e == cudaSuccess ? EIR_SUCCESS : eir::api_cuda_fail(e, "cudaEventRecord(workspace)");
+  if (e == cudaSuccess && cap == cudaStreamCaptureStatusNone) {
+    e = cudaEventRecord(p->ws_used, st);
+    p->ws_stream = st;
+  }
+  return rc != EIR_SUCCESS || e == cudaSuccess ? rc : eir::api_cuda_fail(e, "cudaEventRecord(workspace)");
 }
 
 // Tiling of an 8-bit contraction on the tensor cores. Pair tiles once there are
@@ -271,9 +286,10 @@ int eir_norm_backward(eir_plan *p, void const *dy, void const *h, void const *we
     ProfScope prof(p, st);
     rc = launched(eir::launch_norm_backward(n, a, err, num_sms, st, &parts), "norm backward launch");
   }
-  if (rc != EIR_SUCCESS || dweight == nullptr) return rc;
-  rc = launched(eir::launch_norm_dweight(n, a.part, parts, dweight, st), "norm weight gradient launch");
-  return rc == EIR_SUCCESS ? workspace_used(p, st) : rc;
+  if (dweight == nullptr) return rc;
+  if (rc == EIR_SUCCESS)
+    rc = launched(eir::launch_norm_dweight(n, a.part, parts, dweight, st), "norm weight gradient launch");
+  return workspace_used(p, st, rc);
 }
 
 // ---------------------------------------------------------------- quantize
@@ -366,14 +382,14 @@ int eir_contract_int8(eir_plan *p, void const *left, void const *right, float co
   const eir::I8Ptrs a{static_cast<int8_t const *>(left), static_cast<int8_t const *>(right),
                       scale_left, scale_right, bias, out};
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  if (p->family != EIR_FAMILY_TC) {
-    ProfScope prof(p, st);
-    return launched(eir::launch_i8_simt(p->i8, a, st), "8-bit contraction launch");
-  }
   int num_sms = 0;
   uint32_t *err = nullptr;
   int rc = eir::api_device(&num_sms, &err);
   if (rc != EIR_SUCCESS) return rc;
+  if (p->i8.k == 0) {
+    ProfScope prof(p, st);
+    return launched(eir::launch_i8_bias(p->i8, a, num_sms, st), "8-bit contraction launch");
+  }
   // one token: the row kernel, but for large layers that TMA can stream in
   // place (4096 x 4096: 4.4 us against 6.0; 8192 x 28672: 40.6 against 37.9)
   I8Operand ops[2] = {i8_operand(left, p->i8.m, p->i8.k, p->i8.s_l), i8_operand(right, p->i8.n, p->i8.k, p->i8.s_r)};
@@ -382,11 +398,12 @@ int eir_contract_int8(eir_plan *p, void const *left, void const *right, float co
     return launched(eir::launch_i8_row(p->i8, a, num_sms, st), "8-bit contraction launch");
   }
   const int64_t ld = packed_stride(p->i8.k);
-  if (ops[0].copy || ops[1].copy) {
+  const bool copies = ops[0].copy || ops[1].copy;
+  eir::I8Pack packs[2] = {};
+  if (copies) {
     void *ws = nullptr;
     rc = workspace(p, st, &ws);
     if (rc != EIR_SUCCESS) return rc;
-    eir::I8Pack packs[2] = {};
     for (int i = 0; i < 2; ++i) {
       I8Operand &o = ops[i];
       if (!o.copy) continue;
@@ -395,19 +412,18 @@ int eir_contract_int8(eir_plan *p, void const *left, void const *right, float co
       o.ptr = to;
       o.stride = ld;
     }
-    rc = launched(eir::launch_i8_pack(packs[0], packs[1], p->i8.k, ld, num_sms, st), "8-bit operand copy");
-    if (rc != EIR_SUCCESS) return rc;
   }
   CUtensorMap map_t, map_c;
   rc = i8_map(ops[0], p->i8.k, eir::i8_box_tokens(p->i8_tc), false, &map_t);
   if (rc != EIR_SUCCESS) return rc;
   rc = i8_map(ops[1], p->i8.k, 128, p->i8.act == EIR_ACT_GATED_SILU, &map_c);
   if (rc != EIR_SUCCESS) return rc;
-  {
+  if (copies) rc = launched(eir::launch_i8_pack(packs[0], packs[1], p->i8.k, ld, num_sms, st), "8-bit operand copy");
+  if (rc == EIR_SUCCESS) {
     ProfScope prof(p, st);
     rc = launched(eir::launch_i8_tc(p->i8_tc, map_c, map_t, p->i8, a, err, st), "8-bit contraction launch");
   }
-  return rc == EIR_SUCCESS && (ops[0].copy || ops[1].copy) ? workspace_used(p, st) : rc;
+  return copies ? workspace_used(p, st, rc) : rc;
 }
 
 // ---------------------------------------------------------------- log probabilities

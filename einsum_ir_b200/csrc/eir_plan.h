@@ -118,6 +118,7 @@ struct eir_plan {
   int64_t split_ws_offset = 0;  // split-K partial tiles: ws + this offset
   int ws_device = -1;
   cudaEvent_t ws_used = nullptr;  // the workspace is pool memory, in use until this event
+  cudaStream_t ws_stream = nullptr;  // of its last use
 
   // ---- output gather (eir_contract_gather)
   bool out_dense = false;         // the output is one contiguous block of out_elems

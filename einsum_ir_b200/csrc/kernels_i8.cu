@@ -1,83 +1,30 @@
-// Contraction of 8-bit integers on the CUDA cores, for operands that the
-// tensor cores cannot take, and the copy that lays rows out for them.
+// The 8-bit contraction's smaller kernels: a contraction over nothing (k = 0), and the copy that
+// lays rows out for the tensor cores.
 #include "eir_launch.h"
 #include "i8_common.cuh"
 #include "row_vec.cuh"
 
 namespace eir {
 
-// 64 tokens x 64 channels (gated: 32 gates and their 32 values) a CTA, K
-// staged in shared memory byte by byte in blocks of 64, so that any stride
-// and alignment will do; 4-way byte dot products (dp4a).
-constexpr int kI8Tile = 64, kI8Block = 64, kI8Pitch = kI8Block / 4 + 1;
-
-__global__ void __launch_bounds__(256) i8_simt_kernel(const I8Params p, const I8Ptrs a) {
-  __shared__ uint32_t sl[kI8Tile * kI8Pitch], sr[kI8Tile * kI8Pitch];
+// k = 0: every sum is 0, and the epilogue alone is left; an output a thread at a time
+__global__ void __launch_bounds__(256) i8_bias_kernel(const I8Params p, const I8Ptrs a) {
   pdl_launch_dependents();
   pdl_wait();
   const bool gated = p.act == EIR_ACT_GATED_SILU;
-  const int64_t n_out = gated ? p.n / 2 : p.n;
-  const int per = gated ? kI8Tile / 2 : kI8Tile;  // output channels of a CTA
-  const uint32_t c_tiles = (uint32_t)((n_out + per - 1) / per);
-  const int64_t t0 = (int64_t)(blockIdx.x / c_tiles) * kI8Tile, c0 = (int64_t)(blockIdx.x % c_tiles) * per;
-  // the tile's right row j: channel c0 + j, or for the values of a gated tile its value channel
-  auto channel = [&](int j) { return j < per ? c0 + j : c0 + (j - per) + n_out; };
-  const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
-  int32_t acc[4][4] = {};
-  for (int64_t k0 = 0; k0 < p.k; k0 += kI8Block) {
-    __syncthreads();
-    for (int i = threadIdx.x; i < kI8Tile * kI8Block; i += 256) {
-      const int j = i / kI8Block, b = i % kI8Block;
-      const int64_t k = k0 + b, t = t0 + j, c = channel(j);
-      const bool own = j < per ? c < n_out : c < p.n;
-      reinterpret_cast<int8_t *>(sl + j * kI8Pitch)[b] = (k < p.k && t < p.m) ? a.l[t * p.s_l + k] : 0;
-      reinterpret_cast<int8_t *>(sr + j * kI8Pitch)[b] = (k < p.k && own) ? a.r[c * p.s_r + k] : 0;
-    }
-    __syncthreads();
-#pragma unroll
-    for (int kk = 0; kk < kI8Block / 4; ++kk) {
-      uint32_t l[4], r[4];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        l[i] = sl[(ty + 16 * i) * kI8Pitch + kk];
-        r[i] = sr[(tx + 16 * i) * kI8Pitch + kk];
-      }
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) acc[i][j] = __dp4a((int)l[i], (int)r[j], acc[i][j]);
-    }
-  }
+  const int64_t n_out = gated ? p.n / 2 : p.n, step = (int64_t)gridDim.x * 256;
   const float low = p.act == EIR_ACT_RELU ? 0.f : -INFINITY;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int64_t t = t0 + ty + 16 * i;
-    if (t >= p.m) continue;
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < p.m * n_out; i += step) {
+    const int64_t t = i / n_out, c = i - t * n_out;
     const float sa = a.scale_l ? a.scale_l[t] : 1.f;
-    auto z = [&](int j) {  // tile column tx + 16 j
-      const int64_t c = channel(tx + 16 * j);
-      return i8_scaled(acc[i][j], sa, a.scale_r ? a.scale_r[c] : 1.f, a.bias ? a.bias[c] : 0.f);
-    };
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int64_t c = c0 + tx + 16 * j;
-      if (gated && j >= 2) break;
-      if (c >= n_out) continue;
-      float v = z(j);
-      if (gated) v = silu(v) * z(j + 2 < 4 ? j + 2 : 3);
-      else v = relu_from(v, low);
-      st_any(a.out, p.dt_out, t * p.s_out + c, v);
-    }
+    auto z = [&](int64_t ch) { return i8_scaled(0, sa, a.scale_r ? a.scale_r[ch] : 1.f, a.bias ? a.bias[ch] : 0.f); };
+    st_any(a.out, p.dt_out, t * p.s_out + c, gated ? silu(z(c)) * z(c + n_out) : relu_from(z(c), low));
   }
 }
 
-cudaError_t launch_i8_simt(I8Params const &p, I8Ptrs const &a, cudaStream_t st) {
-  const bool gated = p.act == EIR_ACT_GATED_SILU;
-  const int64_t n_out = gated ? p.n / 2 : p.n, per = gated ? kI8Tile / 2 : kI8Tile;
-  const int64_t tiles = ((n_out + per - 1) / per) * ((p.m + kI8Tile - 1) / kI8Tile);
-  if (tiles > INT32_MAX) return cudaErrorInvalidConfiguration;
-  const dim3 grid((unsigned)tiles);
-  return launch_kernel(i8_simt_kernel, grid, dim3(256), 0, st, p, a);
+cudaError_t launch_i8_bias(I8Params const &p, I8Ptrs const &a, int num_sms, cudaStream_t st) {
+  const int64_t n_out = p.act == EIR_ACT_GATED_SILU ? p.n / 2 : p.n;
+  const int64_t blocks = (p.m * n_out + 255) / 256, most = (int64_t)num_sms * 8;
+  return launch_kernel(i8_bias_kernel, dim3((unsigned)(blocks < most ? blocks : most)), dim3(256), 0, st, p, a);
 }
 
 // Rows of k bytes of one or two operands into rows `ld` bytes apart (a multiple of 16): TMA

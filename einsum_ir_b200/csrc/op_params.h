@@ -85,7 +85,8 @@ cudaError_t launch_norm_dweight(NormParams const &p, float const *part, int64_t 
                                 cudaStream_t st);
 cudaError_t launch_quantize(QuantizeParams const &p, void const *x, int8_t *q, float *scale, uint32_t *err,
                             int num_sms, cudaStream_t st);
-cudaError_t launch_i8_simt(I8Params const &p, I8Ptrs const &a, cudaStream_t st);
+// k = 0: scales, bias and activation alone
+cudaError_t launch_i8_bias(I8Params const &p, I8Ptrs const &a, int num_sms, cudaStream_t st);
 cudaError_t launch_i8_tc(I8TcPlan const &tp, CUtensorMap const &map_channels, CUtensorMap const &map_tokens,
                          I8Params const &p, I8Ptrs const &a, uint32_t *err, cudaStream_t st);
 // one token (m = 1), any stride and alignment

@@ -12,9 +12,11 @@
  * The conventions are those of eir_cuda.h: int status codes, no exceptions,
  * plans that are destroyed with eir_plan_destroy, device pointers owned by the
  * caller, calls asynchronous on `stream` (NULL = the legacy default stream).
- * A plan with a workspace (eir_plan_workspace_bytes() > 0; allocated on the
- * first call on a device, so make that call before a stream capture) must not
- * run on two streams at once.
+ * A plan with a workspace (eir_plan_workspace_bytes() > 0) takes its memory on the first
+ * call on a device that needs it; such a call is refused in a stream capture
+ * (EIR_INVALID_ARGUMENT). On another stream the next call waits for the last one's use
+ * of it; a captured call does not, so graphs that hold one plan's calls run one
+ * after another, and end before the plan is destroyed.
  *
  * Matrices are row-major with unit column stride; a row stride is in elements.
  * An input's row stride may be any value >= 0 (0: every row is the same

@@ -361,6 +361,14 @@ def test_contract_int8_empty_sum_broadcast_and_nan(cuda, m):
     assert torch.isnan(y[1]).all() and torch.equal(y[0], want[0]) and torch.equal(y[2:], want[2:])
 
 
+@pytest.mark.parametrize("out", [F32, BF16])
+@pytest.mark.parametrize("act", ACTS)
+@pytest.mark.parametrize("m,n", [(1, 2), (33, 130), (3001, 2050)])
+def test_contract_int8_no_sum(cuda, m, n, act, out):
+    """k = 0: scales, bias and activation alone"""
+    contract_case(m, n, 0, act, out)
+
+
 def test_contract_int8_other_stream_and_reuse(cuda):
     s = torch.cuda.Stream()
     for m in (1, 24, 300):
@@ -580,3 +588,59 @@ def test_repeats_are_equal(cuda, case):
     for _ in range(60):
         for k, v in again().items():
             assert v is None or torch.equal(v, first[k]), k
+
+
+def test_workspaces_over_streams(cuda):
+    """calls of one plan on two streams share its workspace in turn"""
+    g = gen(11)
+    rows, cols, m, n, k = 700, 1500, 300, 520, 1023
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    norm, product = op.NormPlan(rows, cols, cabi.FP32), op.Int8ContractPlan(m, n, k, dtype_out=cabi.FP32)
+    rstd = torch.rand(rows, generator=g, device="cuda") + 0.5
+    h = torch.randn(rows, cols, generator=g, device="cuda")
+    dy = [torch.randn(rows, cols, generator=g, device="cuda") for _ in range(2)]
+    b = codes(g, n, k)
+    a = [codes(g, m, k) for _ in range(2)]
+    dw = [torch.empty(cols, device="cuda") for _ in range(20)]
+    y = [torch.empty(m, n, device="cuda") for _ in range(20)]
+    dx = torch.empty(2, rows, cols, device="cuda")
+    torch.cuda.synchronize()
+    for i in range(20):
+        s = streams[i % 2].cuda_stream
+        norm.backward(dy[i % 2], h, rstd, dx[i % 2], dweight=dw[i], stream=s)
+        product.contract(a[i % 2], b, None, None, y[i], stream=s)
+    torch.cuda.synchronize()
+    cabi.check_device_errors()
+    for i in range(2):
+        exact = contract64(a[i], b, None, None, None, 0).float()
+        want = (dy[i].double() * h.double() * rstd.double()[:, None]).sum(0)
+        assert all(torch.equal(v, exact) for v in y[i::2]) and all(torch.equal(v, dw[i]) for v in dw[i::2])
+        # a product's two roundings and the order of `rows` sums
+        close(dw[i], want, (rows + 3) * U * (dy[i].double() * h.double() * rstd.double()[:, None]).abs().sum(0))
+
+
+def test_workspaces_in_a_capture(cuda):
+    """a first call that needs memory is refused in a capture; one after it is captured and replayed"""
+    contract_case(2, 16, 32, op.ACT_NONE, F32)  # the device's own state exists
+    g = gen(12)
+    a, b = codes(g, 300, 1023), codes(g, 520, 1023)
+    y = torch.empty(300, 520, device="cuda")
+    plan = op.Int8ContractPlan(300, 520, 1023, dtype_out=cabi.FP32)
+    exact = contract64(a, b, None, None, None, 0).float()
+    graph, stream = torch.cuda.CUDAGraph(), torch.cuda.Stream()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph, stream=stream):
+        y.zero_()
+        with pytest.raises(cabi.EirError):
+            plan.contract(a, b, None, None, y, stream=stream.cuda_stream)
+    plan.contract(a, b, None, None, y)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=stream):
+        plan.contract(a, b, None, None, y, stream=stream.cuda_stream)
+    y.zero_()
+    graph.replay()
+    torch.cuda.synchronize()
+    cabi.check_device_errors()
+    assert torch.equal(y, exact)
+    del graph

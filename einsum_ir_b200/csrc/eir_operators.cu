@@ -225,7 +225,7 @@ int eir_norm_plan_create(eir_norm_desc const *d, eir_plan **out) {
     n.s_dx = d->stride_dx;
     p->empty = d->rows == 0;
     // partial rows of the weight gradient
-    p->ws_bytes = eir::norm_backward_parts(n, eir::kMaxSms) * d->cols * 4;
+    p->ws_bytes = eir::norm_backward_parts(n, eir::kMaxSms) * eir::norm_part_pitch(d->cols) * 4;
     p->text = std::string("norm ") + type_text(n.dt) + " -> " + type_text(n.dt_out) + " rows=" +
               std::to_string(n.rows) + " cols=" + std::to_string(n.cols);
   });

@@ -541,19 +541,31 @@ struct NormBackRow {
   }
 };
 
+// V columns of a partial row (column a multiple of V; the pitch has room for whole 16-byte pieces)
+template <int V>
+__device__ __forceinline__ void put_part(float *part, int64_t column, int64_t cols, float const (&v)[V]) {
+#pragma unroll
+  for (int e = 0; e < V; e += 4)
+    if (column + e < cols)
+      *reinterpret_cast<float4 *>(part + column + e) = make_float4(v[e], v[e + 1], v[e + 2], v[e + 3]);
+}
+
 // Narrow rows: a warp a row, the next one loaded early. The weight gradient of the
-// warp's columns stays in registers over all rows that it sees and is written as one
-// partial row, summed by norm_dweight_kernel: no atomics, so the order is fixed. (So too below, a
-// block a partial row.)
+// warp's columns stays in registers over all rows that it sees; the block's warps add theirs through
+// shared memory into one partial row, summed by norm_dweight_kernel: no atomics, so the order is
+// fixed. (So too below, a block a partial row.)
+constexpr int kBackWarps = 16;
 template <typename T, typename G, bool GRID>
-__global__ void __launch_bounds__(128) norm_backward_kernel(const NormParams p, const NormGradPtrs a) {
+__global__ void __launch_bounds__(kBackWarps * 32) norm_backward_kernel(const NormParams p, const NormGradPtrs a) {
   using Row = NormBackRow<T, G, GRID>;
   constexpr int V = Row::V, N = kPerBack / V;
   pdl_launch_dependents();
   pdl_wait();
   const Row op(p, a);
   const int lane = threadIdx.x & 31;
-  const int64_t at_once = (int64_t)gridDim.x * 4, first = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5);
+  const int warp = threadIdx.x >> 5;
+  const int64_t at_once = (int64_t)gridDim.x * kBackWarps, first = (int64_t)blockIdx.x * kBackWarps + warp;
+  extern __shared__ float warp_dw[];  // [warp][column]
   auto column = [&](int j) { return (int64_t)(j * 32 + lane) * V; };
   typename Row::PieceH h[N];
   typename Row::PieceG dy[N], ds[N];
@@ -589,13 +601,19 @@ __global__ void __launch_bounds__(128) norm_backward_kernel(const NormParams p, 
 #pragma unroll
     for (int j = 0; j < N; ++j) op.give(row, column(j), held[j], hr[j], k);
   }
-  if (a.part != nullptr && first < p.rows) {
-    float *part = a.part + first * p.cols;
+  if (a.part == nullptr) return;
 #pragma unroll
-    for (int j = 0; j < N; ++j)
+  for (int j = 0; j < N; ++j)
 #pragma unroll
-      for (int e = 0; e < V; ++e)
-        if (column(j) + e < p.cols) part[column(j) + e] = dw[j][e];
+    for (int e = 0; e < V; ++e)
+      if (column(j) + e < p.cols) warp_dw[warp * p.cols + column(j) + e] = dw[j][e];
+  __syncthreads();
+  float *part = a.part + (int64_t)blockIdx.x * norm_part_pitch(p.cols);
+  for (int c = threadIdx.x; c < p.cols; c += kBackWarps * 32) {
+    float sum = warp_dw[c];
+#pragma unroll
+    for (int w = 1; w < kBackWarps; ++w) sum += warp_dw[w * p.cols + c];
+    part[c] = sum;
   }
 }
 
@@ -688,12 +706,9 @@ __global__ void __launch_bounds__(kBackThreads + 32, back_blocks(N * NormBackRow
     }
   }
   if (a.part != nullptr) {
-    float *part = a.part + (int64_t)blockIdx.x * p.cols;
+    float *part = a.part + (int64_t)blockIdx.x * norm_part_pitch(p.cols);
 #pragma unroll
-    for (int j = 0; j < N; ++j)
-#pragma unroll
-      for (int e = 0; e < V; ++e)
-        if (column(j) + e < p.cols) part[column(j) + e] = dw[j][e];
+    for (int j = 0; j < N; ++j) put_part<V>(part, column(j), p.cols, dw[j]);
   }
 }
 
@@ -713,7 +728,7 @@ __global__ void __launch_bounds__(512) norm_backward_wide_kernel(const NormParam
   uint32_t *held_h = held_words + threadIdx.x;
   float *held_g = reinterpret_cast<float *>(held_h + pieces * W * threads);
   float *held_w = held_g + pieces * V * threads;
-  float *part = a.part ? a.part + (int64_t)blockIdx.x * p.cols : nullptr;
+  float *part = a.part ? a.part + (int64_t)blockIdx.x * norm_part_pitch(p.cols) : nullptr;
   auto column = [&](int j) { return ((int64_t)j * threads + threadIdx.x) * V; };
   if (CACHED) {
     for (int i = 0; i < pieces * V; ++i) held_w[i * threads] = 0.f;
@@ -785,25 +800,41 @@ __global__ void __launch_bounds__(512) norm_backward_wide_kernel(const NormParam
   }
 }
 
-// dw[c] = sum of the partial rows: 32 columns a block, thread row y adds the
-// rows y, y + 32, ..., and the 32 sums are added in order
+// dw[c] = sum of the partial rows: COLS columns a block in 16-byte pieces (the partial rows' pitch
+// is a multiple of 16 bytes), ROWS rows at once, whose sums are added in order
+template <int COLS>
 __global__ void __launch_bounds__(1024) norm_dweight_kernel(int64_t cols, float const *__restrict__ part,
-                                                            int64_t n_part, float *__restrict__ dw) {
-  __shared__ float sums[32][33];
+                                                            int64_t pitch, int64_t n_part, float *__restrict__ dw) {
+  constexpr int ROWS = 4096 / COLS;
+  __shared__ float sums[ROWS][COLS + 1];
   pdl_launch_dependents();
   pdl_wait();
-  const int x = threadIdx.x & 31, y = threadIdx.x >> 5;
-  const int64_t c = (int64_t)blockIdx.x * 32 + x;
-  float s = 0.f;
+  const int x = threadIdx.x % (COLS / 4) * 4, y = threadIdx.x / (COLS / 4);
+  const int64_t c = (int64_t)blockIdx.x * COLS + x;
+  float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
   if (c < cols) {
-#pragma unroll 8
-    for (int64_t i = y; i < n_part; i += 32) s += part[i * cols + c];
+    for (int64_t i = y; i < n_part; i += 4 * ROWS) {
+      float4 v[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        v[j] = i + ROWS * j < n_part ? *reinterpret_cast<float4 const *>(part + (i + ROWS * j) * pitch + c)
+                                     : make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) s = make_float4(s.x + v[j].x, s.y + v[j].y, s.z + v[j].z, s.w + v[j].w);
+    }
   }
-  sums[y][x] = s;
+  sums[y][x] = s.x;
+  sums[y][x + 1] = s.y;
+  sums[y][x + 2] = s.z;
+  sums[y][x + 3] = s.w;
   __syncthreads();
-  // the warp y adds column y's partial sums
-  s = warp_sum(sums[x][y]);
-  if (x == 0 && (int64_t)blockIdx.x * 32 + y < cols) dw[(int64_t)blockIdx.x * 32 + y] = s;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;  // a warp a column
+  if (warp >= COLS) return;
+  float t = 0.f;
+#pragma unroll
+  for (int i = 0; i < ROWS; i += 32) t += sums[i + lane][warp];
+  t = warp_sum(t);
+  if (lane == 0 && (int64_t)blockIdx.x * COLS + warp < cols) dw[(int64_t)blockIdx.x * COLS + warp] = t;
 }
 
 // ---------------------------------------------------------------- launchers
@@ -931,8 +962,8 @@ static int64_t back_ring_blocks(int64_t cols, int *threads) {
 }
 
 int64_t norm_backward_parts(NormParams const &p, int num_sms) {
-  int threads = 0;  // (narrow rows: 8 blocks of 4 warps an SM; wide ones: 2 blocks)
-  const int64_t an_sm = p.cols <= 32 * kPerBack ? 32 : std::max<int64_t>(2, back_ring_blocks(p.cols, &threads));
+  int threads = 0;  // (narrow rows and wide ones: 2 blocks an SM)
+  const int64_t an_sm = p.cols <= 32 * kPerBack ? 2 : std::max<int64_t>(2, back_ring_blocks(p.cols, &threads));
   return std::min<int64_t>(p.rows, num_sms * an_sm);
 }
 
@@ -946,10 +977,9 @@ static cudaError_t launch_norm_backward_t(NormParams const &p, NormGradPtrs cons
                     row_vec_ok(a.dx, p.s_dx, p.rows, sizeof(G), V) &&
                     row_vec_ok(a.w, 0, 1, p.dt_w == EIR_FP32 ? 4 : 2, V);
   if (p.cols <= 32 * kPerBack) {
-    const RowGrid g = row_grid(p.rows, p.cols, kPerBack, num_sms);
-    *parts = std::min(g.grid * 4, p.rows);
+    *parts = std::min<int64_t>((p.rows + kBackWarps - 1) / kBackWarps, num_sms * 2);
     auto kern = grid ? norm_backward_kernel<T, G, true> : norm_backward_kernel<T, G, false>;
-    return launch_kernel(kern, dim3((unsigned)g.grid), dim3(g.threads), 0, st, p, a);
+    return launch_kernel(kern, dim3((unsigned)*parts), dim3(kBackWarps * 32), (size_t)(kBackWarps * 4 * p.cols), st, p, a);
   }
   const int per = back_per(p.cols);
   RingShape r;
@@ -986,8 +1016,11 @@ cudaError_t launch_norm_backward(NormParams const &p, NormGradPtrs const &a, uin
 
 cudaError_t launch_norm_dweight(NormParams const &p, float const *part, int64_t n_part, float *dw,
                                 cudaStream_t st) {
-  return launch_kernel(norm_dweight_kernel, dim3((unsigned)((p.cols + 31) / 32)), dim3(1024), 0, st, p.cols, part,
-                       n_part, dw);
+  // narrower blocks where wide ones leave SMs without work
+  const int n = p.cols >= 4096 ? 32 : p.cols >= 2048 ? 16 : 8;
+  auto kern = n == 32 ? norm_dweight_kernel<32> : n == 16 ? norm_dweight_kernel<16> : norm_dweight_kernel<8>;
+  return launch_kernel(kern, dim3((unsigned)((p.cols + n - 1) / n)), dim3(1024), 0, st, p.cols, part,
+                       norm_part_pitch(p.cols), n_part, dw);
 }
 
 }  // namespace eir

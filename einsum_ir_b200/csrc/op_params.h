@@ -77,6 +77,8 @@ struct LogprobGradPtrs {
 };
 
 cudaError_t launch_norm(NormParams const &p, NormPtrs const &a, uint32_t *err, int num_sms, cudaStream_t st);
+// elements between the partial rows of the weight gradient: 16-byte pieces
+__host__ __device__ inline int64_t norm_part_pitch(int64_t cols) { return (cols + 3) & ~(int64_t)3; }
 // the most partial rows of the weight gradient that the backward kernels write; *parts: how many
 int64_t norm_backward_parts(NormParams const &p, int num_sms);
 cudaError_t launch_norm_backward(NormParams const &p, NormGradPtrs const &a, uint32_t *err, int num_sms,

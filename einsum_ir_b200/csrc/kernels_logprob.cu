@@ -1,23 +1,26 @@
 // Log probabilities of given tokens, log-sum-exp, entropy and top alternatives
 // of rows of logits, and the gradient of the first and third.
 //
-// One pass over a row, in base 2 (L = log2 e): with a reference R >= about the row's
+// One pass over a row, in base 2 (L = log2 e): with a reference R near the row's
 // maximum times L, S = sum 2^d and U = sum d 2^d for d = x L - R give
 // lse = (R + log2 S) / L, log p = (d - log2 S) / L and entropy = (log2 S - U / S) / L. Any R will do, so
 // rounding it costs nothing; a thread raises its own when it meets a larger logit and its
 // sums shrink by 2^(R - R'). Logits are floored at -1e37, where 2^d is 0, so that
 // a ruled-out one (-infinity) adds 0 d = 0 to U.
 //
-// Bound by HBM (a logit is read once; the one exponential an element takes 73 %
-// of the SM's rate at BF16 and full bandwidth). A piece is 16 bytes of memory on
+// At BF16 bound by the SM's pipes (4096 x 32768: 53 us, 5.1 TB/s; exponentials 63 % of their
+// rate, issue 62 %), at FP32 by HBM (4096 x 32768, 5 alternatives: 105 us, 5.1 TB/s). A logit is read once. A piece is 16 bytes of memory on
 // the 16-byte grid, so rows of any alignment stream alike; the elements of
 // the first and last piece that lie outside the row count as ruled out.
 //
-// Top alternatives without a second pass: each thread keeps its largest logit and the
-// piece it came from. The k-th largest of these (ties: the earlier piece) is a
-// lower bound of the row's k-th largest logit, and only the k threads that hold
-// larger ones can hold an alternative: their pieces are read again (k / threads of the row, from
-// L2), and the few candidates above the bound are sorted. Order by one 64-bit key,
+// Top alternatives without a second pass: each thread keeps its largest logit, the
+// piece it came from, and the largest logit of its other chunks. The k-th largest of the threads'
+// logits (ties: the earlier piece) is a lower bound of the row's k-th largest, and only the k threads that
+// hold larger ones can hold an alternative: the chunk of their largest logit is read again (4 pieces of
+// 16 bytes), their other chunks only where the largest logit of these reaches the bound too (all
+// chunks: 65.8 us instead of 61.4 for 4096 x 32768 BF16 and 5 alternatives, 95 instead of 77
+// for 20; a looser bound from fewer maxima that each thread compares with its own: 81 and 133).
+// The few candidates above the bound are sorted. Order by one 64-bit key,
 // logit first and lower index second, so that the result does not depend on the order of work.
 //
 // Rows that do not fill the GPU by number are split over a cluster of up to 8 blocks, joined
@@ -75,32 +78,43 @@ __device__ __forceinline__ float log_ref(float m) { return m < kLowest ? 0.f : m
 __device__ __forceinline__ float log_prob(float x, LogSums const &v, float log_s) {
   return x < kLowest ? x - v.m : (fmaf(x, kLog2e, -log_ref(v.m)) - log_s) * kLn2;
 }
-// sums moved to the reference of a larger maximum (sums of 0 may stand beside any reference)
-__device__ __forceinline__ LogSums log_rebase(LogSums v, float m) {
-  const float d = log_ref(v.m) - log_ref(m), e = exp2_fast(d);
-  if (v.S == 0.f) return LogSums{m, 0.f, 0.f};
-  return LogSums{m, e * v.S, e * (v.U + d * v.S)};
+// sums against R moved to the reference of the maximum m (sums of 0 may stand beside any reference)
+__device__ __forceinline__ LogSums log_moved(float R, float S, float U, float m) {
+  const float d = R - log_ref(m), e = exp2_fast(d);
+  if (S == 0.f) return LogSums{m, 0.f, 0.f};
+  return LogSums{m, e * S, e * (U + d * S)};
 }
 // the sums of the warp's lanes
 __device__ __forceinline__ LogSums log_join_lanes(LogSums v) {
   // (signed integers in the order of the floats; a NaN is no maximum here, but stays in S)
   const int b = __float_as_int(v.m == v.m ? v.m : -INFINITY);
   const int most = __reduce_max_sync(0xffffffffu, b ^ ((b >> 31) & 0x7fffffff));
-  v = log_rebase(v, __int_as_float(most ^ ((most >> 31) & 0x7fffffff)));
+  v = log_moved(log_ref(v.m), v.S, v.U, __int_as_float(most ^ ((most >> 31) & 0x7fffffff)));
   v.S = warp_sum(v.S);
   v.U = warp_sum(v.U);
   return v;
 }
 
+// a row's target: its place (-1: left out; vocab: off the row) and its logit
+struct LogTarget {
+  int place;
+  float x;
+};
+template <typename T>
+__device__ __forceinline__ LogTarget log_target(LogprobParams const &p, LogprobPtrs const &a, int64_t row) {
+  const int64_t t = a.targets ? a.targets[row] : -1;
+  LogTarget g{t < 0 ? -1 : (int)(t < p.vocab ? t : p.vocab), 0.f};
+  if (t >= 0 && t < p.vocab) g.x = to_f32(static_cast<T const *>(a.x)[row * p.s_x + t]);
+  return g;
+}
+
 // one row's values, written by one thread
 __device__ __forceinline__ void logprob_row_values(LogprobParams const &p, LogprobPtrs const &a, int64_t row, bool none,
-                                                   float lse, float entropy, float target_logprob) {
+                                                   float lse, float entropy, int target, float target_logprob) {
   if (a.lse) a.lse[row] = lse;
   if (a.entropy) a.entropy[row] = none ? 0.f : entropy;
-  if (a.targets) {
-    const int64_t t = a.targets[row];
-    a.logprob[row] = t < 0 ? 0.f : (t >= p.vocab ? logit_nan() : (none ? -INFINITY : target_logprob));
-  }
+  if (a.targets)
+    a.logprob[row] = target < 0 ? 0.f : (target >= p.vocab ? logit_nan() : (none ? -INFINITY : target_logprob));
 }
 
 // A row by plain passes (all threads of the block): right for every row, a
@@ -139,9 +153,8 @@ __device__ __noinline__ void logprob_plain_row(LogprobParams const &p, LogprobPt
   const bool none = S == 0.f;
   const float log_s = logf(S);
   if (threadIdx.x == 0) {
-    const int64_t t = a.targets ? a.targets[row] : -1;
-    const float xt = t >= 0 && t < p.vocab ? to_f32(x[t]) : 0.f;
-    logprob_row_values(p, a, row, none, none ? -INFINITY : ref + log_s, log_s - U / S, xt - ref - log_s);
+    const LogTarget t = log_target<T>(p, a, row);
+    logprob_row_values(p, a, row, none, none ? -INFINITY : ref + log_s, log_s - U / S, t.place, t.x - ref - log_s);
   }
   uint64_t last = ~0ull;
   for (int i = 0; i < p.top; ++i) {
@@ -253,6 +266,7 @@ struct LogShared {
   static constexpr int kCandidates = THREADS < 64 ? 256 : 4 * THREADS;  // (a merge of 8 blocks takes 8 x 32)
   float red[96];           // (m, S, U) of the warps; the plain row's words
   uint64_t keys[THREADS];  // the threads' largest logits
+  float second[THREADS];   // and the largest ones of their other chunks
   uint64_t plain[32];      // the plain row's words
   uint64_t top[32];        // the block's alternatives
   uint64_t found[kCandidates];
@@ -331,13 +345,19 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS)
     for (int s = 0; s < kLogStages; ++s)
       if (inner(k0 + s * warps)) copy(k0 + s * warps, s);
   }
+  LogTarget target{-1, 0.f};  // (read now: the end of the row would wait for it twice)
+  if (threadIdx.x == 0 && rank == 0) target = log_target<T>(p, a, row);
   uint32_t phases = 0;  // of the warp's stages
   int stage = 0;
   // ---- the pass
   LogSums v{-INFINITY, 0.f, 0.f};
   float2 S2 = make_float2(0.f, 0.f), U2 = make_float2(0.f, 0.f);
-  float R = 0.f;
+  // The reference stays while no logit is more than 5.5 above it (S grows by 2^8 at most, which
+  // costs U / S 2^-21 of rounding): a new maximum, which some lane meets in most
+  // chunks, then is no branch
+  float R = 0.f, limit = -INFINITY;
   int best = p0 + warp * kChunk + lane;  // the piece that holds v.m
+  float second = -INFINITY;  // the largest logit of the thread's other chunks
   auto add_pieces = [&](Piece const (&c)[AT_ONCE], int q) {
     float l[AT_ONCE], most = -INFINITY;
 #pragma unroll
@@ -345,17 +365,20 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS)
       l[i] = Row::largest(c[i]);
       most = fmaxf(most, l[i]);
     }
-    if (most > v.m) {
-      v.m = most;
+    int first = AT_ONCE - 1;
 #pragma unroll
-      for (int i = AT_ONCE - 1; i >= 0; --i)
-        if (l[i] == most) best = q + i * 32;
+    for (int i = AT_ONCE - 2; i >= 0; --i) first = l[i] == most ? i : first;
+    best = most > v.m ? q + 32 * first : best;
+    second = fmaxf(second, fminf(v.m, most));
+    v.m = fmaxf(v.m, most);
+    if (most > limit) {
       const float to = log_ref(most), d = R - to, e = exp2_fast(d);
       if (S2.x + S2.y != 0.f) {  // (sums of 0 may stand beside any reference)
         U2 = make_float2(e * (U2.x + d * S2.x), e * (U2.y + d * S2.y));
         S2 = make_float2(e * S2.x, e * S2.y);
       }
       R = to;
+      limit = most + 5.5f;
     }
 #pragma unroll
     for (int i = 0; i < AT_ONCE; ++i) {
@@ -391,56 +414,76 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS)
     }
     add_pieces(c, q);
   }
-  v.S = S2.x + S2.y;
-  v.U = U2.x + U2.y;
-  // ---- the block's sums, and the threads' largest logits
   const float own = v.m;
+  v = log_moved(R, S2.x + S2.y, U2.x + U2.y, own);
+  // ---- the block's sums, and the threads' largest logits
   v = log_join_lanes(v);
   if (lane == 0) {
     sh.red[warp] = v.m;
     sh.red[32 + warp] = v.S;
     sh.red[64 + warp] = v.U;
   }
-  if (p.top > 0)  // (the end of the piece stands for the logit's place: a lower bound)
+  if (p.top > 0) {  // (the end of the piece stands for the logit's place: a lower bound)
     sh.keys[threadIdx.x] = best < p1 ? rank_key(own, (uint32_t)(x.first_index(best) + V - 1)) : 0;
-  if (threadIdx.x == 0) sh.n_found = 0;
+    sh.second[threadIdx.x] = second;
+  }
   __syncthreads();
-  v = log_join_lanes(lane < warps ? LogSums{sh.red[lane], sh.red[32 + lane], sh.red[64 + lane]}
-                                  : LogSums{-INFINITY, 0.f, 0.f});
+  if (warp == 0) {
+    v = log_join_lanes(lane < warps ? LogSums{sh.red[lane], sh.red[32 + lane], sh.red[64 + lane]}
+                                    : LogSums{-INFINITY, 0.f, 0.f});
+    if (lane == 0) {
+      sh.sums = v;
+      sh.n_found = 0;
+    }
+    if (p.top > 0) {  // the k largest of the threads' logits
+      uint64_t keys[warps], last = ~0ull, mine = 0;
+#pragma unroll
+      for (int i = 0; i < warps; ++i) keys[i] = sh.keys[32 * i + lane];
+      for (int i = 0; i < p.top; ++i) {
+        last = next_largest<warps>(keys, last);
+        if (last == 0) break;
+        if (lane == i) mine = last;
+      }
+      sh.top[lane] = mine;
+    }
+  }
+  __syncthreads();
+  v = sh.sums;
   // ---- the block's alternatives
   bool full = false;
   if (p.top > 0) {
-    // every warp finds the k largest of the threads' logits, and reads the pieces of some of these threads
-    uint64_t keys[warps], last = ~0ull, mine = 0;
+    const uint64_t bound = sh.top[p.top - 1];  // 0: fewer threads than alternatives, every logit may be one
+    const uint32_t bound_bits = (uint32_t)(bound >> 32);
+    auto find = [&](int q) {
+      const Piece c = x.load(q);
+      if (rank_bits(Row::largest(c)) < bound_bits) return;
 #pragma unroll
-    for (int i = 0; i < warps; ++i) keys[i] = sh.keys[32 * i + lane];
-    int n = 0;
-    for (int i = 0; i < p.top; ++i) {
-      last = next_largest<warps>(keys, last);
-      if (last == 0) break;
-      ++n;
-      if (lane == i) mine = last;
+      for (int e = 0; e < V; ++e) {
+        const int at = x.first_index(q) + e;
+        const uint64_t key = rank_key(c.get(e), (uint32_t)at);
+        if (at < 0 || at >= x.vocab || key < bound) continue;
+        const int slot = atomicAdd(&sh.n_found, 1);
+        if (slot < kCandidates) sh.found[slot] = key;
+      }
+    };
+    auto piece_of = [&](uint64_t key) { return ((int)~(uint32_t)key - (V - 1) + x.off) / V - p0; };
+    // of each thread that holds one of these, the chunk with its largest logit
+    for (int u = threadIdx.x; u < AT_ONCE * p.top; u += THREADS) {
+      const uint64_t key = sh.top[u / AT_ONCE];
+      if (key == 0) break;
+      const int piece = piece_of(key), q = p0 + piece / kChunk * kChunk + u % AT_ONCE * 32 + piece % 32;
+      if (q < p1) find(q);
     }
-    const uint64_t bound = last;  // 0: fewer threads than alternatives, every logit may be one
-    for (int i = warp; i < n; i += warps) {
-      // the pieces of the thread that holds the i-th: one in 32 of its warp's chunks
-      const int end = (int)~(uint32_t)__shfl_sync(0xffffffffu, mine, i);
-      const int piece = (end - (V - 1) + x.off) / V - p0;
-      const int its_warp = piece / kChunk % warps;
+    // and its others where the largest of these reaches the bound
+    for (int i = warp; i < p.top; i += warps) {
+      const uint64_t key = sh.top[i];
+      if (key == 0) break;
+      const int piece = piece_of(key), its_warp = piece / kChunk % warps;
+      if (rank_bits(sh.second[its_warp * 32 + piece % 32]) < bound_bits) continue;
       for (int j = lane;; j += 32) {
-        const int q = p0 + (j / AT_ONCE * warps + its_warp) * kChunk + j % AT_ONCE * 32 + piece % 32;
-        if (q - j % AT_ONCE * 32 >= p1) break;
-        if (q >= p1) continue;
-        const Piece c = x.load(q);
-        if (rank_key(Row::largest(c), 0) < bound) continue;  // (no index is above 2^32 - 1 - 0)
-#pragma unroll
-        for (int e = 0; e < V; ++e) {
-          const int at = x.first_index(q) + e;
-          const uint64_t key = rank_key(c.get(e), (uint32_t)at);
-          if (at < 0 || at >= x.vocab || key < bound) continue;
-          const int slot = atomicAdd(&sh.n_found, 1);
-          if (slot < kCandidates) sh.found[slot] = key;
-        }
+        const int chunk = j / AT_ONCE * warps + its_warp, q = p0 + chunk * kChunk + j % AT_ONCE * 32 + piece % 32;
+        if (chunk >= chunks) break;
+        if (q < p1 && chunk != piece / kChunk) find(q);
       }
     }
     __syncthreads();
@@ -454,10 +497,7 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS)
   // (S is NaN where the row holds a NaN or +infinity)
   bool odd = full || !(v.S == v.S) || v.m > 1e37f || (v.m < kLowest && v.m != -INFINITY);
   if (blocks_a_row > 1) {
-    if (threadIdx.x == 0) {
-      sh.sums = v;
-      sh.odd = odd;
-    }
+    if (threadIdx.x == 0) sh.odd = odd;
     __syncwarp();
     cluster_sync();  // every block's sums and alternatives are in its shared memory
     if (rank == 0) {
@@ -495,11 +535,8 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS)
       const bool none = v.S == 0.f;
       const float ref = log_ref(v.m), log_s = log2f(v.S);
       if (lane == 0) {
-        const int64_t t = a.targets ? a.targets[row] : -1;
-        float xt = 0.f;
-        if (t >= 0 && t < p.vocab) xt = to_f32(static_cast<T const *>(a.x)[row * p.s_x + t]);
         logprob_row_values(p, a, row, none, none ? -INFINITY : (ref + log_s) * kLn2, (log_s - v.U / v.S) * kLn2,
-                           log_prob(xt, v, log_s));
+                           target.place, log_prob(target.x, v, log_s));
       }
       if (lane < p.top) {
         const uint64_t key = (blocks_a_row > 1 ? sh.found : sh.top)[lane];

@@ -504,6 +504,20 @@ def test_logprob_backward(cuda, rows, vocab, pad, offset, dtype):
 
 
 @pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("rows", [2, 400])
+@pytest.mark.parametrize("step", [1, 4, 8, 128, 512, 1024, 2048, 4096, 8192])
+def test_logprob_alternatives_at_a_distance(cuda, step, rows, dtype):
+    """the most likely tokens `step` apart, so that threads, warps and chunks hold several of them"""
+    g = gen(step)
+    x = logits_of(g, rows, 70000, dtype)
+    for r in range(rows):
+        at = (r * 37 + step * torch.arange(8, device="cuda")) % 70000
+        x[r, at] = 40 - torch.randperm(8, generator=g, device="cuda").to(dtype) // 2  # (pairs are ties)
+    t = torch.randint(70000, (rows,), generator=g, device="cuda")
+    check_logprob(x, t, 8, run_logprob(x, t, 8))
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
 @pytest.mark.parametrize("rows,vocab", [(2, 6528), (74, 4736), (568, 3136), (96, 6117), (30, 10007), (9, 24001), (1, 1500)])
 def test_logprob_backward_every_target(cuda, rows, vocab, dtype):
     """targets spread over the whole row: the one-hot term lands in its column whatever thread holds it"""

@@ -133,13 +133,15 @@ int workspace_used(eir_plan *p, cudaStream_t st, int rc) {
 // a cluster, 4 K blocks a CTA at least (the exchange takes 1 to 3 us): the largest cluster of
 // which all tiles' clusters fit the GPU at once, two CTAs an SM (measured
 // limits; a second wave costs more than the split gains: 256 tokens x 4096 x
-// 4096, 64 tiles, take 14.4 us unsplit, 12.5 split by 4 and 21.7 split by 8).
+// 4096, 64 tiles, take 14.4 us unsplit, 11.8 split by 4 and 21.7 split by 8).
 eir::I8TcPlan i8_tiling(eir::I8Params const &p) {
   eir::I8TcPlan t;
   t.c_tiles = (p.n + 255) / 256;  // gated: 128 gates and their values a tile
   t.t_tiles = (p.m + 255) / 256;
   if (p.m > 128 && t.c_tiles * t.t_tiles >= (p.k <= 2048 ? 16 : 32)) return t;
-  t.tokens = p.m <= 16 ? 16 : p.m <= 32 ? 32 : p.m <= 64 ? 64 : 128;
+  t.tokens = 128;
+  for (int n : {96, 80, 64, 32, 16})
+    if (p.m <= n) t.tokens = n;
   t.c_tiles = (p.n + 127) / 128;
   t.t_tiles = (p.m + t.tokens - 1) / t.tokens;
   struct {

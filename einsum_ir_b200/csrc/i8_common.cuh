@@ -60,6 +60,16 @@ __device__ __forceinline__ void tma_load_3d_pair(void *dst, void const *map, uin
       : "memory");
 }
 
+// the same boxes into L2 only. L2 is where all of the GPU's writes meet, so what a kernel that
+// still runs writes afterwards is what a later load reads
+__device__ __forceinline__ void tma_prefetch_2d(void const *map, int c0, int c1) {
+  asm volatile("cp.async.bulk.prefetch.tensor.2d.L2.global [%0, {%1, %2}];" ::"l"(map), "r"(c0), "r"(c1) : "memory");
+}
+__device__ __forceinline__ void tma_prefetch_3d(void const *map, int c0, int c1, int c2) {
+  asm volatile("cp.async.bulk.prefetch.tensor.3d.L2.global [%0, {%1, %2, %3}];" ::"l"(map), "r"(c0), "r"(c1), "r"(c2)
+               : "memory");
+}
+
 // arrive on an mbarrier of any CTA of the cluster without ordering earlier memory accesses
 __device__ __forceinline__ void mbar_arrive_cluster_relaxed(uint32_t bar_cluster) {
   asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar_cluster) : "memory");

@@ -15,7 +15,8 @@
 // * i8_pair_kernel: CTA pairs (cta_group::2) over tiles of 256 rows x 256
 //   tokens, persistent, accumulators double-buffered in TMEM so that the
 //   epilogue runs under the next tile.
-// * i8_split_kernel: one tile of 128 rows x NT tokens (NT = 16 .. 128) for
+// * i8_split_kernel: one tile of 128 rows x NT tokens (NT = 16 .. 128; 77 tokens x 32768 x 1024
+//   take 9.9 us in tiles of 128, 9.1 in tiles of 80) for
 //   problems with too few pair tiles to fill the GPU. A cluster of 1 to 8 CTAs
 //   shares the tile's K walk; each holds a partial accumulator, and the
 //   cluster adds them through distributed shared memory.
@@ -410,7 +411,7 @@ struct I8Split {
   // about 100 KB a CTA, two CTAs on an SM: enough bytes in flight for HBM
   static constexpr int kStages = 104 * 1024 / kStageBytes;
   static constexpr int kRing = kStages * kStageBytes;
-  static constexpr int kCols = NT < 32 ? 32 : NT;  // TMEM
+  static constexpr int kCols = NT <= 32 ? 32 : NT <= 64 ? 64 : 128;  // TMEM
   static constexpr int kThreads = 192;
   static constexpr int kSmemBytes = 1024 + kRing + 512 + 512;
   static_assert(kAccBytes <= kRing, "the exchange reuses the ring");
@@ -465,6 +466,14 @@ __global__ void __launch_bounds__(192, 2)
   tc_fence_after();
   const uint32_t tmem_base = *tmem_slot;
   pdl_launch_dependents();
+  if (threadIdx.x == 0) {
+    // the channels' rows of the first ring set out for L2 while the kernels before this one end
+    // (4 tokens x 32768 x 4096: 23.3 us, 23.9 without; of more K blocks: slower)
+    for (int kb = kb0; kb < min(kb1, kb0 + S); ++kb)
+      i8_load_rows<GATED>(
+          sA, kb * kI8BlockK, (int)c0, [&](void *, int x, int y) { tma_prefetch_2d(&map_c, x, y); },
+          [&](void *, int x, int y) { tma_prefetch_3d(&map_c, x, y, 0); });
+  }
   pdl_wait();
 
   const int64_t t0 = (int64_t)tt * NT;
@@ -596,17 +605,7 @@ __global__ void __launch_bounds__(192, 2)
       const uint32_t at = smem_u32(s_acc) + 16u * (uint32_t)lane;
       T *out = static_cast<T *>(a.out) + t0 * p.s_out + cq;
       const bool wide = p.s_out % 4 == 0 && reinterpret_cast<uintptr_t>(a.out) % (4 * sizeof(T)) == 0 && cq + 4 <= n_out;
-#pragma unroll 2
-      for (int j = (int)rank + warp * (int)split; j < tokens; j += 6 * (int)split) {
-        int4 acc = make_int4(0, 0, 0, 0);
-#pragma unroll 8
-        for (uint32_t r = 0; r < split; ++r) {
-          const int4 v = ld_cluster_v4(mapa_shared(at + (uint32_t)(j * kI8Rows * 4), r));
-          acc.x += v.x;
-          acc.y += v.y;
-          acc.z += v.z;
-          acc.w += v.w;
-        }
+      auto finish = [&](int j, int4 const &acc) {
         const float sa = s_scale[j];
         float z[4] = {i8_scaled(acc.x, sa, h[0].sb, h[0].bias), i8_scaled(acc.y, sa, h[1].sb, h[1].bias),
                       i8_scaled(acc.z, sa, h[2].sb, h[2].bias), i8_scaled(acc.w, sa, h[3].sb, h[3].bias)};
@@ -615,7 +614,7 @@ __global__ void __launch_bounds__(192, 2)
           if (GATED) z[e] = silu(z[e]) * __shfl_xor_sync(0xffffffffu, z[e], 4);
           else z[e] = relu_from(z[e], low);
         }
-        if (value) continue;
+        if (value) return;
         T *o = out + j * p.s_out;
         if (wide) {
           if (sizeof(T) == 2) {
@@ -630,6 +629,33 @@ __global__ void __launch_bounds__(192, 2)
           for (int e = 0; e < 4; ++e)
             if (cq + e < n_out) o[e] = from_f32<T>(z[e]);
         }
+      };
+      // two tokens' reads (of up to four CTAs) are under way before the first is added
+      const int step = 6 * (int)split;
+      for (int j = (int)rank + warp * (int)split; j < tokens; j += 2 * step) {
+        int4 acc[2] = {make_int4(0, 0, 0, 0), make_int4(0, 0, 0, 0)};
+        const bool second = j + step < tokens;
+        for (uint32_t r0 = 0; r0 < split; r0 += 4) {
+          int4 v[2][4];
+#pragma unroll
+          for (int i = 0; i < 2; ++i)
+#pragma unroll
+            for (uint32_t r = 0; r < 4; ++r)
+              v[i][r] = r0 + r < split && (i == 0 || second)
+                            ? ld_cluster_v4(mapa_shared(at + (uint32_t)((j + i * step) * kI8Rows * 4), r0 + r))
+                            : make_int4(0, 0, 0, 0);
+#pragma unroll
+          for (int i = 0; i < 2; ++i)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+              acc[i].x += v[i][r].x;
+              acc[i].y += v[i][r].y;
+              acc[i].z += v[i][r].z;
+              acc[i].w += v[i][r].w;
+            }
+        }
+        finish(j, acc[0]);
+        if (second) finish(j + step, acc[1]);
       }
     }
     __syncwarp();
@@ -722,6 +748,8 @@ static cudaError_t launch_i8_tc_t(I8TcPlan const &tp, CUtensorMap const &mc, CUt
     case 16: return launch_split<16, GATED, T>(tp, mc, mt, p, a, err, st);
     case 32: return launch_split<32, GATED, T>(tp, mc, mt, p, a, err, st);
     case 64: return launch_split<64, GATED, T>(tp, mc, mt, p, a, err, st);
+    case 80: return launch_split<80, GATED, T>(tp, mc, mt, p, a, err, st);
+    case 96: return launch_split<96, GATED, T>(tp, mc, mt, p, a, err, st);
     case 128: return launch_split<128, GATED, T>(tp, mc, mt, p, a, err, st);
     default: return cudaErrorInvalidValue;
   }

@@ -318,6 +318,13 @@ def test_contract_int8(cuda, m, n, k, act, out):
     contract_case(m, n, k, act, out)
 
 
+@pytest.mark.parametrize("act", ACTS)
+@pytest.mark.parametrize("m", [15, 31, 32, 63, 65, 79, 80, 81, 96, 97, 127])
+@pytest.mark.parametrize("n,k", [(200, 256), (262, 2100), (40000, 130)])
+def test_contract_int8_token_tiles(cuda, n, k, m, act):
+    contract_case(m, n, k, act, BF16)
+
+
 @pytest.mark.parametrize("m", [1, 3, 40, 300])
 @pytest.mark.parametrize("ld,offset", [(544, 0), (513, 0), (512, 1), (528, 16), (520, 8)])
 def test_contract_int8_strides_and_alignment(cuda, m, ld, offset):

@@ -126,19 +126,23 @@ int workspace_used(eir_plan *p, cudaStream_t st, int rc) {
   return rc != EIR_SUCCESS || e == cudaSuccess ? rc : eir::api_cuda_fail(e, "cudaEventRecord(workspace)");
 }
 
-// Tiling of an 8-bit contraction on the tensor cores. Pair tiles once there are
-// 32 of them (of the GPU's 74 CTA pairs), or 16 of a short K walk: one-CTA tiles
-// move twice the operand bytes (512 tokens x 4096 x 2048: 10.1 us against
-// 11.4). Else one-CTA tiles of just enough tokens, the K walk of each split over
-// a cluster, 4 K blocks a CTA at least (the exchange takes 1 to 3 us): the largest cluster of
-// which all tiles' clusters fit the GPU at once, two CTAs an SM (measured
-// limits; a second wave costs more than the split gains: 256 tokens x 4096 x
-// 4096, 64 tiles, take 14.4 us unsplit, 11.8 split by 4 and 21.7 split by 8).
+// Tiling of an 8-bit contraction on the tensor cores. Pair tiles where one-CTA
+// tiles would not all fit the GPU at once (two an SM), and from 32 of them (of the GPU's 74 CTA pairs)
+// on for a longer K walk, since one-CTA tiles move twice the operand bytes (512 tokens x 4096 x 2048:
+// 10.1 us against 11.3; 1024 x 4096 x 1024: 8.1 against 7.2). Else one-CTA tiles of just enough
+// tokens, the K walk of each split over a cluster. The split is the one with the least time by this
+// account, in tenths of a K block (0.25 us): the CTA's own K blocks, and for the exchange 45, half the
+// tile's tokens, and 6 to 10 a CTA (100 tokens x 4096: K = 1024 takes 5.7 us unsplit and 8.2 split by 4,
+// K = 4096 12.1 and 10.4, 10.8 split by 8). All tiles' clusters have to fit the GPU at once, two CTAs
+// an SM (measured limits; a second wave costs more than the split gains: 256 tokens x 4096 x 4096,
+// 64 tiles, take 14.4 us unsplit, 11.8 split by 4 and 21.7 split by 8).
 eir::I8TcPlan i8_tiling(eir::I8Params const &p) {
   eir::I8TcPlan t;
+  const int64_t blocks = (p.k + 127) / 128;
   t.c_tiles = (p.n + 255) / 256;  // gated: 128 gates and their values a tile
   t.t_tiles = (p.m + 255) / 256;
-  if (p.m > 128 && t.c_tiles * t.t_tiles >= (p.k <= 2048 ? 16 : 32)) return t;
+  const int64_t single = ((p.n + 127) / 128) * ((p.m + 127) / 128);
+  if (p.m > 128 && (single > 296 || (t.c_tiles * t.t_tiles >= 32 && blocks > 8))) return t;
   t.tokens = 128;
   for (int n : {96, 80, 64, 32, 16})
     if (p.m <= n) t.tokens = n;
@@ -146,9 +150,14 @@ eir::I8TcPlan i8_tiling(eir::I8Params const &p) {
   t.t_tiles = (p.m + t.tokens - 1) / t.tokens;
   struct {
     int split, tiles;
-  } const fits[] = {{8, 32}, {4, 66}, {3, 90}, {2, 148}};
+  } const fits[] = {{2, 148}, {3, 90}, {4, 66}, {8, 32}};
+  int64_t least = 10 * blocks;
   for (auto const &f : fits) {
-    if (t.split == 1 && t.c_tiles * t.t_tiles <= f.tiles && (p.k + 127) / 128 >= 4 * f.split) t.split = f.split;
+    const int64_t cost =
+        10 * ((blocks + f.split - 1) / f.split) + 45 + t.tokens / 2 + f.split * (6 + t.tokens / 32);
+    if (t.c_tiles * t.t_tiles > f.tiles || blocks < f.split || cost >= least) continue;
+    t.split = f.split;
+    least = cost;
   }
   return t;
 }

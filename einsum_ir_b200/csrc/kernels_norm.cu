@@ -16,6 +16,7 @@
 // the rows lie on the pieces' grid they load their next row before they reduce the present
 // one. Wider rows stay in shared memory, and rows too wide for that are read twice.
 #include <algorithm>
+#include <type_traits>
 #include "eir_launch.h"
 #include "eir_common.cuh"
 #include "op_params.h"
@@ -58,6 +59,7 @@ struct RingShape {
   int threads;  // that work on rows: whole warps
   int stages;
   int64_t stage_bytes;
+  int64_t more;  // bytes behind the stages
 };
 __host__ __device__ constexpr int64_t ring_slot(int64_t bytes) { return ((bytes + 15) / 16 + 4) * 16; }
 
@@ -524,6 +526,13 @@ struct NormBackRow {
   }
   // the factor of h in dx = g - h rstd^2 mean(g h) + dsum
   __device__ __forceinline__ float factor(float rstd, float gh) const { return rstd * rstd * (gh / (float)p.cols); }
+  // the elements inside the row of a piece that reaches outside it
+  __device__ __forceinline__ void give_some(int64_t row, int64_t c, float const (&held)[V], PieceH const &h, float k) const {
+    G *out = static_cast<G *>(a.dx) + row * p.s_dx;
+#pragma unroll
+    for (int e = 0; e < V; ++e)
+      if (c + e >= 0 && c + e < p.cols) out[c + e] = from_f32<G>(fmaf(h.get(e), -k, held[e]));
+  }
   // every lane of a warp calls it
   __device__ __forceinline__ void give(int64_t row, int64_t c, float const (&held)[V], PieceH const &h, float k) const {
     float d[V];
@@ -622,11 +631,19 @@ constexpr int kBackThreads = 512;  // of a block, at most
 // blocks an SM of that many threads, by a thread's elements
 __host__ __device__ constexpr int back_blocks(int per) { return per > 8 ? 1 : 2; }
 
-template <typename T, typename G, int N, bool GRID>
-__global__ void __launch_bounds__(kBackThreads + 32, back_blocks(N * NormBackRow<T, G, GRID>::V))
+// How a block's rows lie on the grid of 16-byte pieces: anyhow (pieces are shifted into place), on it, or
+// all tensors alike and by the same in every row of the block (the launch's grid is a multiple of the rows after which
+// it repeats): then the block's pieces lie on the grid of memory, and only a row's first and last one may be partial.
+// There the weight waits in shared memory, laid out like the pieces. (1237 x 2311 FP32: 19.1 us shifted, 14.0
+// alike, 12.4 for 2312 columns on the grid; 8192 x 4095 BF16: 103, 69 and 49.)
+enum RowsLie { kRowsAnyhow, kRowsOnGrid, kRowsAlike };
+
+template <typename T, typename G, int N, RowsLie LIE>
+__global__ void __launch_bounds__(kBackThreads + 32, back_blocks(N * NormBackRow<T, G, false>::V))
     norm_backward_ring_kernel(const NormParams p, const NormGradPtrs a, const RingShape ring, uint32_t *err) {
-  using Row = NormBackRow<T, G, GRID>;
+  using Row = NormBackRow<T, G, LIE != kRowsAnyhow>;
   constexpr int V = Row::V;
+  constexpr bool GRID = LIE == kRowsOnGrid, ALIKE = LIE == kRowsAlike;
   extern __shared__ __align__(128) uint8_t stages[];
   __shared__ uint32_t red[2][64];
   __shared__ RowRing<3> rr;
@@ -647,7 +664,28 @@ __global__ void __launch_bounds__(kBackThreads + 32, back_blocks(N * NormBackRow
   const Row op(p, a);
   const uint32_t slot_h = (uint32_t)ring_slot(p.cols * sizeof(T)), slot_g = (uint32_t)ring_slot(p.cols * sizeof(G));
   const float inv_cols = 1.f / (float)p.cols;
-  auto column = [&](int j) { return (j * ring.threads + (int)threadIdx.x) * V; };
+  const int lead = ALIKE ? (int)(rr.t[0].off(blockIdx.x) / sizeof(T)) : 0;
+  auto column = [&](int j) { return (j * ring.threads + (int)threadIdx.x) * V - lead; };
+  float *held_w = reinterpret_cast<float *>(stages + ring.stages * ring.stage_bytes);  // ALIKE: from column -lead on
+  if (ALIKE) {
+    const bool w_grid = lead == 0 && row_vec_ok(a.w, 0, 1, p.dt_w == EIR_FP32 ? 4 : 2, V);
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+      const int c = column(j);
+      float w[V];
+#pragma unroll
+      for (int e = 0; e < V; ++e) w[e] = 1.f;
+      if (a.w && w_grid && c < p.cols) {
+        load_shared_any<V>(a.w, p.dt_w, c, p.cols, true, w);
+      } else if (a.w) {
+#pragma unroll
+        for (int e = 0; e < V; ++e) w[e] = c + e >= 0 && c + e < p.cols ? ld_any(a.w, p.dt_w, c + e) : 0.f;
+      }
+#pragma unroll
+      for (int e = 0; e < V; e += 4)
+        *reinterpret_cast<float4 *>(held_w + c + lead + e) = make_float4(w[e], w[e + 1], w[e + 2], w[e + 3]);
+    }
+  }
   float dw[N][V];
 #pragma unroll
   for (int j = 0; j < N; ++j)
@@ -670,13 +708,26 @@ __global__ void __launch_bounds__(kBackThreads + 32, back_blocks(N * NormBackRow
     for (int j = 0; j < N; ++j) {
       const int c = column(j);
       typename Row::PieceG dy, s;
-      if (GRID && c >= p.cols) continue;
+      if ((GRID || ALIKE) && c >= p.cols) continue;
       float w[V];
-      op.weight(c, w);
-      if (GRID) {
-        h[j].template load<false>(at + c * (int)sizeof(T));
-        dy.template load<false>(dy_at + c * (int)sizeof(G));
-        if (a.dsum) s.template load<false>(sum_at + c * (int)sizeof(G));
+      if (ALIKE) {
+#pragma unroll
+        for (int e = 0; e < V; e += 4) {
+          const float4 q = *reinterpret_cast<float4 const *>(held_w + c + lead + e);
+          w[e] = q.x, w[e + 1] = q.y, w[e + 2] = q.z, w[e + 3] = q.w;
+        }
+      } else {
+        op.weight(c, w);
+      }
+      if (GRID || ALIKE) {
+        h[j].template load<false>(at + (c + lead) * (int)sizeof(T));
+        dy.template load<false>(dy_at + (c + lead) * (int)sizeof(G));
+        if (a.dsum) s.template load<false>(sum_at + (c + lead) * (int)sizeof(G));
+        if (ALIKE && (c < 0 || c + V > p.cols)) {  // bytes of other rows, or of none
+          h[j].clear_outside(c, (int)p.cols);
+          dy.clear_outside(c, (int)p.cols);
+          if (a.dsum) s.clear_outside(c, (int)p.cols);
+        }
       } else {
         h[j].load_slot(at, off_h, c, p.cols);
         dy.load_slot(dy_at, off_d, c, p.cols);
@@ -699,7 +750,11 @@ __global__ void __launch_bounds__(kBackThreads + 32, back_blocks(N * NormBackRow
     gh = warp_sum(lane < warps ? __uint_as_float(red[turn][lane]) : 0.f);
     const float k = unit * unit * (gh * inv_cols);
 #pragma unroll
-    for (int j = 0; j < N; ++j) op.give(row, column(j), held[j], h[j], k);
+    for (int j = 0; j < N; ++j) {
+      const int c = column(j);
+      if (ALIKE && (c < 0 || c + V > p.cols)) op.give_some(row, c, held[j], h[j], k);
+      else op.give(row, c, held[j], h[j], k);
+    }
     if (++stage == ring.stages) {
       stage = 0;
       phase ^= 1u;
@@ -707,8 +762,17 @@ __global__ void __launch_bounds__(kBackThreads + 32, back_blocks(N * NormBackRow
   }
   if (a.part != nullptr) {
     float *part = a.part + (int64_t)blockIdx.x * norm_part_pitch(p.cols);
+    if (ALIKE && lead != 0) {  // through the weight's place, into whole lines
 #pragma unroll
-    for (int j = 0; j < N; ++j) put_part<V>(part, column(j), p.cols, dw[j]);
+      for (int j = 0; j < N; ++j)
+#pragma unroll
+        for (int e = 0; e < V; ++e) held_w[column(j) + lead + e] = dw[j][e];
+      ring_sync(ring.threads);
+      for (int c = threadIdx.x; c < p.cols; c += ring.threads) part[c] = held_w[c + lead];
+    } else {
+#pragma unroll
+      for (int j = 0; j < N; ++j) put_part<V>(part, column(j), p.cols, dw[j]);
+    }
   }
 }
 
@@ -881,12 +945,13 @@ static cudaError_t launch_wide(void (*kern)(KArgs...), WideGrid const &g, cudaSt
   return launch_kernel(kern, dim3((unsigned)g.grid), dim3(g.threads), (size_t)g.bytes, st, args...);
 }
 
-// stages of a ring for `blocks` blocks an SM at most (fewer where two stages a block do not
+// stages of a ring for `blocks` blocks an SM at most, `more` bytes behind them (fewer where two stages a block do not
 // fit otherwise); 0 stages: too wide
-static int64_t ring_fit(int64_t stage_bytes, int64_t blocks, RingShape *r) {
+static int64_t ring_fit(int64_t stage_bytes, int64_t blocks, RingShape *r, int64_t more = 0) {
   r->stage_bytes = stage_bytes;
-  while (blocks > 1 && (2 * stage_bytes + 2048) * blocks > kSmemMost) --blocks;
-  r->stages = (int)std::min<int64_t>(kMostStages, (kSmemMost / blocks - 2048) / stage_bytes);
+  r->more = more;
+  while (blocks > 1 && (2 * stage_bytes + more + 2048) * blocks > kSmemMost) --blocks;
+  r->stages = (int)std::min<int64_t>(kMostStages, (kSmemMost / blocks - 2048 - more) / stage_bytes);
   if (r->stages < 2) r->stages = 0;
   return blocks;
 }
@@ -894,7 +959,7 @@ static int64_t ring_fit(int64_t stage_bytes, int64_t blocks, RingShape *r) {
 template <typename... KArgs, typename... Args>
 static cudaError_t launch_ring(void (*kern)(KArgs...), RingShape const &r, int64_t grid, cudaStream_t st,
                                Args const &...args) {
-  const size_t bytes = (size_t)(r.stages * r.stage_bytes);
+  const size_t bytes = (size_t)(r.stages * r.stage_bytes + r.more);
   cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
   if (e != cudaSuccess) return e;
   return launch_kernel(kern, dim3((unsigned)grid), dim3(r.threads + 32), bytes, st, args...);
@@ -981,22 +1046,40 @@ static cudaError_t launch_norm_backward_t(NormParams const &p, NormGradPtrs cons
     auto kern = grid ? norm_backward_kernel<T, G, true> : norm_backward_kernel<T, G, false>;
     return launch_kernel(kern, dim3((unsigned)*parts), dim3(kBackWarps * 32), (size_t)(kBackWarps * 4 * p.cols), st, p, a);
   }
-  const int per = back_per(p.cols);
-  RingShape r;
-  const int64_t most = back_ring_blocks(p.cols, &r.threads);
-  if (most > 0) {
+  // all rows of a block alike: the same offset of a row's tensors, whose strides step alike
+  auto same = [&](void const *q, int64_t stride) {
+    return q == nullptr || ((reinterpret_cast<uintptr_t>(q) - reinterpret_cast<uintptr_t>(a.h)) % 16 == 0 &&
+                            (p.rows == 1 || (stride - p.s_h) * (int64_t)sizeof(T) % 16 == 0));
+  };
+  const bool could = std::is_same<T, G>::value && same(a.dy, p.s_dy) && same(a.dsum, p.s_dsum) && same(a.dx, p.s_dx);
+  for (bool alike : {true, false}) {  // (with the weight in shared memory a ring may be too wide)
+    if (alike && !could) continue;
+    const int64_t cols = p.cols + (alike && !grid ? V - 1 : 0);  // that the pieces cover
+    const int per = back_per(cols);
+    RingShape r;
+    const int64_t most = back_ring_blocks(cols, &r.threads);
+    if (most == 0) continue;
     const int64_t bytes = ring_slot(p.cols * sizeof(T)) + ring_slot(p.cols * sizeof(G)) * (a.dsum ? 2 : 1);
-    const int64_t blocks = ring_fit(bytes, most, &r);
-    if (r.stages > 0) {
-      *parts = std::min<int64_t>(p.rows, num_sms * blocks);
-      auto kern = grid ? (per == 8    ? norm_backward_ring_kernel<T, G, 8 / V, true>
-                          : per == 16 ? norm_backward_ring_kernel<T, G, 16 / V, true>
-                                      : norm_backward_ring_kernel<T, G, 32 / V, true>)
-                       : (per == 8    ? norm_backward_ring_kernel<T, G, 8 / V, false>
-                          : per == 16 ? norm_backward_ring_kernel<T, G, 16 / V, false>
-                                      : norm_backward_ring_kernel<T, G, 32 / V, false>);
-      return launch_ring(kern, r, *parts, st, p, a, r, err);
+    const int64_t blocks = ring_fit(bytes, most, &r, alike ? (int64_t)r.threads * per * 4 : 0);
+    if (r.stages == 0) continue;
+    *parts = std::min<int64_t>(p.rows, num_sms * blocks);
+    // rows on the grid read the weight where it is unless a block has several of them (8192 x 4096
+    // BF16: 52.2 us so, 49.2 from shared memory; 2048 x 1024: 9.8 and 11.2)
+    if (alike && grid && p.rows < 4 * *parts) continue;
+    constexpr int kPeriod = 16 / (int)sizeof(T);
+    if (alike && !grid && *parts < p.rows) *parts = *parts / kPeriod * kPeriod;
+    auto pick = [&](auto lie) {
+      constexpr RowsLie L = decltype(lie)::value;
+      return per == 8    ? norm_backward_ring_kernel<T, G, 8 / V, L>
+             : per == 16 ? norm_backward_ring_kernel<T, G, 16 / V, L>
+                         : norm_backward_ring_kernel<T, G, 32 / V, L>;
+    };
+    auto kern = grid ? pick(std::integral_constant<RowsLie, kRowsOnGrid>{})
+                     : pick(std::integral_constant<RowsLie, kRowsAnyhow>{});
+    if constexpr (std::is_same<T, G>::value) {
+      if (alike) kern = pick(std::integral_constant<RowsLie, kRowsAlike>{});
     }
+    return launch_ring(kern, r, *parts, st, p, a, r, err);
   }
   const WideGrid g = wide_grid(p.rows, p.cols, 512, V, sizeof(T) + 8, num_sms);
   *parts = g.grid;

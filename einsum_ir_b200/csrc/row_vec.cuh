@@ -135,6 +135,16 @@ struct RowPiece {
     }
   }
 
+  // zeros in place of the elements outside columns 0 .. cols - 1 of a piece at column c
+  __device__ __forceinline__ void clear_outside(int c, int cols) {
+#pragma unroll
+    for (int e = 0; e < V; ++e) {
+      if (c + e >= 0 && c + e < cols) continue;
+      if constexpr (sizeof(T) == 4) w[e] = 0;
+      else w[e / 2] &= e % 2 ? 0x0000ffffu : 0xffff0000u;
+    }
+  }
+
   // elements first .. last - 1 of the piece, one by one
   __device__ __forceinline__ void store_some(T *p, int first, int last) const {
 #pragma unroll

@@ -635,7 +635,7 @@ __host__ __device__ constexpr int back_blocks(int per) { return per > 8 ? 1 : 2;
 // all tensors alike and by the same in every row of the block (the launch's grid is a multiple of the rows after which
 // it repeats): then the block's pieces lie on the grid of memory, and only a row's first and last one may be partial.
 // There the weight waits in shared memory, laid out like the pieces. (1237 x 2311 FP32: 19.1 us shifted, 14.0
-// alike, 12.4 for 2312 columns on the grid; 8192 x 4095 BF16: 103, 69 and 49.)
+// alike, 12.4 for 2312 columns on the grid; 8192 x 4095 BF16: 103, 49 and 45.)
 enum RowsLie { kRowsAnyhow, kRowsOnGrid, kRowsAlike };
 
 template <typename T, typename G, int N, RowsLie LIE>
@@ -1017,18 +1017,26 @@ cudaError_t launch_quantize(QuantizeParams const &p, void const *x, int8_t *q, f
                           : launch_norm_out<__nv_bfloat16, int8_t, true>(n, a, err, num_sms, st);
 }
 
-// elements of a thread: 8, 16 or 32
-static int back_per(int64_t cols) { return cols <= kBackThreads * 8 ? 8 : cols <= kBackThreads * 16 ? 16 : 32; }
-// blocks an SM of the backward ring, if their stages fit
-static int64_t back_ring_blocks(int64_t cols, int *threads) {
-  const int per = back_per(cols);
+// Elements of a thread of the backward ring: 8, 16 or 32. Few threads with much to do each make a row's barriers
+// cheap where many rows follow one another, more threads make few rows quick (8192 x 4096 BF16: 45.0 us
+// with 16 elements, 49.2 with 8; 8192 x 2048: 26.0 and 29.5; 1237 x 2312 FP32: 14.8 and 12.1).
+static int back_per(int64_t rows, int64_t cols, int num_sms) {
+  const int least = rows >= 32 * (int64_t)num_sms ? 16 : 8;
+  return cols <= kBackThreads * least ? least : cols <= kBackThreads * 16 ? 16 : 32;
+}
+// blocks an SM, if their stages fit, by the registers of a thread; 0: too wide
+static int64_t back_ring_blocks(int64_t cols, int per, int *threads) {
   *threads = (int)((cols + per - 1) / per + 31) / 32 * 32;
-  return *threads > kBackThreads ? 0 : std::min(8, back_blocks(per) * (kBackThreads + 32) / (*threads + 32));
+  const int on_sm = per == 8 ? 2 * (kBackThreads + 32) : per == 16 ? 640 : kBackThreads + 32;
+  return *threads > kBackThreads ? 0 : std::min(8, on_sm / (*threads + 32));
 }
 
 int64_t norm_backward_parts(NormParams const &p, int num_sms) {
-  int threads = 0;  // (narrow rows and wide ones: 2 blocks an SM)
-  const int64_t an_sm = p.cols <= 32 * kPerBack ? 2 : std::max<int64_t>(2, back_ring_blocks(p.cols, &threads));
+  int threads = 0;
+  int64_t an_sm = 2;  // narrow rows and wide ones
+  if (p.cols > 32 * kPerBack) {
+    for (int per : {8, 16, 32}) an_sm = std::max(an_sm, back_ring_blocks(p.cols, per, &threads));
+  }
   return std::min<int64_t>(p.rows, num_sms * an_sm);
 }
 
@@ -1055,16 +1063,16 @@ static cudaError_t launch_norm_backward_t(NormParams const &p, NormGradPtrs cons
   for (bool alike : {true, false}) {  // (with the weight in shared memory a ring may be too wide)
     if (alike && !could) continue;
     const int64_t cols = p.cols + (alike && !grid ? V - 1 : 0);  // that the pieces cover
-    const int per = back_per(cols);
+    const int per = back_per(p.rows, cols, num_sms);
     RingShape r;
-    const int64_t most = back_ring_blocks(cols, &r.threads);
+    const int64_t most = back_ring_blocks(cols, per, &r.threads);
     if (most == 0) continue;
     const int64_t bytes = ring_slot(p.cols * sizeof(T)) + ring_slot(p.cols * sizeof(G)) * (a.dsum ? 2 : 1);
     const int64_t blocks = ring_fit(bytes, most, &r, alike ? (int64_t)r.threads * per * 4 : 0);
     if (r.stages == 0) continue;
     *parts = std::min<int64_t>(p.rows, num_sms * blocks);
     // rows on the grid read the weight where it is unless a block has several of them (8192 x 4096
-    // BF16: 52.2 us so, 49.2 from shared memory; 2048 x 1024: 9.8 and 11.2)
+    // BF16, 8 elements a thread: 52.2 us so, 49.2 from shared memory; 2048 x 1024: 9.8 and 11.2)
     if (alike && grid && p.rows < 4 * *parts) continue;
     constexpr int kPeriod = 16 / (int)sizeof(T);
     if (alike && !grid && *parts < p.rows) *parts = *parts / kPeriod * kPeriod;

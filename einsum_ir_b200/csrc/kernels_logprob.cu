@@ -3,10 +3,12 @@
 //
 // One pass over a row, in base 2 (L = log2 e): with a reference R near the row's
 // maximum times L, S = sum 2^d and U = sum d 2^d for d = x L - R give
-// lse = (R + log2 S) / L, log p = (d - log2 S) / L and entropy = (log2 S - U / S) / L. Any R will do, so
-// rounding it costs nothing; a thread raises its own when it meets a larger logit and its
-// sums shrink by 2^(R - R'). Logits are floored at -1e37, where 2^d is 0, so that
-// a ruled-out one (-infinity) adds 0 d = 0 to U.
+// lse = (R + log2 S) / L, log p = (d - log2 S) / L and entropy = (log2 S - U / S) / L. Any R near m L will
+// do, so that R may be rounded: by 2^-4 at most for |m| <= 2^20, and rows whose maximum is larger or
+// lower than that are redone (from 1.5e9 on the rounding alone could take 2^d out of FP32's range). A
+// thread raises its own R when it meets a larger logit and its sums shrink by 2^(R - R'). Logits are
+// floored at -2^21, where 2^d is 0 for every such m, so that a ruled-out one (-infinity, or a large finite
+// value) adds 0 d = 0 to U.
 //
 // At BF16 bound by the SM's pipes (4096 x 32768: 53 us, 5.1 TB/s; exponentials 63 % of their
 // rate, issue 62 %), at FP32 by HBM (4096 x 32768, 5 alternatives: 105 us, 5.1 TB/s). A logit is read once. A piece is 16 bytes of memory on
@@ -26,8 +28,8 @@
 // Rows that do not fill the GPU by number are split over a cluster of up to 8 blocks, joined
 // through distributed shared memory.
 //
-// Rows with a NaN or +infinity, with nothing above -1e37, or with more candidates
-// than their buffer holds are redone by logprob_plain_row: a pass for each value.
+// Rows with a NaN or +infinity, with a maximum above 2^20 or below -2^20 (but -infinity), or with more
+// candidates than their buffer holds are redone by logprob_plain_row: a pass for each value.
 //
 // Backward: dx = dlogprob (onehot - p) - dentropy p (x - lse + H), bound by HBM (2048 x 50021 BF16 with
 // entropy 73 us, 5.6 TB/s).
@@ -40,7 +42,8 @@
 namespace eir {
 
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
-constexpr float kLowest = -1e37f;  // logits below count as ruled out in the fast pass
+constexpr float kLowest = -2097152.f;  // -2^21: logits below count as ruled out in the fast pass,
+constexpr float kLargest = 1048576.f;  // 2^20: whose sums hold where the row's maximum is no larger than this
 
 __device__ __forceinline__ float exp2_fast(float x) {
   float r;
@@ -75,9 +78,13 @@ struct LogSums {
   float m, S, U;
 };
 __device__ __forceinline__ float log_ref(float m) { return m < kLowest ? 0.f : m * kLog2e; }
-// log p of a logit (one below kLowest may leave FP32's range in base 2)
+// log p of a logit: its distance from the maximum, whose own d is the rounding of R
 __device__ __forceinline__ float log_prob(float x, LogSums const &v, float log_s) {
-  return x < kLowest ? x - v.m : (fmaf(x, kLog2e, -log_ref(v.m)) - log_s) * kLn2;
+  return (x - v.m) + (fmaf(v.m, kLog2e, -log_ref(v.m)) - log_s) * kLn2;
+}
+// whether a row's sums do not hold (S is NaN where the row has a NaN or +infinity)
+__device__ __forceinline__ bool log_odd(LogSums const &v) {
+  return !(v.S == v.S) || v.m > kLargest || (v.m < -kLargest && v.m != -INFINITY);
 }
 // sums against R moved to the reference of the maximum m (sums of 0 may stand beside any reference)
 __device__ __forceinline__ LogSums log_moved(float R, float S, float U, float m) {
@@ -271,7 +278,7 @@ struct LogShared {
   uint64_t plain[32];      // the plain row's words
   uint64_t top[32];        // the block's alternatives
   uint64_t found[kCandidates];
-  int n_found, odd;
+  int n_found, full_up;    // candidates; more than fit
   volatile int abort;      // a bounded wait has given up
   LogSums sums;            // of the block
   alignas(8) uint64_t full[THREADS / 32][kLogStages];
@@ -495,10 +502,10 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS)
       __syncwarp();
     }
   }
-  // (S is NaN where the row holds a NaN or +infinity)
-  bool odd = full || !(v.S == v.S) || v.m > 1e37f || (v.m < kLowest && v.m != -INFINITY);
+  bool odd = full || log_odd(v);
   if (blocks_a_row > 1) {
-    if (threadIdx.x == 0) sh.odd = odd;
+    // (whether the sums hold shows in the whole row's: a part may well have nothing but masked logits)
+    if (threadIdx.x == 0) sh.full_up = full;
     __syncwarp();
     cluster_sync();  // every block's sums and alternatives are in its shared memory
     if (rank == 0) {
@@ -509,12 +516,10 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS)
         const uint32_t sums = mapa_shared(smem_u32(&sh.sums), lane);
         w = LogSums{__uint_as_float(ld_cluster_u32(sums)), __uint_as_float(ld_cluster_u32(sums + 4)),
                     __uint_as_float(ld_cluster_u32(sums + 8))};
-        any = (int)ld_cluster_u32(mapa_shared(smem_u32(&sh.odd), lane));
+        any = (int)ld_cluster_u32(mapa_shared(smem_u32(&sh.full_up), lane));
       }
       v = log_join_lanes(w);
-      // a part that is odd by itself (nothing above kLowest) need not be so in the whole row
-      odd = !(v.S == v.S) || v.m > 1e37f || (v.m < kLowest && v.m != -INFINITY);
-      if (p.top > 0) odd = odd || __any_sync(0xffffffffu, any != 0);
+      odd = log_odd(v) || __any_sync(0xffffffffu, any != 0);
       if (p.top > 0 && !odd && warp == 0) {
         for (int i = lane; i < p.top * (int)blocks_a_row; i += 32) {
           const uint32_t key = mapa_shared(smem_u32(&sh.top[i % p.top]), i / p.top);

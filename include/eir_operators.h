@@ -108,7 +108,8 @@ int eir_contract_int8(eir_plan *plan, void const *left, void const *right, float
  * index. Logits of -infinity have probability 0 and add 0 to the entropy; a
  * row with nothing but -infinity gives lse = -infinity, logprob = -infinity
  * (top_logprob alike) and entropy 0; a NaN or +infinity makes the row's
- * values NaN. A negative target is ignored (logprob 0); one >= vocab gives
+ * values NaN. Finite logits may have any size (a row whose largest is beyond
+ * 2^20 in magnitude takes a slower way), as masks too. A negative target is ignored (logprob 0); one >= vocab gives
  * NaN. */
 typedef struct {
   int64_t rows, vocab;        /* 1 <= vocab < 2^31 */
@@ -127,7 +128,8 @@ int eir_logprob(eir_plan *plan, void const *logits, int64_t const *targets, floa
  * both or neither (neither: that term is 0); dentropy may be NULL (entropy is
  * read only with it); dlogits may be logits itself (same pointer and stride).
  * An ignored target takes no part; one >= vocab makes the row NaN; a row of
- * nothing but -infinity gets zeros. The alternatives carry no gradient. */
+ * nothing but -infinity gets zeros. p is exp(x - lse) of the lse given, which
+ * FP32 holds to 2^-24 of its size. The alternatives carry no gradient. */
 int eir_logprob_backward(eir_plan *plan, void const *logits, int64_t const *targets,
                          float const *lse, float const *entropy, float const *dlogprob,
                          float const *dentropy, void *dlogits, void *stream);

@@ -8,6 +8,7 @@
 
 #include <cuda_runtime.h>
 #include <cstdlib>
+#include <mutex>
 
 namespace eir {
 
@@ -33,6 +34,31 @@ cudaError_t launch_kernel(void (*kern)(KArgs...), dim3 grid, dim3 block, size_t 
   cfg.attrs = attr;
   cfg.numAttrs = pdl_enabled() ? 1 : 0;
   return cudaLaunchKernelEx(&cfg, kern, args...);
+}
+
+// Allows a kernel all the dynamic shared memory that its static words leave of a block's 227 KB, on the current
+// device. The limit belongs to the kernel, not to a call: one that set it to its own size could lower it between
+// another host thread's setting and launch, which is refused then. So it is set once, to the same value by all.
+inline cudaError_t allow_all_smem(void const *kern) {
+  struct Done {
+    void const *kern;
+    int dev;
+  };
+  static std::mutex mu;
+  static Done done[1024];
+  static int n = 0;  // (beyond the table's end a kernel's limit is set on every call)
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return e;
+  std::lock_guard<std::mutex> lk(mu);
+  for (int i = 0; i < n; ++i)
+    if (done[i].kern == kern && done[i].dev == dev) return cudaSuccess;
+  cudaFuncAttributes fa;
+  e = cudaFuncGetAttributes(&fa, kern);
+  if (e != cudaSuccess) return e;
+  e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024 - (int)fa.sharedSizeBytes);
+  if (e == cudaSuccess && n < 1024) done[n++] = Done{kern, dev};
+  return e;
 }
 
 }  // namespace eir

@@ -28,6 +28,7 @@
 // gives up raises the CTA's (or pair's) abort flag and records a device error.
 #include <cuda.h>
 #include <algorithm>
+#include <atomic>
 #include "eir_launch.h"
 #include "i8_common.cuh"
 
@@ -674,30 +675,18 @@ __global__ void __launch_bounds__(192, 2)
 
 // ---------------------------------------------------------------- launchers
 
-template <typename Kern>
-static cudaError_t i8_allow_smem(Kern kern, int bytes, bool (&done)[32]) {
-  int dev = 0;
-  cudaError_t e = cudaGetDevice(&dev);
-  if (e != cudaSuccess) return e;
-  if (dev < 32 && done[dev]) return cudaSuccess;
-  e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
-  if (e == cudaSuccess && dev < 32) done[dev] = true;
-  return e;
-}
-
 template <bool GATED, typename T>
 static cudaError_t launch_pair(I8TcPlan const &tp, CUtensorMap const &mc, CUtensorMap const &mt, I8Params const &p,
                                I8Ptrs const &a, uint32_t *err, cudaStream_t st) {
   using Cfg = I8Pair;
   auto kern = i8_pair_kernel<GATED, T>;
-  static bool done[32] = {};
-  cudaError_t e = i8_allow_smem(kern, Cfg::kSmemBytes, done);
+  cudaError_t e = allow_all_smem(reinterpret_cast<void const *>(kern));
   if (e != cudaSuccess) return e;
-  static int clusters[32] = {};  // per device: pairs that can run at once
+  static std::atomic<int> clusters[32] = {};  // per device: pairs that can run at once
   int dev = 0;
   e = cudaGetDevice(&dev);
   if (e != cudaSuccess) return e;
-  int most = dev < 32 ? clusters[dev] : 0;
+  int most = dev < 32 ? clusters[dev].load() : 0;
   if (most == 0) {
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(2);
@@ -718,8 +707,7 @@ static cudaError_t launch_split(I8TcPlan const &tp, CUtensorMap const &mc, CUten
                                 I8Ptrs const &a, uint32_t *err, cudaStream_t st) {
   using Cfg = I8Split<NT>;
   auto kern = i8_split_kernel<NT, GATED, T>;
-  static bool done[32] = {};
-  cudaError_t e = i8_allow_smem(kern, Cfg::kSmemBytes, done);
+  cudaError_t e = allow_all_smem(reinterpret_cast<void const *>(kern));
   if (e != cudaSuccess) return e;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(tp.c_tiles * tp.t_tiles * tp.split));

@@ -941,7 +941,7 @@ static WideGrid wide_grid(int64_t rows, int64_t cols, int threads, int v, int pe
 template <typename... KArgs, typename... Args>
 static cudaError_t launch_wide(void (*kern)(KArgs...), WideGrid const &g, cudaStream_t st, Args const &...args) {
   if (g.bytes > 48 * 1024 - 1024) {
-    cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)g.bytes);
+    cudaError_t e = allow_all_smem(reinterpret_cast<void const *>(kern));
     if (e != cudaSuccess) return e;
   }
   return launch_kernel(kern, dim3((unsigned)g.grid), dim3(g.threads), (size_t)g.bytes, st, args...);
@@ -962,7 +962,7 @@ template <typename... KArgs, typename... Args>
 static cudaError_t launch_ring(void (*kern)(KArgs...), RingShape const &r, int64_t grid, cudaStream_t st,
                                Args const &...args) {
   const size_t bytes = (size_t)(r.stages * r.stage_bytes + r.more);
-  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
+  cudaError_t e = allow_all_smem(reinterpret_cast<void const *>(kern));
   if (e != cudaSuccess) return e;
   return launch_kernel(kern, dim3((unsigned)grid), dim3(r.threads + 32), bytes, st, args...);
 }

@@ -96,9 +96,21 @@ int encode_map(eir::MapSpec const &s, void const *ptr, CUtensorMap *m) {
   int rc = get_encoder();
   if (rc != EIR_SUCCESS) return rc;
   uint32_t estr[5] = {1, 1, 1, 1, 1};
-  CUresult r = g_encode(m, s.dtype, s.rank, const_cast<void *>(ptr), s.dims, s.strides_bytes, s.box,
-                        estr, CU_TENSOR_MAP_INTERLEAVE_NONE, s.swizzle,
-                        CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  auto encode = [&]() {
+    return g_encode(m, s.dtype, s.rank, const_cast<void *>(ptr), s.dims, s.strides_bytes, s.box, estr,
+                    CU_TENSOR_MAP_INTERLEAVE_NONE, s.swizzle, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                    CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  };
+  CUresult r = encode();
+  if (r == CUDA_ERROR_INVALID_CONTEXT) {
+    // a host thread's first call: the driver's entry point, unlike the runtime's, does not make the
+    // device's context current by itself
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e == cudaSuccess) e = cudaSetDevice(dev);
+    if (e != cudaSuccess) return cuda_fail(e, "cudaSetDevice");
+    r = encode();
+  }
   if (r != CUDA_SUCCESS)
     return set_error(EIR_CUDA_ERROR, "cuTensorMapEncodeTiled failed (" + std::to_string((int)r) + ")");
   return EIR_SUCCESS;

@@ -1,4 +1,4 @@
-"""Plans of the row operators in several host threads at once."""
+"""Plans of the row operators and the contractions in several host threads at once, and in new ones."""
 from __future__ import annotations
 
 import threading
@@ -6,9 +6,9 @@ import threading
 import pytest
 import torch
 
-from einsum_ir_b200 import cabi, operators as op
-from tests._operators import quantized32
-from tests.test_gpu_operators import CODE, F32, gen, rows_of
+from einsum_ir_b200 import binary, cabi, operators as op
+from tests._operators import contract64, quantized32
+from tests.test_gpu_operators import CODE, F32, codes, gen, rows_of
 
 pytestmark = pytest.mark.gpu
 
@@ -62,5 +62,37 @@ def quantize_work(g, rows, cols, dtype, offset):
 def test_plans_of_several_widths(cuda, make):
     works = make(gen(3))
     in_threads([w for w, _ in works], 2000)
+    for _, right in works:
+        assert right()
+
+
+def contract_work(g, m, n, k):
+    a, b = codes(g, m, k), codes(g, n, k)
+    y = torch.empty((m, n), device="cuda")
+    plan = op.Int8ContractPlan(m, n, k, dtype_out=cabi.FP32)
+    want = contract64(a, b, None, None, None, 0).float()
+    return (lambda stream: plan.contract(a, b, None, None, y, stream=stream)), lambda: torch.equal(y, want)
+
+
+def bf16_work(g, m, n, k):
+    # small whole numbers: the FP32 sums are exact
+    a, b = (torch.randint(-8, 9, s, generator=g, device="cuda").bfloat16() for s in ((m, k), (n, k)))
+    y = torch.empty((m, n), device="cuda")
+    il, ir, io, names = binary.parse_binary("mk,nk->mn")
+    sizes = {i: dict(m=m, n=n, k=k)[c] for i, c in enumerate(names)}
+    plan = cabi.ContractPlan(binary.contraction_dims(il, ir, io, sizes), cabi.BF16, cabi.BF16, cabi.FP32)
+    assert plan.family == cabi.FAMILY_TC
+    want = (a.float() @ b.float().T)
+    return (lambda stream: plan.contract(a, b, y, stream=stream)), lambda: torch.equal(y, want)
+
+
+@pytest.mark.parametrize("make", [
+    lambda g: [contract_work(g, 40, 512, 1024), contract_work(g, 300, 512, 1024), contract_work(g, 60, 512, 1000)],
+    lambda g: [bf16_work(g, 1024, 1024, 512)],
+])
+def test_first_call_of_a_host_thread(cuda, make):
+    """contractions that set up tensor maps before anything has made the context current in the thread"""
+    works = make(gen(4))
+    in_threads([w for w, _ in works], 200)
     for _, right in works:
         assert right()

@@ -830,20 +830,6 @@ int api_set_error(int code, char const *msg) { return set_error(code, msg); }
 int api_cuda_fail(cudaError_t e, char const *where) { return cuda_fail(e, where); }
 int api_encode_map(MapSpec const &s, void const *ptr, CUtensorMap *m) { return encode_map(s, ptr, m); }
 void api_count_launch() { g_launches.fetch_add(1, std::memory_order_relaxed); }
-void api_free_workspace(eir_plan *p) {
-  if (p->ws) {
-    int cur = 0;
-    cudaGetDevice(&cur);
-    if (p->ws_device >= 0 && p->ws_device != cur) cudaSetDevice(p->ws_device);
-    // cudaFree of pool memory does not wait for its use
-    if (p->ws_used) cudaEventSynchronize(p->ws_used);
-    cudaFree(p->ws);
-    if (p->ws_device >= 0 && p->ws_device != cur) cudaSetDevice(cur);
-  }
-  if (p->ws_used) cudaEventDestroy(p->ws_used);
-  p->ws = nullptr;
-  p->ws_used = nullptr;
-}
 int api_device(int *num_sms, uint32_t **err) {
   DeviceState *ds = nullptr;
   int rc = device_state(&ds);
@@ -1573,7 +1559,14 @@ int eir_plan_destroy(eir_plan *p) {
   if (p->pre_r) eir_plan_destroy(p->pre_r);
   if (p->cpx_inner) eir_plan_destroy(p->cpx_inner);
   release_gather(p);
-  eir::api_free_workspace(p);
+  if (p->ws) {
+    int cur = 0;
+    cudaGetDevice(&cur);
+    if (p->ws_device >= 0 && p->ws_device != cur) cudaSetDevice(p->ws_device);
+    cudaFree(p->ws);
+    if (p->ws_device >= 0 && p->ws_device != cur) cudaSetDevice(cur);
+  }
+  p->op_ws.release();
   delete p;
   return EIR_SUCCESS;
 }

@@ -1,7 +1,6 @@
 // C-ABI of the row operators and the 8-bit contraction (eir_operators.h):
 // argument checks, workspaces and launches.
 #include <algorithm>
-#include <mutex>
 #include <new>
 #include <string>
 #include "eir_operators.h"
@@ -46,84 +45,6 @@ int make_plan(eir_plan **out, int what, int family, Fill fill) {
   }
   *out = p;
   return EIR_SUCCESS;
-}
-
-// The workspaces' memory comes from a pool of the library's own per device, so
-// that a plan made for a new shape does not pay for cudaMalloc on its first call
-// (0.5 ms and more; it synchronises the device too). Up to 256 MiB stay with the
-// pool when plans are destroyed.
-int workspace_pool(int dev, cudaMemPool_t *pool) {
-  static std::mutex mu;
-  static cudaMemPool_t pools[64] = {};
-  if (dev < 0 || dev >= 64) return fail(EIR_CUDA_ERROR, "device index out of range");
-  std::lock_guard<std::mutex> lk(mu);
-  if (pools[dev] == nullptr) {
-    cudaMemPoolProps props = {};
-    props.allocType = cudaMemAllocationTypePinned;
-    props.location.type = cudaMemLocationTypeDevice;
-    props.location.id = dev;
-    cudaMemPool_t made = nullptr;
-    cudaError_t e = cudaMemPoolCreate(&made, &props);
-    if (e != cudaSuccess) return eir::api_cuda_fail(e, "cudaMemPoolCreate");
-    uint64_t keep = (uint64_t)256 << 20;
-    e = cudaMemPoolSetAttribute(made, cudaMemPoolAttrReleaseThreshold, &keep);
-    if (e != cudaSuccess) {
-      cudaMemPoolDestroy(made);
-      return eir::api_cuda_fail(e, "cudaMemPoolSetAttribute");
-    }
-    pools[dev] = made;
-  }
-  *pool = pools[dev];
-  return EIR_SUCCESS;
-}
-
-// The plan's own workspace on the current device, allocated on first use in
-// `st`'s order; on another stream than the last use's it waits for that. A capture
-// gets the workspace that is there: memory allocated in it would be the graph's own, and an
-// event from outside cannot be waited for (the caller orders a graph's launches).
-int workspace(eir_plan *p, cudaStream_t st, void **ws) {
-  int dev = 0;
-  cudaError_t e = cudaGetDevice(&dev);
-  if (e != cudaSuccess) return eir::api_cuda_fail(e, "cudaGetDevice");
-  cudaStreamCaptureStatus cap = cudaStreamCaptureStatusNone;
-  e = cudaStreamIsCapturing(st, &cap);
-  if (e != cudaSuccess) return eir::api_cuda_fail(e, "cudaStreamIsCapturing");
-  const bool captured = cap != cudaStreamCaptureStatusNone;
-  if (p->ws == nullptr || p->ws_device != dev) {
-    if (captured) return bad_argument("a plan with a workspace needs a call on the device before it is captured");
-    eir::api_free_workspace(p);
-    cudaMemPool_t pool = nullptr;
-    int rc = workspace_pool(dev, &pool);
-    if (rc != EIR_SUCCESS) return rc;
-    e = cudaEventCreateWithFlags(&p->ws_used, cudaEventDisableTiming);
-    if (e != cudaSuccess) return eir::api_cuda_fail(e, "cudaEventCreate(workspace)");
-    e = cudaMallocFromPoolAsync(&p->ws, (size_t)p->ws_bytes, pool, st);
-    if (e != cudaSuccess) {
-      p->ws = nullptr;
-      cudaEventDestroy(p->ws_used);
-      p->ws_used = nullptr;
-      return eir::api_cuda_fail(e, "cudaMallocFromPoolAsync(workspace)");
-    }
-    p->ws_device = dev;
-    p->ws_stream = st;
-  } else if (!captured && st != p->ws_stream) {
-    e = cudaStreamWaitEvent(st, p->ws_used, 0);
-    if (e != cudaSuccess) return eir::api_cuda_fail(e, "cudaStreamWaitEvent(workspace)");
-  }
-  *ws = p->ws;
-  return EIR_SUCCESS;
-}
-
-// marks the end of the workspace's use, which other streams and the plan's destruction wait
-// for; rc: the launches' status, returned
-int workspace_used(eir_plan *p, cudaStream_t st, int rc) {
-  cudaStreamCaptureStatus cap = cudaStreamCaptureStatusNone;
-  cudaError_t e = cudaStreamIsCapturing(st, &cap);
-  if (e == cudaSuccess && cap == cudaStreamCaptureStatusNone) {
-    e = cudaEventRecord(p->ws_used, st);
-    p->ws_stream = st;
-  }
-  return rc != EIR_SUCCESS || e == cudaSuccess ? rc : eir::api_cuda_fail(e, "cudaEventRecord(workspace)");
 }
 
 // Tiling of an 8-bit contraction on the tensor cores. Pair tiles where one-CTA
@@ -289,7 +210,7 @@ int eir_norm_backward(eir_plan *p, void const *dy, void const *h, void const *we
   int64_t parts = 0;
   if (dweight != nullptr) {
     void *ws = nullptr;
-    rc = workspace(p, st, &ws);
+    rc = p->op_ws.take(p->ws_bytes, st, &ws);
     if (rc != EIR_SUCCESS) return rc;
     a.part = static_cast<float *>(ws);
   }
@@ -300,7 +221,7 @@ int eir_norm_backward(eir_plan *p, void const *dy, void const *h, void const *we
   if (dweight == nullptr) return rc;
   if (rc == EIR_SUCCESS)
     rc = launched(eir::launch_norm_dweight(n, a.part, parts, dweight, st), "norm weight gradient launch");
-  return workspace_used(p, st, rc);
+  return p->op_ws.used(st, rc);
 }
 
 // ---------------------------------------------------------------- quantize
@@ -413,7 +334,7 @@ int eir_contract_int8(eir_plan *p, void const *left, void const *right, float co
   eir::I8Pack packs[2] = {};
   if (copies) {
     void *ws = nullptr;
-    rc = workspace(p, st, &ws);
+    rc = p->op_ws.take(p->ws_bytes, st, &ws);
     if (rc != EIR_SUCCESS) return rc;
     for (int i = 0; i < 2; ++i) {
       I8Operand &o = ops[i];
@@ -434,7 +355,7 @@ int eir_contract_int8(eir_plan *p, void const *left, void const *right, float co
     ProfScope prof(p, st);
     rc = launched(eir::launch_i8_tc(p->i8_tc, map_c, map_t, p->i8, a, err, st), "8-bit contraction launch");
   }
-  return copies ? workspace_used(p, st, rc) : rc;
+  return copies ? p->op_ws.used(st, rc) : rc;
 }
 
 // ---------------------------------------------------------------- log probabilities

@@ -10,6 +10,7 @@
 #include "eir_params.h"
 #include "eir_cuda.h"
 #include "op_params.h"
+#include "op_workspace.h"
 
 struct eir_plan;
 
@@ -42,8 +43,6 @@ int api_set_error(int code, char const *msg);
 int api_cuda_fail(cudaError_t e, char const *where);
 int api_encode_map(MapSpec const &s, void const *ptr, CUtensorMap *m);
 void api_count_launch();
-// frees the plan's workspace (and waits for its use, where it is pool memory)
-void api_free_workspace(eir_plan *p);
 // the current device's SM count and error word (allocated on first use)
 int api_device(int *num_sms, uint32_t **err);
 
@@ -117,8 +116,6 @@ struct eir_plan {
   int64_t ws_bytes = 0;
   int64_t split_ws_offset = 0;  // split-K partial tiles: ws + this offset
   int ws_device = -1;
-  cudaEvent_t ws_used = nullptr;  // the workspace is pool memory, in use until this event
-  cudaStream_t ws_stream = nullptr;  // of its last use
 
   // ---- output gather (eir_contract_gather)
   bool out_dense = false;         // the output is one contiguous block of out_elems
@@ -148,6 +145,7 @@ struct eir_plan {
   eir::I8Params i8;
   eir::I8TcPlan i8_tc;
   eir::LogprobParams logprob;
+  eir::OpWorkspace op_ws;  // of ws_bytes
 
   // ---- main-kernel timing (eir_plan_profile)
   bool profile = false;

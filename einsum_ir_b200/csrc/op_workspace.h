@@ -1,0 +1,130 @@
+// Workspaces of the operators' plans (host only).
+//
+// The memory comes from a pool of the library's own per device, so that a plan made
+// for a new shape does not pay for cudaMalloc on its first call (0.5 ms and more; it
+// synchronises the device too). Up to 256 MiB stay with the pool when plans are
+// destroyed.
+#pragma once
+
+#include <cuda_runtime_api.h>
+#include <cstdint>
+#include <mutex>
+#include "eir_cuda.h"
+
+namespace eir {
+
+int api_set_error(int code, char const *msg);
+int api_cuda_fail(cudaError_t e, char const *where);
+
+inline int workspace_pool(int dev, cudaMemPool_t *pool) {
+  static std::mutex mu;
+  static cudaMemPool_t pools[64] = {};
+  if (dev < 0 || dev >= 64) return api_set_error(EIR_CUDA_ERROR, "device index out of range");
+  std::lock_guard<std::mutex> lk(mu);
+  if (pools[dev] == nullptr) {
+    cudaMemPoolProps props = {};
+    props.allocType = cudaMemAllocationTypePinned;
+    props.location.type = cudaMemLocationTypeDevice;
+    props.location.id = dev;
+    cudaMemPool_t made = nullptr;
+    cudaError_t e = cudaMemPoolCreate(&made, &props);
+    if (e != cudaSuccess) return api_cuda_fail(e, "cudaMemPoolCreate");
+    uint64_t keep = (uint64_t)256 << 20;
+    e = cudaMemPoolSetAttribute(made, cudaMemPoolAttrReleaseThreshold, &keep);
+    if (e != cudaSuccess) {
+      cudaMemPoolDestroy(made);
+      return api_cuda_fail(e, "cudaMemPoolSetAttribute");
+    }
+    pools[dev] = made;
+  }
+  *pool = pools[dev];
+  return EIR_SUCCESS;
+}
+
+// A plan's own workspace on the current device, allocated on first use in `st`'s order; on
+// another stream than the last use's it waits for that. A capture gets the workspace that is
+// there: memory allocated in it would be the graph's own, and an event from outside cannot
+// be waited for (the caller orders a graph's launches).
+class OpWorkspace {
+ public:
+  // take() before the launches that use the memory, used() behind them
+  int take(int64_t bytes, cudaStream_t st, void **ws) {
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) return api_cuda_fail(e, "cudaGetDevice");
+    cudaStreamCaptureStatus cap = cudaStreamCaptureStatusNone;
+    e = cudaStreamIsCapturing(st, &cap);
+    if (e != cudaSuccess) return api_cuda_fail(e, "cudaStreamIsCapturing");
+    const bool captured = cap != cudaStreamCaptureStatusNone;
+    unsigned long long id = 0;
+    if (!captured) {
+      e = cudaStreamGetId(st, &id);
+      if (e != cudaSuccess) return api_cuda_fail(e, "cudaStreamGetId");
+    }
+    if (ptr_ == nullptr || device_ != dev) {
+      if (captured)
+        return api_set_error(EIR_INVALID_ARGUMENT,
+                             "a plan with a workspace needs a call on the device before it is captured");
+      release();
+      cudaMemPool_t pool = nullptr;
+      int rc = workspace_pool(dev, &pool);
+      if (rc != EIR_SUCCESS) return rc;
+      e = cudaEventCreateWithFlags(&used_, cudaEventDisableTiming);
+      if (e != cudaSuccess) {
+        used_ = nullptr;
+        return api_cuda_fail(e, "cudaEventCreate(workspace)");
+      }
+      e = cudaMallocFromPoolAsync(&ptr_, (size_t)bytes, pool, st);
+      if (e != cudaSuccess) {
+        ptr_ = nullptr;
+        release();
+        return api_cuda_fail(e, "cudaMallocFromPoolAsync(workspace)");
+      }
+      device_ = dev;
+      // (another stream's call is ordered behind the allocation even if nothing uses the memory here)
+      e = cudaEventRecord(used_, st);
+      if (e != cudaSuccess) return api_cuda_fail(e, "cudaEventRecord(workspace)");
+      stream_ = id;
+    } else if (!captured && id != stream_) {
+      e = cudaStreamWaitEvent(st, used_, 0);
+      if (e != cudaSuccess) return api_cuda_fail(e, "cudaStreamWaitEvent(workspace)");
+    }
+    *ws = ptr_;
+    return EIR_SUCCESS;
+  }
+  // marks the end of the use, which other streams and release() wait for; rc: the launches' status, returned
+  int used(cudaStream_t st, int rc) {
+    cudaStreamCaptureStatus cap = cudaStreamCaptureStatusNone;
+    cudaError_t e = cudaStreamIsCapturing(st, &cap);
+    if (e == cudaSuccess && cap == cudaStreamCaptureStatusNone) {
+      unsigned long long id = 0;
+      e = cudaStreamGetId(st, &id);
+      if (e == cudaSuccess) e = cudaEventRecord(used_, st);
+      if (e == cudaSuccess) stream_ = id;
+    }
+    return rc != EIR_SUCCESS || e == cudaSuccess ? rc : api_cuda_fail(e, "cudaEventRecord(workspace)");
+  }
+  void release() {
+    if (ptr_ != nullptr) {
+      int cur = 0;
+      cudaGetDevice(&cur);
+      if (device_ != cur) cudaSetDevice(device_);
+      cudaEventSynchronize(used_);  // cudaFree of pool memory does not wait for its use
+      cudaFree(ptr_);
+      if (device_ != cur) cudaSetDevice(cur);
+    }
+    if (used_ != nullptr) cudaEventDestroy(used_);
+    ptr_ = nullptr;
+    used_ = nullptr;
+  }
+
+ private:
+  void *ptr_ = nullptr;
+  int device_ = -1;
+  cudaEvent_t used_ = nullptr;
+  // of the last use: a stream's number, since handles are used again and the per-thread default stream has one
+  // for all threads
+  unsigned long long stream_ = 0;
+};
+
+}  // namespace eir

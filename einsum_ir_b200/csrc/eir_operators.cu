@@ -1,6 +1,7 @@
 // C-ABI of the row operators and the 8-bit contraction (eir_operators.h):
 // argument checks, workspaces and launches.
 #include <algorithm>
+#include <mutex>
 #include <new>
 #include <string>
 #include "eir_operators.h"
@@ -208,8 +209,10 @@ int eir_norm_backward(eir_plan *p, void const *dy, void const *h, void const *we
   num_sms = std::min(num_sms, eir::kMaxSms);
   eir::NormGradPtrs a{dy, h, weight, dsum, rstd, dx, dweight, nullptr};
   int64_t parts = 0;
+  std::unique_lock<std::mutex> held;
   if (dweight != nullptr) {
     void *ws = nullptr;
+    held = p->op_ws.hold();
     rc = p->op_ws.take(p->ws_bytes, st, &ws);
     if (rc != EIR_SUCCESS) return rc;
     a.part = static_cast<float *>(ws);
@@ -332,8 +335,10 @@ int eir_contract_int8(eir_plan *p, void const *left, void const *right, float co
   const int64_t ld = packed_stride(p->i8.k);
   const bool copies = ops[0].copy || ops[1].copy;
   eir::I8Pack packs[2] = {};
+  std::unique_lock<std::mutex> held;
   if (copies) {
     void *ws = nullptr;
+    held = p->op_ws.hold();
     rc = p->op_ws.take(p->ws_bytes, st, &ws);
     if (rc != EIR_SUCCESS) return rc;
     for (int i = 0; i < 2; ++i) {

@@ -47,7 +47,9 @@ inline int workspace_pool(int dev, cudaMemPool_t *pool) {
 // be waited for (the caller orders a graph's launches).
 class OpWorkspace {
  public:
-  // take() before the launches that use the memory, used() behind them
+  // A host thread holds the workspace from take(), before the launches that use the memory, to used(), behind
+  // them: another one's call of the plan comes behind all of them
+  std::unique_lock<std::mutex> hold() { return std::unique_lock<std::mutex>(mu_); }
   int take(int64_t bytes, cudaStream_t st, void **ws) {
     int dev = 0;
     cudaError_t e = cudaGetDevice(&dev);
@@ -119,6 +121,7 @@ class OpWorkspace {
   }
 
  private:
+  std::mutex mu_;
   void *ptr_ = nullptr;
   int device_ = -1;
   cudaEvent_t used_ = nullptr;

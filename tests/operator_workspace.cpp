@@ -6,6 +6,7 @@
 #include <map>
 #include <set>
 #include <string>
+#include <thread>
 #include <vector>
 #include "op_workspace.h"
 
@@ -132,11 +133,54 @@ void captures() {
   w.release();
   take_log();
 }
+
+// two host threads with a stream each call one plan: no call's take() comes between another's take() and used()
+void host_threads() {
+  eir::OpWorkspace w;
+  cudaStream_t s[2] = {stream(16, 1), stream(32, 2)};
+  void *p = nullptr;
+  CHECK(w.take(64, s[0], &p) == 0 && w.used(s[0], 0) == 0);
+  take_log();
+  auto calls = [&](int i) {
+    for (int j = 0; j < 2000; ++j) {
+      auto held = w.hold();
+      void *q = nullptr;
+      CHECK(w.take(64, s[i], &q) == 0 && q == p);
+      g_log += "launch in " + name(s[i]) + "; ";
+      std::this_thread::yield();
+      CHECK(w.used(s[i], 0) == 0);
+    }
+  };
+  std::thread t0(calls, 0), t1(calls, 1);
+  t0.join();
+  t1.join();
+  // a launch, its record, and a wait before the next launch where that is on the other stream
+  std::string log = take_log(), last = "1";
+  for (size_t at = 0; at < log.size();) {
+    auto next = [&]() {
+      const size_t end = log.find("; ", at);
+      std::string word = log.substr(at, end - at);
+      at = end + 2;
+      return word;
+    };
+    std::string word = next(), now = word.substr(word.size() - 1);
+    if (now != last) {
+      CHECK(word == "wait in " + now);
+      word = next();
+    }
+    CHECK(word == "launch in " + now);
+    CHECK(next() == "record in " + now);
+    last = now;
+  }
+  w.release();
+  take_log();
+}
 }  // namespace
 
 int main() {
   order_over_streams();
   captures();
+  host_threads();
   std::printf("ok\n");
   return 0;
 }

@@ -96,3 +96,23 @@ def test_first_call_of_a_host_thread(cuda, make):
     in_threads([w for w, _ in works], 200)
     for _, right in works:
         assert right()
+
+
+def test_one_plan_in_several_host_threads(cuda):
+    """plans whose calls share a workspace: packed operands, and partial weight gradients"""
+    g = gen(6)
+    m, n, k, rows, cols = 300, 1000, 1023, 700, 1500
+    b, a = codes(g, n, k), [codes(g, m, k) for _ in range(3)]
+    y = [torch.empty((m, n), device="cuda") for _ in range(3)]
+    plan = op.Int8ContractPlan(m, n, k, dtype_out=cabi.FP32)
+    in_threads([lambda s, i=i: plan.contract(a[i], b, None, None, y[i], stream=s) for i in range(3)], 300)
+    for i in range(3):
+        assert torch.equal(y[i], contract64(a[i], b, None, None, None, 0).float())
+    norm = op.NormPlan(rows, cols, cabi.FP32)
+    h, rstd = torch.randn(rows, cols, generator=g, device="cuda"), torch.rand(rows, generator=g, device="cuda") + 0.5
+    dy = [torch.randn(rows, cols, generator=g, device="cuda") for _ in range(3)]
+    dx, dw, once = torch.empty(3, rows, cols, device="cuda"), torch.empty(3, cols, device="cuda"), torch.empty(3, cols, device="cuda")
+    for i in range(3):
+        norm.backward(dy[i], h, rstd, dx[i], dweight=once[i])
+    in_threads([lambda s, i=i: norm.backward(dy[i], h, rstd, dx[i], dweight=dw[i], stream=s) for i in range(3)], 300)
+    assert torch.equal(dw, once)

@@ -145,7 +145,7 @@ struct eir_plan {
   eir::I8Params i8;
   eir::I8TcPlan i8_tc;
   eir::LogprobParams logprob;
-  eir::OpWorkspace op_ws;  // of ws_bytes
+  eir::OpWorkspace op_ws;  // of ws_bytes a device
 
   // ---- main-kernel timing (eir_plan_profile)
   bool profile = false;

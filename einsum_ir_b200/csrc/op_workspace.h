@@ -9,6 +9,7 @@
 #include <cuda_runtime_api.h>
 #include <cstdint>
 #include <mutex>
+#include <new>
 #include "eir_cuda.h"
 
 namespace eir {
@@ -41,10 +42,11 @@ inline int workspace_pool(int dev, cudaMemPool_t *pool) {
   return EIR_SUCCESS;
 }
 
-// A plan's own workspace on the current device, allocated on first use in `st`'s order; on
-// another stream than the last use's it waits for that. A capture gets the workspace that is
-// there: memory allocated in it would be the graph's own, and an event from outside cannot
-// be waited for (the caller orders a graph's launches).
+// A plan's own workspaces, one a device that it has been called on, each allocated on first use in
+// `st`'s order and kept until release() (a graph captured on one device goes on using its memory
+// there whatever the plan does on another). On another stream than the last use's a call waits for that. A
+// capture gets the workspace that is there: memory allocated in it would be the graph's own, and an event from
+// outside cannot be waited for (the caller orders a graph's launches).
 class OpWorkspace {
  public:
   // A host thread holds the workspace from take(), before the launches that use the memory, to used(), behind
@@ -63,71 +65,94 @@ class OpWorkspace {
       e = cudaStreamGetId(st, &id);
       if (e != cudaSuccess) return api_cuda_fail(e, "cudaStreamGetId");
     }
-    if (ptr_ == nullptr || device_ != dev) {
+    Memory *m = on(dev);
+    if (m == nullptr) {
       if (captured)
         return api_set_error(EIR_INVALID_ARGUMENT,
                              "a plan with a workspace needs a call on the device before it is captured");
-      release();
-      cudaMemPool_t pool = nullptr;
-      int rc = workspace_pool(dev, &pool);
+      int rc = allocate(bytes, dev, st, &m);
       if (rc != EIR_SUCCESS) return rc;
-      e = cudaEventCreateWithFlags(&used_, cudaEventDisableTiming);
-      if (e != cudaSuccess) {
-        used_ = nullptr;
-        return api_cuda_fail(e, "cudaEventCreate(workspace)");
-      }
-      e = cudaMallocFromPoolAsync(&ptr_, (size_t)bytes, pool, st);
-      if (e != cudaSuccess) {
-        ptr_ = nullptr;
-        release();
-        return api_cuda_fail(e, "cudaMallocFromPoolAsync(workspace)");
-      }
-      device_ = dev;
-      // (another stream's call is ordered behind the allocation even if nothing uses the memory here)
-      e = cudaEventRecord(used_, st);
-      if (e != cudaSuccess) return api_cuda_fail(e, "cudaEventRecord(workspace)");
-      stream_ = id;
-    } else if (!captured && id != stream_) {
-      e = cudaStreamWaitEvent(st, used_, 0);
+      m->stream = id;
+    } else if (!captured && id != m->stream) {
+      e = cudaStreamWaitEvent(st, m->used, 0);
       if (e != cudaSuccess) return api_cuda_fail(e, "cudaStreamWaitEvent(workspace)");
     }
-    *ws = ptr_;
+    *ws = m->ptr;
     return EIR_SUCCESS;
   }
   // marks the end of the use, which other streams and release() wait for; rc: the launches' status, returned
   int used(cudaStream_t st, int rc) {
+    int dev = 0;
     cudaStreamCaptureStatus cap = cudaStreamCaptureStatusNone;
-    cudaError_t e = cudaStreamIsCapturing(st, &cap);
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e == cudaSuccess) e = cudaStreamIsCapturing(st, &cap);
     if (e == cudaSuccess && cap == cudaStreamCaptureStatusNone) {
+      Memory *m = on(dev);  // taken before
       unsigned long long id = 0;
       e = cudaStreamGetId(st, &id);
-      if (e == cudaSuccess) e = cudaEventRecord(used_, st);
-      if (e == cudaSuccess) stream_ = id;
+      if (e == cudaSuccess) e = cudaEventRecord(m->used, st);
+      if (e == cudaSuccess) m->stream = id;
     }
     return rc != EIR_SUCCESS || e == cudaSuccess ? rc : api_cuda_fail(e, "cudaEventRecord(workspace)");
   }
   void release() {
-    if (ptr_ != nullptr) {
-      int cur = 0;
-      cudaGetDevice(&cur);
-      if (device_ != cur) cudaSetDevice(device_);
-      cudaEventSynchronize(used_);  // cudaFree of pool memory does not wait for its use
-      cudaFree(ptr_);
-      if (device_ != cur) cudaSetDevice(cur);
+    int cur = 0;
+    if (first_ != nullptr) cudaGetDevice(&cur);
+    while (first_ != nullptr) {
+      Memory *m = first_;
+      first_ = m->next;
+      if (m->device != cur) cudaSetDevice(m->device);
+      cudaEventSynchronize(m->used);  // cudaFree of pool memory does not wait for its use
+      cudaFree(m->ptr);
+      cudaEventDestroy(m->used);
+      if (m->device != cur) cudaSetDevice(cur);
+      delete m;
     }
-    if (used_ != nullptr) cudaEventDestroy(used_);
-    ptr_ = nullptr;
-    used_ = nullptr;
   }
 
  private:
+  struct Memory {
+    void *ptr = nullptr;
+    int device = -1;
+    cudaEvent_t used = nullptr;
+    // of the last use: a stream's number, since handles are used again and the per-thread default stream has one
+    // for all threads
+    unsigned long long stream = 0;
+    Memory *next = nullptr;
+  };
+  Memory *on(int dev) const {
+    Memory *m = first_;
+    while (m != nullptr && m->device != dev) m = m->next;
+    return m;
+  }
+  int allocate(int64_t bytes, int dev, cudaStream_t st, Memory **made) {
+    cudaMemPool_t pool = nullptr;
+    int rc = workspace_pool(dev, &pool);
+    if (rc != EIR_SUCCESS) return rc;
+    Memory *m = new (std::nothrow) Memory;
+    if (m == nullptr) return api_set_error(EIR_UNDEFINED_ERROR, "out of host memory");
+    m->device = dev;
+    char const *where = "cudaEventCreate(workspace)";
+    cudaError_t e = cudaEventCreateWithFlags(&m->used, cudaEventDisableTiming);
+    if (e == cudaSuccess) {
+      where = "cudaMallocFromPoolAsync(workspace)";
+      e = cudaMallocFromPoolAsync(&m->ptr, (size_t)bytes, pool, st);
+      if (e != cudaSuccess) cudaEventDestroy(m->used);
+    }
+    if (e != cudaSuccess) {
+      delete m;
+      return api_cuda_fail(e, where);
+    }
+    m->next = first_;
+    first_ = m;
+    *made = m;
+    // (another stream's call is ordered behind the allocation even if nothing uses the memory here)
+    e = cudaEventRecord(m->used, st);
+    return e == cudaSuccess ? EIR_SUCCESS : api_cuda_fail(e, "cudaEventRecord(workspace)");
+  }
+
   std::mutex mu_;
-  void *ptr_ = nullptr;
-  int device_ = -1;
-  cudaEvent_t used_ = nullptr;
-  // of the last use: a stream's number, since handles are used again and the per-thread default stream has one
-  // for all threads
-  unsigned long long stream_ = 0;
+  Memory *first_ = nullptr;
 };
 
 }  // namespace eir

@@ -13,10 +13,12 @@
  * plans that are destroyed with eir_plan_destroy, device pointers owned by the
  * caller, calls asynchronous on `stream` (NULL = the legacy default stream).
  * A plan with a workspace (eir_plan_workspace_bytes() > 0) takes its memory on the first
- * call on a device that needs it; such a call is refused in a stream capture
- * (EIR_INVALID_ARGUMENT). On another stream the next call waits for the last one's use
- * of it; a captured call does not, so graphs that hold one plan's calls run one
- * after another, and end before the plan is destroyed.
+ * call on a device that needs it, and keeps it until it is destroyed; such a call is
+ * refused in a stream capture (EIR_INVALID_ARGUMENT). Calls that need it may come from
+ * several streams and host threads: the next one waits for the last one's use. A
+ * captured call cannot: the caller orders the replays of graphs that hold a plan's calls
+ * against one another and against the plan's other calls, and they end before the plan
+ * is destroyed.
  *
  * Matrices are row-major with unit column stride; a row stride is in elements.
  * An input's row stride may be any value >= 0 (0: every row is the same

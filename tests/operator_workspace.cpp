@@ -134,6 +134,32 @@ void captures() {
   take_log();
 }
 
+// each device has memory of its own, which stays where a graph may use it until the plan is destroyed
+void devices() {
+  eir::OpWorkspace w;
+  cudaStream_t a = stream(16, 1), b = stream(32, 2);
+  void *p = nullptr, *q = nullptr;
+  CHECK(w.take(64, a, &p) == 0 && w.used(a, 0) == 0);
+  CHECK_LOG("alloc on 0 in 1; record in 1; record in 1; ");
+  g_device = 1;
+  g_capturing.insert(b);
+  CHECK(w.take(64, b, &q) == EIR_INVALID_ARGUMENT);
+  g_capturing.erase(b);
+  CHECK_LOG("");
+  CHECK(w.take(64, b, &q) == 0 && q != p && w.used(b, 0) == 0);
+  CHECK_LOG("alloc on 1 in 2; record in 2; record in 2; ");
+  CHECK(g_live.count(p) == 1);
+  g_device = 0;
+  g_capturing.insert(a);
+  CHECK(w.take(64, a, &q) == 0 && q == p);
+  g_capturing.erase(a);
+  CHECK(w.take(64, b, &q) == 0 && q == p);
+  CHECK_LOG("wait in 2; ");
+  w.release();
+  CHECK_LOG("host waits; free on 1; host waits; free on 0; ");
+  CHECK(g_device == 0 && g_live.empty() && g_events == 0);
+}
+
 // two host threads with a stream each call one plan: no call's take() comes between another's take() and used()
 void host_threads() {
   eir::OpWorkspace w;
@@ -180,6 +206,7 @@ void host_threads() {
 int main() {
   order_over_streams();
   captures();
+  devices();
   host_threads();
   std::printf("ok\n");
   return 0;

@@ -40,7 +40,7 @@ EXPORTS = [
     "eir_top_create", "eir_top_destroy", "eir_top_setup", "eir_top_execute", "eir_top_plan",
     "eir_top_default_optimization_config", "eir_top_optimize",
     # include/eir_operators.h
-    "eir_norm_plan_create", "eir_norm", "eir_norm_backward", "eir_quantize_plan_create",
+    "eir_norm_plan_create", "eir_norm", "eir_norm_backward", "eir_norm_backward_strided", "eir_quantize_plan_create",
     "eir_quantize", "eir_contract_int8_plan_create", "eir_contract_int8", "eir_logprob_plan_create",
     "eir_logprob", "eir_logprob_backward",
 ]
@@ -151,6 +151,7 @@ def lib() -> ctypes.CDLL:
         L.eir_norm_plan_create.argtypes = [POINTER(EirNormDesc), POINTER(c_void_p)]
         L.eir_norm.argtypes = [c_void_p] * 9
         L.eir_norm_backward.argtypes = [c_void_p] * 9
+        L.eir_norm_backward_strided.argtypes = [c_void_p] * 3 + [c_int64] + [c_void_p] * 6
         L.eir_quantize_plan_create.argtypes = [POINTER(EirQuantizeDesc), POINTER(c_void_p)]
         L.eir_quantize.argtypes = [c_void_p] * 5
         L.eir_contract_int8_plan_create.argtypes = [POINTER(EirContractInt8Desc), POINTER(c_void_p)]

@@ -188,7 +188,15 @@ int eir_norm(eir_plan *p, void const *x, void const *residual, void const *weigh
 int eir_norm_backward(eir_plan *p, void const *dy, void const *h, void const *weight, float const *rstd,
                       void const *dsum, void *dx, float *dweight, void *stream) {
   if (p == nullptr || p->what != kWhatNorm) return bad_argument("not a norm plan");
-  eir::NormParams const &n = p->norm;
+  return eir_norm_backward_strided(p, dy, h, p->norm.s_h, weight, rstd, dsum, dx, dweight, stream);
+}
+
+int eir_norm_backward_strided(eir_plan *p, void const *dy, void const *h, int64_t stride_h, void const *weight,
+                              float const *rstd, void const *dsum, void *dx, float *dweight, void *stream) {
+  if (p == nullptr || p->what != kWhatNorm) return bad_argument("not a norm plan");
+  if (!stride_in_ok(stride_h)) return bad_argument("norm backward: the row stride of h must be >= 0");
+  eir::NormParams n = p->norm;
+  n.s_h = stride_h;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   if (!aligned(dweight, 4)) return bad_argument("norm backward: a pointer is not aligned to its element");
   if (p->empty) {  // a sum over no rows

@@ -18,6 +18,7 @@ from . import cabi
 from .cabi import BF16, FP32, INT8, check
 
 ACT_NONE, ACT_RELU, ACT_GATED_SILU = 0, 1, 2
+INVALID_ARGUMENT = 52  # a status code (eir_cuda.h)
 
 __all__ = ["ACT_NONE", "ACT_RELU", "ACT_GATED_SILU", "FP32", "BF16", "INT8", "NormPlan", "QuantizePlan",
            "Int8ContractPlan", "LogprobPlan"]
@@ -50,7 +51,7 @@ class NormPlan(_OpPlan):
     """h = x + residual; y = h * rstd * weight with rstd = (mean(h^2) + eps)^(-1/2)
     over rows of ``cols`` elements. ``dtype``: x, residual, sum and h;
     ``dtype_out``: y, FP32, BF16 or INT8 (default: dtype); ``dtype_grad``: dy, dsum and
-    dx (default: dtype)."""
+    dx (default: dtype). ``stride_h``: of the backward pass's h (default: see backward)."""
 
     def __init__(self, rows, cols, dtype, dtype_weight=None, dtype_out=None, dtype_grad=None, eps=1e-6,
                  stride_x=None, stride_residual=None, stride_sum=None, stride_out=None, stride_h=None,
@@ -63,7 +64,10 @@ class NormPlan(_OpPlan):
             sx if stride_h is None else stride_h, _packed(stride_dy, cols), _packed(stride_dsum, cols),
             _packed(stride_dx, cols)))
         self._norm = cabi.lib().eir_norm
-        self._backward = cabi.lib().eir_norm_backward
+        self._backward = cabi.lib().eir_norm_backward_strided
+        self._rows, self._cols, self._esize = rows, cols, 4 if dtype == FP32 else 2
+        self._stride_h = stride_h
+        self._stride_x, self._stride_sum = sx, _packed(stride_sum, cols)
 
     def norm(self, x, out, weight=None, residual=None, sum=None, scale=None, rstd=None, stream: int = 0) -> None:
         """out = y, or with INT8 output its integers (``scale``: FP32 [rows]);
@@ -82,10 +86,31 @@ class NormPlan(_OpPlan):
     def backward(self, dy, h, rstd, dx, weight=None, dsum=None, dweight=None, stream: int = 0) -> None:
         """dx: the gradient of x and of residual from dy and dsum (the
         gradient that reaches h past the norm); dweight: FP32 [cols]. ``h``
-        is the forward call's sum, or its x where it had no residual; its rows
-        are ``stride_h`` apart (default: stride_x)."""
-        check(self._backward(self._h, _ptr(dy), _ptr(h), _ptr(weight), _ptr(rstd), _ptr(dsum), _ptr(dx),
-                             _ptr(dweight), stream))
+        is the forward call's sum, or its x where it had no residual. Its rows
+        are the plan's ``stride_h`` apart; where that was not given, a tensor
+        [..., cols] says itself whether they lie like x's or the sum's, and an
+        address stands for rows ``stride_x`` apart."""
+        check(self._backward(self._h, _ptr(dy), _ptr(h), self._row_stride_h(h), _ptr(weight), _ptr(rstd),
+                             _ptr(dsum), _ptr(dx), _ptr(dweight), stream))
+
+    def _row_stride_h(self, h):
+        x, sum = self._stride_x, self._stride_sum
+        if self._stride_h is not None:
+            return self._stride_h
+        if x == sum or self._rows < 2 or not hasattr(h, "element_size"):
+            return x
+        if h.dim() > 1 and h.shape[-1] == self._cols and h.numel() == self._rows * self._cols:
+            try:
+                stride = h.view(self._rows, self._cols).stride(0)
+            except RuntimeError:  # rows that are not one distance apart
+                stride = -1
+            if stride in (x, sum):
+                return stride
+            raise cabi.EirError(INVALID_ARGUMENT, f"norm backward: the rows of h are not stride_x ({x}) or stride_sum "
+                                f"({sum}) apart: give stride_h")
+        # a buffer of another shape: x's rows, unless it ends before theirs
+        room = h.numel() * h.element_size() // self._esize - self._cols
+        return sum if sum * (self._rows - 1) <= room < x * (self._rows - 1) else x
 
 
 class QuantizePlan(_OpPlan):

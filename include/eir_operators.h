@@ -70,6 +70,11 @@ int eir_norm(eir_plan *plan, void const *x, void const *residual, void const *we
  * NULL; dx may be dy or dsum itself (same pointer and stride). */
 int eir_norm_backward(eir_plan *plan, void const *dy, void const *h, void const *weight,
                       float const *rstd, void const *dsum, void *dx, float *dweight, void *stream);
+/* the same with h's row stride given by the call (>= 0), not the plan: for a plan
+ * whose backward pass reads x in one place and a sum with other rows in another */
+int eir_norm_backward_strided(eir_plan *plan, void const *dy, void const *h, int64_t stride_h,
+                              void const *weight, float const *rstd, void const *dsum, void *dx,
+                              float *dweight, void *stream);
 
 /* --- rows to 8-bit integers ---------------------------------------------------
  * m = max|x| of a row, q = round-to-even(x * (127 / m)), s = m / 127, with

@@ -116,6 +116,10 @@ int i8_map(I8Operand const &o, int64_t k, int box_rows, bool halves, CUtensorMap
   return eir::api_encode_map(m, o.ptr, map);
 }
 
+// One token: the row kernel, but for large layers that TMA can stream in place (4096 x 4096: 4.4 us against
+// 6.0; 8192 x 28672: 40.6 against 37.9). It reads operands of any alignment, so that one token copies none
+bool i8_large_row(eir::I8Params const &p) { return p.n * p.k >= ((int64_t)1 << 26); }
+
 int launched(cudaError_t e, char const *where) {
   if (e != cudaSuccess) return eir::api_cuda_fail(e, where);
   eir::api_count_launch();
@@ -301,15 +305,18 @@ int eir_contract_int8_plan_create(eir_contract_int8_desc const *d, eir_plan **ou
     q.s_r = d->stride_right;
     q.s_out = d->stride_out;
     p->empty = d->m == 0 || n_out == 0;
-    if (d->k > 0 && !p->empty) {
+    const bool row = d->m == 1 && !i8_large_row(q), products = d->k > 0 && !p->empty;
+    if (products && !row) {
       p->family = EIR_FAMILY_TC;
       p->i8_tc = i8_tiling(q);
       // copies of operands that TMA cannot read in place
-      p->ws_bytes = (d->m + d->n) * packed_stride(d->k);
+      if (d->m > 1) p->ws_bytes = (d->m + d->n) * packed_stride(d->k);
     }
-    p->text = std::string("int8 ") + (p->family != EIR_FAMILY_TC ? "simt" : p->i8_tc.tokens == 0 ? "pair" : "split") +
-              " tokens=" + std::to_string(p->i8_tc.tokens) + " split=" + std::to_string(p->i8_tc.split) +
-              " m=" + std::to_string(d->m) + " n=" + std::to_string(d->n) + " k=" + std::to_string(d->k);
+    p->text = std::string("int8 ") + (!products ? "simt" : row ? "row" : p->i8_tc.tokens == 0 ? "pair" : "split");
+    if (p->family == EIR_FAMILY_TC)
+      p->text += " tokens=" + std::to_string(p->i8_tc.tokens) + " split=" + std::to_string(p->i8_tc.split);
+    p->text += " m=" + std::to_string(d->m) + " n=" + std::to_string(d->n) + " k=" + std::to_string(d->k);
+    if (d->m == 1 && p->family == EIR_FAMILY_TC) p->text += " (row where operands are off the 16-byte grid)";
   });
 }
 
@@ -333,10 +340,8 @@ int eir_contract_int8(eir_plan *p, void const *left, void const *right, float co
     ProfScope prof(p, st);
     return launched(eir::launch_i8_bias(p->i8, a, num_sms, st), "8-bit contraction launch");
   }
-  // one token: the row kernel, but for large layers that TMA can stream in
-  // place (4096 x 4096: 4.4 us against 6.0; 8192 x 28672: 40.6 against 37.9)
   I8Operand ops[2] = {i8_operand(left, p->i8.m, p->i8.k, p->i8.s_l), i8_operand(right, p->i8.n, p->i8.k, p->i8.s_r)};
-  if (p->i8.m == 1 && (ops[0].copy || ops[1].copy || p->i8.n * p->i8.k < ((int64_t)1 << 26))) {
+  if (p->i8.m == 1 && (ops[0].copy || ops[1].copy || !i8_large_row(p->i8))) {
     ProfScope prof(p, st);
     return launched(eir::launch_i8_row(p->i8, a, num_sms, st), "8-bit contraction launch");
   }

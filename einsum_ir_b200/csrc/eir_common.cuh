@@ -128,6 +128,11 @@ __device__ __forceinline__ bool mbar_wait_bounded(uint64_t *bar, uint32_t parity
   }
 }
 
+// After a wait that gave up: copies issued before it land while the block's shared memory is still its own
+__device__ __forceinline__ void wait_for_copies() {
+  for (int i = 0; i < 1000; ++i) __nanosleep(1000);
+}
+
 // Bounded wait for a whole warp that is not on the latency-critical path (the
 // epilogue waiting for an accumulator, the TF32 splitter waiting for a stage):
 // only lane 0 polls the barrier, with a short sleep between polls, while the

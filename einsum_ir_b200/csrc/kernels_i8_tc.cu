@@ -393,9 +393,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(I8Pair::kThreads, 1)
 
   // After an abort, copies or commits issued before it may still be landing in
   // this CTA's shared memory: give them time before the CTA can exit.
-  if (threadIdx.x == 0 && *abort_flag) {
-    for (int i = 0; i < 1000; ++i) __nanosleep(1000);
-  }
+  if (threadIdx.x == 0 && *abort_flag) wait_for_copies();
   __syncwarp();
   tc_fence_before();
   cluster_sync();  // both CTAs done: no remote arrive or TMEM read is outstanding
@@ -568,8 +566,9 @@ __global__ void __launch_bounds__(192, 2)
     *abort_flag = 1;
   }
   __syncwarp();
-  if (*abort_flag) {
-    for (int i = 0; i < 1000; ++i) __nanosleep(1000);  // copies issued before the abort land first
+  // (one answer for the warp, whatever another one writes meanwhile: the reads of TMEM below take all lanes)
+  if (__any_sync(0xffffffffu, *abort_flag != 0)) {
+    wait_for_copies();
     ok = false;
   }
   __syncwarp();

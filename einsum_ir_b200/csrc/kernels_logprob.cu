@@ -400,6 +400,7 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS)
       }
     }
   };
+  bool landed = true;  // every copy that was waited for
   for (int k = warp; k < chunks; k += warps) {
     const int q = p0 + k * kChunk + lane;
     Piece c[AT_ONCE];
@@ -407,6 +408,7 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS)
       if (!mbar_wait_bounded(&sh.full[warp][stage], (phases >> stage) & 1u, &sh.abort)) {
         if (!sh.abort) record_error(err, kErrTimeoutProducer);
         sh.abort = 1;
+        landed = false;
       }
       phases ^= 1u << stage;
 #pragma unroll
@@ -414,7 +416,8 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS)
       // (without the fence a read that is still queued can meet the next copy's bytes)
       fence_proxy_async_smem();
       __syncwarp();
-      if (lane == 0 && inner(k + kLogStages * warps)) copy(k + kLogStages * warps, stage);
+      // (no copy follows one that did not land)
+      if (lane == 0 && landed && inner(k + kLogStages * warps)) copy(k + kLogStages * warps, stage);
       stage = stage + 1 == kLogStages ? 0 : stage + 1;
     } else {
 #pragma unroll
@@ -422,6 +425,7 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS)
     }
     add_pieces(c, q);
   }
+  if (!landed) wait_for_copies();
   const float own = v.m;
   v = log_moved(R, S2.x + S2.y, U2.x + U2.y, own);
   // ---- the block's sums, and the threads' largest logits

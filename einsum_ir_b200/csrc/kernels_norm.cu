@@ -147,10 +147,11 @@ struct RowRing {
     int stage = 0;
     uint32_t phase = 0;
     for (int64_t row = blockIdx.x; row < rows; row += gridDim.x) {
-      if (!mbar_wait_bounded(&empty[stage], phase ^ 1u, stop)) {
+      // (a stage is freed by threads that gave up waiting for it, too: no copy follows one that did not land)
+      if (!mbar_wait_bounded(&empty[stage], phase ^ 1u, stop) || *stop) {
         if (!*stop) record_error(err, kErrTimeoutProducer);
         *stop = 1;
-        for (int i = 0; i < 1000; ++i) __nanosleep(1000);  // copies under way land before the block ends
+        wait_for_copies();
         return;
       }
       ring_copy(t, row, stages + stage * ring.stage_bytes, &full[stage]);
@@ -166,6 +167,7 @@ struct RowRing {
     if (mbar_wait_bounded(&full[stage], phase, stop)) return true;
     if (!*stop) record_error(err, kErrTimeoutEpilogue);
     *stop = 1;
+    wait_for_copies();
     return false;
   }
 };

@@ -77,22 +77,17 @@ class OpWorkspace {
       e = cudaStreamWaitEvent(st, m->used, 0);
       if (e != cudaSuccess) return api_cuda_fail(e, "cudaStreamWaitEvent(workspace)");
     }
+    taken_ = m;
+    id_ = id;
+    captured_ = captured;
     *ws = m->ptr;
     return EIR_SUCCESS;
   }
   // marks the end of the use, which other streams and release() wait for; rc: the launches' status, returned
   int used(cudaStream_t st, int rc) {
-    int dev = 0;
-    cudaStreamCaptureStatus cap = cudaStreamCaptureStatusNone;
-    cudaError_t e = cudaGetDevice(&dev);
-    if (e == cudaSuccess) e = cudaStreamIsCapturing(st, &cap);
-    if (e == cudaSuccess && cap == cudaStreamCaptureStatusNone) {
-      Memory *m = on(dev);  // taken before
-      unsigned long long id = 0;
-      e = cudaStreamGetId(st, &id);
-      if (e == cudaSuccess) e = cudaEventRecord(m->used, st);
-      if (e == cudaSuccess) m->stream = id;
-    }
+    if (captured_) return rc;
+    cudaError_t e = cudaEventRecord(taken_->used, st);
+    if (e == cudaSuccess) taken_->stream = id_;
     return rc != EIR_SUCCESS || e == cudaSuccess ? rc : api_cuda_fail(e, "cudaEventRecord(workspace)");
   }
   void release() {
@@ -153,6 +148,10 @@ class OpWorkspace {
 
   std::mutex mu_;
   Memory *first_ = nullptr;
+  // what the last take() found, for used()
+  Memory *taken_ = nullptr;
+  unsigned long long id_ = 0;
+  bool captured_ = false;
 };
 
 }  // namespace eir

@@ -66,8 +66,9 @@ class NormPlan(_OpPlan):
         self._norm = cabi.lib().eir_norm
         self._backward = cabi.lib().eir_norm_backward_strided
         self._rows, self._cols, self._esize = rows, cols, 4 if dtype == FP32 else 2
-        self._stride_h = stride_h
         self._stride_x, self._stride_sum = sx, _packed(stride_sum, cols)
+        # h's row stride; None: asked of h itself
+        self._stride_h = stride_h if stride_h is not None else sx if sx == self._stride_sum or rows < 2 else None
 
     def norm(self, x, out, weight=None, residual=None, sum=None, scale=None, rstd=None, stream: int = 0) -> None:
         """out = y, or with INT8 output its integers (``scale``: FP32 [rows]);
@@ -90,14 +91,13 @@ class NormPlan(_OpPlan):
         are the plan's ``stride_h`` apart; where that was not given, a tensor
         [..., cols] says itself whether they lie like x's or the sum's, and an
         address stands for rows ``stride_x`` apart."""
-        check(self._backward(self._h, _ptr(dy), _ptr(h), self._row_stride_h(h), _ptr(weight), _ptr(rstd),
-                             _ptr(dsum), _ptr(dx), _ptr(dweight), stream))
+        stride_h = self._stride_h if self._stride_h is not None else self._row_stride_h(h)
+        check(self._backward(self._h, _ptr(dy), _ptr(h), stride_h, _ptr(weight), _ptr(rstd), _ptr(dsum), _ptr(dx),
+                             _ptr(dweight), stream))
 
     def _row_stride_h(self, h):
         x, sum = self._stride_x, self._stride_sum
-        if self._stride_h is not None:
-            return self._stride_h
-        if x == sum or self._rows < 2 or not hasattr(h, "element_size"):
+        if not hasattr(h, "element_size"):
             return x
         if h.dim() > 1 and h.shape[-1] == self._cols and h.numel() == self._rows * self._cols:
             try:

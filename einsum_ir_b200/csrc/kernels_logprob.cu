@@ -1,17 +1,18 @@
 // Log probabilities of given tokens, log-sum-exp, entropy and top alternatives
 // of rows of logits, and the gradient of the first and third.
 //
-// One pass over a row, in base 2 (L = log2 e): with a reference R near the row's
-// maximum times L, S = sum 2^d and U = sum d 2^d for d = x L - R give
-// lse = (R + log2 S) / L, log p = (d - log2 S) / L and entropy = (log2 S - U / S) / L. Any R near m L will
-// do, so that R may be rounded: by 2^-4 at most for |m| <= 2^20, and rows whose maximum is larger or
-// lower than that are redone (from 1.5e9 on the rounding alone could take 2^d out of FP32's range). A
-// thread raises its own R when it meets a larger logit and its sums shrink by 2^(R - R'). Logits are
-// floored at -2^21, where 2^d is 0 for every such m, so that a ruled-out one (-infinity, or a large finite
-// value) adds 0 d = 0 to U.
+// One pass over a row, in base 2 (L = log2 e): with the row's maximum m, S = sum 2^d and U = sum d 2^d
+// for d = (x - m) L give lse = m + log2 S / L, log p = x - m - log2 S / L and entropy = (log2 S - U / S) / L.
+// The pass itself takes d = x L - R, one instruction, with a reference R near m L: any will do, so that R may be
+// rounded, and a thread that meets a larger logit raises its own and shrinks its sums by 2^(R - R'). Its sums
+// move to its exact maximum at the end. Logits are floored at -2^21, where 2^d is 0 for every m of
+// at least -2^20, so that a ruled-out one (-infinity, or a large finite value) adds 0 d = 0 to U. R is off by 2^-4 at
+// most for |m| <= 2^20 (from 1.5e9 on its rounding could take 2^d out of FP32's range): the sums of rows
+// whose maximum lies beyond are taken once more, as differences to it.
 //
-// At BF16 bound by the SM's pipes (4096 x 32768: 53 us, 5.1 TB/s; exponentials 63 % of their
-// rate, issue 62 %), at FP32 by HBM (4096 x 32768, 5 alternatives: 105 us, 5.1 TB/s). A logit is read once. A piece is 16 bytes of memory on
+// At BF16 no unit is full (4096 x 32768 without alternatives: 53 us, 5.1 TB/s; issue 62 %, exponentials 56 % of
+// their rate, HBM 65 % of its peak; with 5 alternatives 61 us, 58, 47 and 55 %: the steps at a row's end keep most of
+// a block's warps waiting). FP32 is bound by HBM (4096 x 32768, 5 alternatives: 105 us, 5.1 TB/s). A logit is read once. A piece is 16 bytes of memory on
 // the 16-byte grid, so rows of any alignment stream alike; the elements of
 // the first and last piece that lie outside the row count as ruled out.
 //
@@ -28,8 +29,8 @@
 // Rows that do not fill the GPU by number are split over a cluster of up to 8 blocks, joined
 // through distributed shared memory.
 //
-// Rows with a NaN or +infinity, with a maximum above 2^20 or below -2^20 (but -infinity), or with more
-// candidates than their buffer holds are redone by logprob_plain_row: a pass for each value.
+// Rows with a NaN or +infinity, or with more candidates than their buffer holds, are redone by
+// logprob_plain_row: a pass for each value.
 //
 // Backward: dx = dlogprob (onehot - p) - dentropy p (x - lse + H), bound by HBM (2048 x 50021 BF16 with
 // entropy 73 us, 5.6 TB/s).
@@ -73,31 +74,34 @@ __device__ __forceinline__ uint64_t warp_max_key(uint64_t k) {
 
 __device__ __forceinline__ float logit_nan() { return __uint_as_float(0x7fc00000u); }
 
-// A row's sums against the reference R = m L (0 below kLowest, where S = 0)
+// a thread's reference (0 below kLowest, where S = 0)
+__device__ __forceinline__ float log_ref(float m) { return m < kLowest ? 0.f : m * kLog2e; }
+// A row's maximum, and its sums as differences to it
 struct LogSums {
   float m, S, U;
 };
-__device__ __forceinline__ float log_ref(float m) { return m < kLowest ? 0.f : m * kLog2e; }
-// log p of a logit: its distance from the maximum, whose own d is the rounding of R
-__device__ __forceinline__ float log_prob(float x, LogSums const &v, float log_s) {
-  return (x - v.m) + (fmaf(v.m, kLog2e, -log_ref(v.m)) - log_s) * kLn2;
-}
-// whether a row's sums do not hold (S is NaN where the row has a NaN or +infinity)
-__device__ __forceinline__ bool log_odd(LogSums const &v) {
-  return !(v.S == v.S) || v.m > kLargest || (v.m < -kLargest && v.m != -INFINITY);
-}
-// sums against R moved to the reference of the maximum m (sums of 0 may stand beside any reference)
-__device__ __forceinline__ LogSums log_moved(float R, float S, float U, float m) {
-  const float d = R - log_ref(m), e = exp2_fast(d);
-  if (S == 0.f) return LogSums{m, 0.f, 0.f};
+__device__ __forceinline__ float log_prob(float x, LogSums const &v, float log_s) { return (x - v.m) - log_s * kLn2; }
+// whether the pass's sums do not hold for a row with this maximum (+infinity: no sums do)
+__device__ __forceinline__ bool log_again(float m) { return fabsf(m) > kLargest && fabsf(m) < INFINITY; }
+// sums with distances from d on instead of 0 (a NaN stays in them)
+__device__ __forceinline__ LogSums log_shifted(float m, float S, float U, float d) {
+  const float e = exp2_fast(d);
   return LogSums{m, e * S, e * (U + d * S)};
+}
+// a thread's sums against R as those of its maximum m (sums of 0 may stand beside any R)
+__device__ __forceinline__ LogSums log_of_pass(float R, float S, float U, float m) {
+  return S == 0.f ? LogSums{m, 0.f, 0.f} : log_shifted(m, S, U, -fmaf(m, kLog2e, -R));
+}
+// sums moved to the larger maximum m (2^-300 is 0; -infinity less itself counts as that too)
+__device__ __forceinline__ LogSums log_moved(LogSums const &v, float m) {
+  return log_shifted(m, v.S, v.U, fmaxf((v.m - m) * kLog2e, -300.f));
 }
 // the sums of the warp's lanes
 __device__ __forceinline__ LogSums log_join_lanes(LogSums v) {
   // (signed integers in the order of the floats; a NaN is no maximum here, but stays in S)
   const int b = __float_as_int(v.m == v.m ? v.m : -INFINITY);
   const int most = __reduce_max_sync(0xffffffffu, b ^ ((b >> 31) & 0x7fffffff));
-  v = log_moved(log_ref(v.m), v.S, v.U, __int_as_float(most ^ ((most >> 31) & 0x7fffffff)));
+  v = log_moved(v, __int_as_float(most ^ ((most >> 31) & 0x7fffffff)));
   v.S = warp_sum(v.S);
   v.U = warp_sum(v.U);
   return v;
@@ -260,6 +264,68 @@ struct LogitRow {
   }
 };
 
+// The sums of pieces p0 .. p1 - 1 of a row whose maximum m is large, as differences to it (all threads of the
+// block; each gets them): 4096 x 32768 BF16 with 5 alternatives takes 62.3 us where 1 in 100 rows holds nothing but
+// -1e30, 112 where all do, 62.0 where none does. red: 2 x 32 words
+template <typename T>
+__device__ __noinline__ LogSums log_large_row(LogitRow<T> const x, int p0, int p1, float m, float *red) {
+  constexpr int V = LogitRow<T>::V, AT_ONCE = 4;
+  const int warps = blockDim.x >> 5, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  float2 S = make_float2(0.f, 0.f), U = make_float2(0.f, 0.f);
+  for (int q = p0 + (int)threadIdx.x; q < p1; q += AT_ONCE * (int)blockDim.x) {
+    typename LogitRow<T>::Piece c[AT_ONCE];
+#pragma unroll
+    for (int i = 0; i < AT_ONCE; ++i) {
+      const int at = q + i * (int)blockDim.x;
+      c[i] = at < p1 ? x.load(at) : LogitRow<T>::none();
+    }
+#pragma unroll
+    for (int i = 0; i < AT_ONCE; ++i)
+#pragma unroll
+      for (int e = 0; e < V; e += 2) {
+        float2 d = mul2(add2(c[i].get2(e), make_float2(-m, -m)), make_float2(kLog2e, kLog2e));
+        d = make_float2(max_nan(d.x, -200.f), max_nan(d.y, -200.f));  // 2^-200 is 0
+        const float2 t = make_float2(exp2_fast(d.x), exp2_fast(d.y));
+        S = add2(S, t);
+        U = fma2(d, t, U);
+      }
+  }
+  LogSums v{m, warp_sum(S.x + S.y), warp_sum(U.x + U.y)};
+  __syncthreads();
+  if (lane == 0) {
+    red[warp] = v.S;
+    red[32 + warp] = v.U;
+  }
+  __syncthreads();
+  v.S = warp_sum(lane < warps ? red[lane] : 0.f);
+  v.U = warp_sum(lane < warps ? red[32 + lane] : 0.f);
+  return v;
+}
+
+// the sums of a cluster's blocks, each lane a block's
+__device__ __forceinline__ LogSums log_join_blocks(LogSums const *at, uint32_t blocks) {
+  LogSums w{-INFINITY, 0.f, 0.f};
+  if ((threadIdx.x & 31) < blocks) {
+    const uint32_t sums = mapa_shared(smem_u32(at), threadIdx.x & 31);
+    w = LogSums{__uint_as_float(ld_cluster_u32(sums)), __uint_as_float(ld_cluster_u32(sums + 4)),
+                __uint_as_float(ld_cluster_u32(sums + 8))};
+  }
+  return log_join_lanes(w);
+}
+// the same for a row in parts, by all blocks of the cluster
+template <typename T>
+__device__ __noinline__ LogSums log_large_blocks(LogitRow<T> const x, int p0, int p1, float m, float *red, LogSums *sums,
+                                                 uint32_t blocks) {
+  const LogSums part = log_large_row<T>(x, p0, p1, m, red);
+  if (threadIdx.x == 0) *sums = part;
+  __syncwarp();
+  cluster_sync();
+  const LogSums v = log_join_blocks(sums, blocks);
+  __syncwarp();
+  cluster_sync();  // no block ends while its sums are read
+  return v;
+}
+
 constexpr int kLogStages = 2;  // of a warp, 2 KB each
 
 __device__ __forceinline__ void bulk_copy(void *dst, void const *src, uint32_t bytes, uint64_t *bar) {
@@ -281,6 +347,7 @@ struct LogShared {
   int n_found, full_up;    // candidates; more than fit
   volatile int abort;      // a bounded wait has given up
   LogSums sums;            // of the block
+  float again;             // the row's maximum, where its sums are taken once more; 0: not so
   alignas(8) uint64_t full[THREADS / 32][kLogStages];
   alignas(128) uint8_t stages[THREADS / 32][kLogStages][2048];
 };
@@ -427,7 +494,7 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS)
   }
   if (!landed) wait_for_copies();
   const float own = v.m;
-  v = log_moved(R, S2.x + S2.y, U2.x + U2.y, own);
+  v = log_of_pass(R, S2.x + S2.y, U2.x + U2.y, own);
   // ---- the block's sums, and the threads' largest logits
   v = log_join_lanes(v);
   if (lane == 0) {
@@ -506,24 +573,24 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS)
       __syncwarp();
     }
   }
-  bool odd = full || log_odd(v);
-  if (blocks_a_row > 1) {
-    // (whether the sums hold shows in the whole row's: a part may well have nothing but masked logits)
-    if (threadIdx.x == 0) sh.full_up = full;
+  bool odd = full;
+  if (blocks_a_row == 1) {
+    if (log_again(v.m)) v = log_large_row<T>(x, 0, x.pieces, v.m, sh.red);
+  } else {
+    if (threadIdx.x == 0) {
+      sh.full_up = full;
+      sh.again = 0.f;
+    }
     __syncwarp();
     cluster_sync();  // every block's sums and alternatives are in its shared memory
     if (rank == 0) {
-      // all blocks' sums (each lane a block's), and the largest of all alternatives
-      LogSums w{-INFINITY, 0.f, 0.f};
-      int any = 0;
-      if (lane < (int)blocks_a_row) {
-        const uint32_t sums = mapa_shared(smem_u32(&sh.sums), lane);
-        w = LogSums{__uint_as_float(ld_cluster_u32(sums)), __uint_as_float(ld_cluster_u32(sums + 4)),
-                    __uint_as_float(ld_cluster_u32(sums + 8))};
-        any = (int)ld_cluster_u32(mapa_shared(smem_u32(&sh.full_up), lane));
-      }
-      v = log_join_lanes(w);
-      odd = log_odd(v) || __any_sync(0xffffffffu, any != 0);
+      // the largest of all alternatives
+      const int any = lane < (int)blocks_a_row ? (int)ld_cluster_u32(mapa_shared(smem_u32(&sh.full_up), lane)) : 0;
+      v = log_join_blocks(&sh.sums, blocks_a_row);
+      odd = __any_sync(0xffffffffu, any != 0);
+      // (whether the pass's sums hold shows in the whole row's: a part may well have nothing but masked logits)
+      if (warp == 0 && log_again(v.m) && lane < (int)blocks_a_row)
+        st_cluster_u32(mapa_shared(smem_u32(&sh.again), lane), __float_as_uint(v.m));
       if (p.top > 0 && !odd && warp == 0) {
         for (int i = lane; i < p.top * (int)blocks_a_row; i += 32) {
           const uint32_t key = mapa_shared(smem_u32(&sh.top[i % p.top]), i / p.top);
@@ -533,33 +600,30 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS)
         const uint64_t t = pick_largest(sh.found, p.top * (int)blocks_a_row, p.top);
         __syncwarp();
         sh.found[lane] = t;
-        __syncwarp();
       }
     }
-  }
-  if (rank == 0) {
-    if (odd) {
-      __syncthreads();
-      logprob_plain_row<T>(p, a, row, sh.red, sh.plain);
-    } else if (warp == 0) {
-      const bool none = v.S == 0.f;
-      const float ref = log_ref(v.m), log_s = log2f(v.S);
-      if (lane == 0) {
-        logprob_row_values(p, a, row, none, none ? -INFINITY : (ref + log_s) * kLn2, (log_s - v.U / v.S) * kLn2,
-                           target.place, log_prob(target.x, v, log_s));
-      }
-      if (lane < p.top) {
-        const uint64_t key = (blocks_a_row > 1 ? sh.found : sh.top)[lane];
-        const float xt = rank_value((uint32_t)(key >> 32));
-        if (a.top_index) a.top_index[row * p.top + lane] = ~(uint32_t)key;
-        if (a.top_logprob)
-          a.top_logprob[row * p.top + lane] = none ? -INFINITY : log_prob(xt, v, log_s);
-      }
-    }
-  }
-  if (blocks_a_row > 1) {
     __syncwarp();
-    cluster_sync();  // no block ends while its shared memory is read
+    cluster_sync();  // no block ends, or writes its sums again, while they are read
+    if (sh.again != 0.f) v = log_large_blocks<T>(x, p0, p1, sh.again, sh.red, &sh.sums, blocks_a_row);
+  }
+  if (rank != 0) return;
+  if (odd || !(v.S == v.S)) {  // (S is NaN where the row has a NaN or +infinity)
+    __syncthreads();
+    logprob_plain_row<T>(p, a, row, sh.red, sh.plain);
+  } else if (warp == 0) {
+    const bool none = v.S == 0.f;
+    const float log_s = log2f(v.S);
+    if (lane == 0) {
+      logprob_row_values(p, a, row, none, none ? -INFINITY : v.m + log_s * kLn2, (log_s - v.U / v.S) * kLn2,
+                         target.place, log_prob(target.x, v, log_s));
+    }
+    if (lane < p.top) {
+      const uint64_t key = (blocks_a_row > 1 ? sh.found : sh.top)[lane];
+      const float xt = rank_value((uint32_t)(key >> 32));
+      if (a.top_index) a.top_index[row * p.top + lane] = ~(uint32_t)key;
+      if (a.top_logprob)
+        a.top_logprob[row * p.top + lane] = none ? -INFINITY : log_prob(xt, v, log_s);
+    }
   }
 }
 

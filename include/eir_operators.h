@@ -41,7 +41,8 @@ enum { EIR_INT8 = 3 };
 /* --- root-mean-square norm with the residual's addition -------------------
  * h = x + residual; rstd = (mean(h^2) + eps)^(-1/2); y = h * rstd * weight.
  * Computed in FP32 from the inputs; h, y are rounded once when stored (y is
- * computed from the unrounded h). With dtype_out EIR_INT8 a row of y is
+ * computed from the unrounded h). The sum of squares is FP32's too: above about
+ * 1.8e19 an element's square is infinite, and rstd 0. With dtype_out EIR_INT8 a row of y is
  * stored as integers q and a scale s with y ~ q s: v = h * weight, m = max|v|,
  * q = round-to-even(v * (127 / m)), s = m * rstd / 127 (rstd cancels in q).
  * A row with m < 2^-100 gives q = 0, s = 0; a row with an infinity or NaN
@@ -115,8 +116,8 @@ int eir_contract_int8(eir_plan *plan, void const *left, void const *right, float
  * index. Logits of -infinity have probability 0 and add 0 to the entropy; a
  * row with nothing but -infinity gives lse = -infinity, logprob = -infinity
  * (top_logprob alike) and entropy 0; a NaN or +infinity makes the row's
- * values NaN. Finite logits may have any size (a row whose largest is beyond
- * 2^20 in magnitude takes a slower way), as masks too. A negative target is ignored (logprob 0); one >= vocab gives
+ * values NaN. Finite logits may have any size, as masks too (a row whose
+ * largest is beyond 2^20 in magnitude is read once more). A negative target is ignored (logprob 0); one >= vocab gives
  * NaN. */
 typedef struct {
   int64_t rows, vocab;        /* 1 <= vocab < 2^31 */

@@ -104,3 +104,21 @@ def test_mixed_masks(cuda, vocab, dtype):
     x[2, 4::5] = torch.finfo(dtype).min
     t = torch.tensor([1, 0, 5], device="cuda")
     check_shifted(x, t, 4, run_logprob(x, t, 4))
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("vocab", [300, 140000])
+def test_nan_and_infinity_beside_large_logits(cuda, vocab, dtype):
+    """a NaN or +infinity in a row of large values makes its results NaN, and leads the alternatives"""
+    x = torch.full((4, vocab), -1e30, device="cuda").to(dtype)
+    x[0, vocab // 2] = float("nan")
+    x[1, 7] = float("inf")
+    x[2] = 1e30
+    x[2, vocab - 1] = float("nan")
+    x[3, 3] = 5e5
+    t = torch.full((4,), 3, device="cuda")
+    o = run_logprob(x, t, 3)
+    for name in ("lse", "entropy", "logprob", "top_logprob"):
+        assert torch.isnan(o[name][:3]).all(), name
+    assert o["top_index"][:3, 0].tolist() == [vocab // 2, 7, vocab - 1]
+    check_shifted(x[3:], t[3:], 3, {k: v[3:] for k, v in o.items()})

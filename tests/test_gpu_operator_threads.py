@@ -27,11 +27,12 @@ def in_threads(works, times):
 
     streams = [torch.cuda.Stream() for _ in works]
     torch.cuda.synchronize()
-    threads = [threading.Thread(target=loop, args=(w, s)) for w, s in zip(works, streams)]
+    threads = [threading.Thread(target=loop, args=(w, s), daemon=True) for w, s in zip(works, streams)]
     for t in threads:
         t.start()
     for t in threads:
-        t.join()
+        t.join(120)
+    assert not any(t.is_alive() for t in threads), "a call did not return"
     torch.cuda.synchronize()
     cabi.check_device_errors()
     assert not failed, failed[0]

@@ -10,8 +10,8 @@
 // most for |m| <= 2^20 (from 1.5e9 on its rounding could take 2^d out of FP32's range): the sums of rows
 // whose maximum lies beyond are taken once more, as differences to it.
 //
-// At BF16 no unit is full (4096 x 32768 without alternatives: 53 us, 5.1 TB/s; issue 62 %, exponentials 56 % of
-// their rate, HBM 65 % of its peak; with 5 alternatives 61 us, 58, 47 and 55 %: the steps at a row's end keep most of
+// At BF16 no unit is full (4096 x 32768 without alternatives: 53 us, 5.1 TB/s; issue 63 %, exponentials 57 % of
+// their rate, HBM 65 % of its peak; with 5 alternatives 61 us, 59, 49 and 57 %: the steps at a row's end keep most of
 // a block's warps waiting). FP32 is bound by HBM (4096 x 32768, 5 alternatives: 105 us, 5.1 TB/s). A logit is read once. A piece is 16 bytes of memory on
 // the 16-byte grid, so rows of any alignment stream alike; the elements of
 // the first and last piece that lie outside the row count as ruled out.

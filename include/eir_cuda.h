@@ -8,8 +8,9 @@
  * stream are asynchronous on that stream (a `void*` holding a cudaStream_t;
  * NULL = the legacy default stream). Plans are immutable after creation and
  * may be used from several host threads on different streams, except where a
- * plan owns a workspace (eir_plan_workspace_bytes() > 0): such a plan must not
- * run on two streams at once.
+ * contraction's or permutation's plan owns a workspace
+ * (eir_plan_workspace_bytes() > 0): such a plan must not run on two streams at
+ * once. (The plans of eir_operators.h order the use of theirs by themselves.)
  *
  * Reference interfaces replaced (paths inside scalable-analyses/einsum_ir):
  *   eir_contract_plan_create  <- backend::BinaryContraction::init + compile
